@@ -462,6 +462,12 @@ extern "C" int b200sd_ffi_register(const void* xla_ffi_api, char* err, size_t er
     if (err && err_len) snprintf(err, err_len, "XLA_FFI_Api pointer is null");
     return 3;
   }
+#ifdef B200SD_FFI_STANDIN
+  if (api->struct_size != XLA_FFI_Api_STRUCT_SIZE || api->api_version.major_version != XLA_FFI_API_MAJOR) {
+    if (err && err_len) snprintf(err, err_len, "this library was built without XLA's FFI headers; rebuild it with XLA_ROOT=<xla checkout>");
+    return 9;
+  }
+#endif
   struct Target {
     const char* name;
     XLA_FFI_Handler_Bundle bundle;
