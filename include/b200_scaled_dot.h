@@ -30,11 +30,14 @@ extern "C" {
 enum {
   B200SD_S8 = 2,
   B200SD_S32 = 4,
+  B200SD_U8 = 6,
   B200SD_F16 = 10,
   B200SD_F32 = 11,
   B200SD_BF16 = 16,
   B200SD_F8E5M2 = 19,
   B200SD_F8E4M3FN = 20,
+  B200SD_S4 = 21,                /* weight types of the 4-bit dot; its buffers are bytes of two values */
+  B200SD_U4 = 22,
   B200SD_F8E8M0FNU = 33          /* the scale type of MX block-scaled operands */
 };
 
@@ -170,6 +173,94 @@ typedef struct B200SD_BlockScaledDotMx {
   int64_t b_scale_cols;
 } B200SD_BlockScaledDotMx;
 
+/* Arguments of one dot with 4-bit weights and a scale for each group of them along k, for few rows:
+ *
+ *   D[m,n] = sum_k x[m,k] * (w[n,k] - z[n,k/group]) * scale[n,k/group]  (+ bias[n])
+ *
+ * The weights are K-minor like the MX call's: byte [n, j] holds w[n, 2j] in its low and w[n, 2j+1] in
+ * its high four bits.  weight_type S4 is two's complement (-8 .. 7) and has no zero points; U4 (0 .. 15)
+ * takes one zero point per group from the low four bits of a byte.  The weights enter the products as
+ * the integers w - z, exactly; sums are f32, a group's sum is multiplied by its scale in f32, and D is
+ * rounded once.  group is 32, 64 or a multiple of 128 that divides k; n is free; m is at most 64.
+ * m == 0 does nothing. */
+typedef struct B200SD_DotW4 {
+  size_t struct_size;            /* sizeof(B200SD_DotW4) */
+  const void* x;                 /* [m, k] */
+  const void* w;                 /* [n, k/2] bytes */
+  const void* scale;             /* [n, k/group] */
+  const void* zero;              /* [n, k/group] bytes, weight_type U4 only */
+  const void* bias;              /* [n], epilogue BIAS only */
+  void* d;                       /* [m, n] */
+  int64_t m, n, k, group;
+  int32_t x_dtype;               /* BF16 or F16 */
+  int32_t weight_type;           /* B200SD_S4 or B200SD_U4 */
+  int32_t scale_dtype;           /* BF16, F16 or F32 */
+  int32_t bias_dtype;            /* BF16, F16 or F32 */
+  int32_t d_dtype;               /* x_dtype or F32 */
+  int32_t epilogue;              /* B200SD_EPILOGUE_DEFAULT or _BIAS */
+} B200SD_DotW4;
+
+/* A cache of keys and values in 8 bits: k_pages and v_pages are [num_pages, kv_heads, page_tokens,
+ * head_dim], a value is its code times the scale of its (page, head).  Position t of sequence b is slot
+ * t % page_tokens of page page_table[b, t / page_tokens].  seq_lens[b] counts the sequence's tokens
+ * INCLUDING the new ones of the call; new_lens[b] (NULL: new_tokens for all) of the new_tokens rows given
+ * for a sequence are in use, at positions seq_lens[b] - new_lens[b] onwards.  Entries of the table behind a
+ * sequence's last page are not read.  An entry or a length that points outside of the cache is skipped
+ * and reported as bit 64 of b200sd_device_status().
+ *
+ * Append: the new tokens' keys and values are stored.  The scale of a (page, head) is a power of two, the
+ * least at which the largest finite new magnitude fits the type (448, 57344 or 127), at least 2^-126, and
+ * at least the scale before when the page holds earlier tokens of the sequence; their codes are rounded
+ * to it again where it grew.  Roundings go to the nearest, ties to even; infinities become the largest
+ * value, NaN stays NaN (s8: 0).  Two sequences of one call must not append to the same page. */
+typedef struct B200SD_KvCacheAppend {
+  size_t struct_size;            /* sizeof(B200SD_KvCacheAppend) */
+  const void* k_new;             /* [batch, new_tokens, kv_heads, head_dim] */
+  const void* v_new;
+  void* k_pages;                 /* updated in place */
+  void* v_pages;
+  float* k_scale;                /* [num_pages, kv_heads], updated in place */
+  float* v_scale;
+  const int32_t* page_table;     /* [batch, table_width] */
+  const int32_t* seq_lens;       /* [batch] */
+  const int32_t* new_lens;       /* [batch] or NULL */
+  int64_t batch, new_tokens, kv_heads, head_dim;
+  int64_t num_pages, page_tokens, table_width;
+  int32_t new_dtype;             /* BF16 or F16 */
+  int32_t cache_dtype;           /* F8E4M3FN, F8E5M2 or S8 */
+} B200SD_KvCacheAppend;
+
+/* Attention of the last tokens of each sequence over such a cache:
+ *
+ *   out[b,i,h] = sum_t softmax_t( softmax_scale * q[b,i,h] . k[t, h / (heads / kv_heads)] ) * v[t, ...]
+ *
+ * over the positions t <= p = seq_lens[b] - new_lens[b] + i, and t > p - window when window > 0.  Rows
+ * that see nothing (i >= new_lens[b] among them) get zeros, and -inf as their logarithm of the sum.
+ * Scores, softmax sums and products are held in f32; a row's weights are rounded to 11 bits for the
+ * product with the values.  new_tokens is at most 64, head_dim a multiple of 16 up to 256, page_tokens
+ * 16, 32, 64 or 128, batch at most 4096. */
+typedef struct B200SD_PagedAttention {
+  size_t struct_size;            /* sizeof(B200SD_PagedAttention) */
+  const void* q;                 /* [batch, new_tokens, heads, head_dim] */
+  const void* k_pages;
+  const void* v_pages;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* new_lens;       /* or NULL */
+  void* out;                     /* as q */
+  float* lse;                    /* [batch, new_tokens, heads], natural logarithm of the softmax sum, or NULL */
+  void* workspace;               /* b200sd_paged_attention_workspace_bytes() bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  int64_t batch, new_tokens, heads, kv_heads, head_dim;
+  int64_t num_pages, page_tokens, table_width;
+  int64_t window;                /* 0: none */
+  int32_t q_dtype;               /* BF16 or F16 */
+  int32_t cache_dtype;           /* F8E4M3FN, F8E5M2 or S8 */
+  float softmax_scale;
+} B200SD_PagedAttention;
+
 /* One-time set-up for the current device (kernel attributes, SM count).  Called implicitly by the
  * first launch on a device; call it yourself before capturing a stream into a CUDA graph. */
 int b200sd_init_device(char* err, size_t err_len);
@@ -184,6 +275,17 @@ int b200sd_dot_s8(const B200SD_DotS8* args, void* cuda_stream, char* err, size_t
  * xla/service/gpu/thunk_emitter.cc:939-988 with GemmConfig::scale_mode == BLOCK_SCALING). */
 int b200sd_block_scaled_dot_mx(const B200SD_BlockScaledDotMx* args, void* cuda_stream, char* err, size_t err_len);
 int b200sd_check_block_scaled_dot_mx(const B200SD_BlockScaledDotMx* args, char* err, size_t err_len);
+
+/* The operators of a decode step with quantised weights and cache, and their checks without pointers or device. */
+int b200sd_dot_w4(const B200SD_DotW4* args, void* cuda_stream, char* err, size_t err_len);
+int b200sd_check_dot_w4(const B200SD_DotW4* args, char* err, size_t err_len);
+int b200sd_kv_cache_append(const B200SD_KvCacheAppend* args, void* cuda_stream, char* err, size_t err_len);
+int b200sd_check_kv_cache_append(const B200SD_KvCacheAppend* args, char* err, size_t err_len);
+int b200sd_paged_attention(const B200SD_PagedAttention* args, void* cuda_stream, char* err, size_t err_len);
+int b200sd_check_paged_attention(const B200SD_PagedAttention* args, char* err, size_t err_len);
+/* Scratch of one attention call; 0 for sizes that the call refuses. */
+size_t b200sd_paged_attention_workspace_bytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads,
+                                              int64_t head_dim);
 
 /* Validate everything about a call except the pointer values (which may be NULL): types, shapes,
  * epilogue, the supported type table (`TypesAreSupportedByCublasLt`,
@@ -219,7 +321,7 @@ int b200sd_load_config_table(const char* path, int32_t* entries, char* err, size
 uint64_t b200sd_launch_count(void);
 
 /* Synchronises the device, then returns and clears the bit mask kernels set when one of their
- * bounded waits expired (0 = healthy).  The host-visible half of failure detection; stands where
+ * bounded waits expired, or a page table led outside of its cache (0 = healthy).  The host-visible half of failure detection; stands where
  * the reference relies on its execution watchdog (xla/service/gpu/execution_watchdog.h:43-61). */
 int b200sd_device_status(uint32_t* bits, char* err, size_t err_len);
 
@@ -380,9 +482,26 @@ void* b200sd_ffi_dot_s8_initialize(void* call_frame);
 void* b200sd_ffi_block_scaled_dot_mx(void* call_frame);
 void* b200sd_ffi_block_scaled_dot_mx_instantiate(void* call_frame);
 void* b200sd_ffi_block_scaled_dot_mx_initialize(void* call_frame);
+/* Target "b200$dot$w4": operands (x, w, scale, [zero iff weight_type is U4], [bias iff the epilogue adds one]), results
+ * (D, [workspace]); attributes weight_type, epilogue (i32). */
+void* b200sd_ffi_dot_w4(void* call_frame);
+void* b200sd_ffi_dot_w4_instantiate(void* call_frame);
+void* b200sd_ffi_dot_w4_initialize(void* call_frame);
+/* Target "b200$kv_cache$append": operands (k_new, v_new, k_pages, v_pages, k_scale, v_scale, page_table, seq_lens,
+ * [new_lens]), results (k_pages, v_pages, k_scale, v_scale, [workspace]) in the operands' own buffers
+ * (output_to_operand_aliasing). */
+void* b200sd_ffi_kv_cache_append(void* call_frame);
+void* b200sd_ffi_kv_cache_append_instantiate(void* call_frame);
+void* b200sd_ffi_kv_cache_append_initialize(void* call_frame);
+/* Target "b200$paged_attention$kv8": operands (q, k_pages, v_pages, k_scale, v_scale, page_table, seq_lens,
+ * [new_lens]), results (out, [lse iff emit_lse], workspace); attributes softmax_scale (f64 or f32), window (i64),
+ * emit_lse (bool). */
+void* b200sd_ffi_paged_attention(void* call_frame);
+void* b200sd_ffi_paged_attention_instantiate(void* call_frame);
+void* b200sd_ffi_paged_attention_initialize(void* call_frame);
 #endif
 
-/* Registers the three bundles with the given `const XLA_FFI_Api*` (what XLA_FFI_REGISTER_HANDLER does,
+/* Registers the six bundles with the given `const XLA_FFI_Api*` (what XLA_FFI_REGISTER_HANDLER does,
  * xla/ffi/api/api.h:2881-2893).  Returns 0 or an error code. */
 int b200sd_ffi_register(const void* xla_ffi_api, char* err, size_t err_len);
 

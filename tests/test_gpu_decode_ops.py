@@ -1,0 +1,422 @@
+"""The decode-step operators on the device against their 64-bit forms, where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+import decode_reference as ref
+import xla_b200
+from decode_reference import E4M3, E5M2, HALF_STEP, S8
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _status():
+    torch.cuda.synchronize()
+    return xla_b200.device_status()
+
+
+# ---- the dot with 4-bit weights ---------------------------------------------------------------
+def _dot_inputs(dev, m, n, k, group, dtype, zeros, bias, scale_dtype=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((m, k), generator=g).to(dtype)
+    w = torch.randint(0, 256, (n, k // 2), generator=g).to(torch.uint8)
+    scale = (torch.rand((n, k // group), generator=g) + 0.5).to(scale_dtype or dtype)
+    zero = torch.randint(0, 16, (n, k // group), generator=g).to(torch.uint8) if zeros else None
+    b = torch.randn((n,), generator=g).to(dtype) if bias else None
+    return [None if t is None else t.to(dev) for t in (x, w, scale, zero, b)]
+
+
+def _check_dot(out, inputs, k):
+    want, size = ref.dot(*inputs)
+    # Products of integers below 32 and 11-bit values are exact in f32; each of the k + groups + 1 additions and the
+    # multiplications by the scales is off by at most one step of 2^-23 of the magnitudes summed; D is rounded once.
+    tolerance = (k + 2 * inputs[2].shape[1] + 2) * 2.0 ** -23 * size + HALF_STEP[out.dtype] * (1 + 2.0 ** -10) * want.abs()
+    off = (out.double() - want).abs()
+    assert bool((off <= tolerance).all()), float((off - tolerance).max())
+    # The additions' errors are independent of one another, about sqrt(k) steps of the result and not k of the terms.
+    norm = float(want.norm())
+    assert float(off.norm()) <= (HALF_STEP[out.dtype] + 4 * math.sqrt(k) * 2.0 ** -23) * norm + 1e-30
+
+
+@pytest.mark.parametrize("m,n,k,group,dtype,zeros,bias", [
+    (1, 256, 512, 128, BF16, False, False),
+    (1, 1, 32, 32, F16, False, True),
+    (1, 17, 64, 64, BF16, True, False),
+    (1, 130, 4096, 64, F16, True, True),
+    (2, 33, 160, 32, BF16, False, True),
+    (3, 1000, 1024, 128, F16, False, False),
+    (5, 515, 4416, 32, F16, True, True),
+    (7, 15, 8192, 128, BF16, True, False),
+    (8, 2048, 2048, 64, BF16, False, False),
+    (9, 16, 96, 32, F16, False, True),
+    (16, 300, 1152, 128, BF16, True, True),
+    (17, 129, 640, 64, BF16, True, False),
+    (31, 77, 256, 256, F16, False, False),
+    (32, 512, 3200, 128, BF16, False, True),
+    (33, 31, 1920, 64, F16, True, False),
+    (64, 200, 1536, 512, BF16, True, True),
+    (64, 5, 64, 32, F16, False, False),
+])
+def test_dot_w4(cuda_device, m, n, k, group, dtype, zeros, bias):
+    inputs = _dot_inputs(cuda_device, m, n, k, group, dtype, zeros, bias, seed=m * n + k)
+    x, w, scale, zero, b = inputs
+    _check_dot(xla_b200.dot_w4(x, w, scale, zero=zero, bias=b), inputs, k)
+    _check_dot(xla_b200.dot_w4(x, w, scale, zero=zero, bias=b, out_dtype=F32), inputs, k)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, F16, BF16])
+def test_dot_w4_scale_types(cuda_device, scale_dtype):
+    for dtype in (BF16, F16):
+        inputs = _dot_inputs(cuda_device, 4, 96, 768, 64, dtype, True, False, scale_dtype)
+        _check_dot(xla_b200.dot_w4(inputs[0], inputs[1], inputs[2], zero=inputs[3]), inputs, 768)
+
+
+def test_dot_w4_every_nibble_and_zero_point(cuda_device):
+    """One group whose weights are all 256 bytes' nibbles, against x of one 1 at a time: exact."""
+    k = 512
+    w = torch.arange(256, dtype=torch.uint8).reshape(1, 256).expand(16, 256).contiguous().to(cuda_device)
+    x = torch.zeros((32, k), dtype=F16, device=cuda_device)
+    for zero in (None, torch.arange(16, dtype=torch.uint8, device=cuda_device).reshape(16, 1).expand(16, 4).contiguous()):
+        scale = torch.ones((16, 4), dtype=F32, device=cuda_device)
+        for start in range(0, k, 32):
+            x.zero_()
+            x[torch.arange(32), start + torch.arange(32)] = 1
+            got = xla_b200.dot_w4(x, w, scale, zero=zero, out_dtype=F32)
+            assert torch.equal(got.double(), ref.dot(x, w, scale, zero)[0])
+
+
+def test_dot_w4_large_magnitudes_and_infinities(cuda_device):
+    x, w, scale, _, _ = _dot_inputs(cuda_device, 3, 40, 256, 64, BF16, False, False)
+    x[0] *= 2.0 ** 100
+    x[1] *= 2.0 ** -100
+    x[2, 17] = math.inf
+    out = xla_b200.dot_w4(x, w, scale, out_dtype=F32)
+    _check_dot(out[:2], [x[:2], w, scale, None, None], 256)
+    full = ref.weights(w, None, 64)[:, 17]
+    assert torch.equal(out[2].isposinf(), full > 0) and torch.equal(out[2].isneginf(), full < 0) and torch.equal(out[2].isnan(), full == 0)
+
+
+def test_dot_w4_no_rows_and_neighbours_untouched(cuda_device):
+    x, w, scale, _, _ = _dot_inputs(cuda_device, 5, 37, 128, 32, F16, False, False)
+    assert xla_b200.dot_w4(x[:0], w, scale).shape == (0, 37)
+    big = torch.full((9, 37), 7.0, dtype=F16, device=cuda_device)
+    xla_b200.dot_w4(x, w, scale, out=big[2:7])
+    assert bool((big[:2] == 7).all()) and bool((big[7:] == 7).all())
+    _check_dot(big[2:7], [x, w, scale, None, None], 128)
+
+
+def test_dot_w4_same_result_every_time(cuda_device):
+    x, w, scale, zero, b = _dot_inputs(cuda_device, 6, 1000, 4096, 128, BF16, True, True)
+    first = xla_b200.dot_w4(x, w, scale, zero=zero, bias=b, out_dtype=F32)
+    assert all(torch.equal(first, xla_b200.dot_w4(x, w, scale, zero=zero, bias=b, out_dtype=F32)) for _ in range(5))
+
+
+# ---- appending to the cache --------------------------------------------------------------------
+def _append_inputs(dev, batch, new, kv_heads, dim, page, lens, code, dtype, new_lens=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    pages = sum(max(0, -(-n // page)) for n in lens) + 2
+    k, v, ks, vs = ref.make_cache(pages, kv_heads, page, dim, code, dev, seed)
+    ks, vs = torch.exp2(torch.round(torch.log2(ks))), torch.exp2(torch.round(torch.log2(vs)))
+    fresh = [(torch.randn((batch, new, kv_heads, dim), generator=g) * torch.exp2(torch.randint(-6, 5, (batch, new, kv_heads, 1), generator=g))).to(dtype).to(dev) for _ in range(2)]
+    table = ref.make_table(lens, page, pages, dev, seed)
+    lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+    new_lens = None if new_lens is None else torch.tensor(new_lens, dtype=torch.int32, device=dev)
+    return fresh + [k, v, ks, vs, table, lens], new_lens
+
+
+def _check_append(args, new_lens):
+    want = ref.append(*args, new_lens)
+    xla_b200.kv_cache_append(*args, new_lens=new_lens)
+    for got, expected in zip(args[2:6], want):
+        assert torch.equal(got.view(torch.uint8), expected.view(torch.uint8))
+
+
+@pytest.mark.parametrize("batch,new,kv_heads,dim,page,lens,code,dtype,new_lens", [
+    (1, 1, 1, 16, 16, [1], E4M3, BF16, None),
+    (3, 1, 2, 64, 16, [16, 17, 33], S8, F16, None),
+    (4, 1, 8, 128, 64, [1, 64, 65, 200], E4M3, BF16, None),
+    (2, 5, 3, 80, 32, [5, 70], E5M2, BF16, None),
+    (2, 33, 2, 96, 16, [40, 49], E4M3, F16, [33, 7]),
+    (3, 100, 1, 256, 128, [100, 128, 300], S8, BF16, [100, 0, 99]),
+    (2, 64, 2, 128, 64, [64, 129], E5M2, F16, [64, 64]),
+    (2, 3, 2, 48, 16, [2, 0], E4M3, BF16, [2, 0]),
+])
+def test_append(cuda_device, batch, new, kv_heads, dim, page, lens, code, dtype, new_lens):
+    args, fresh = _append_inputs(cuda_device, batch, new, kv_heads, dim, page, lens, code, dtype, new_lens, seed=sum(lens))
+    _check_append(args, fresh)
+    _check_append(args, fresh)          # again at the same place: the same cache
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("code", [E4M3, E5M2, S8])
+def test_append_token_by_token_grows_the_scale(cuda_device, code):
+    """Tokens of growing size, one call each: every step equals the definition's."""
+    page, dim = 16, 32
+    k, v, ks, vs = ref.make_cache(3, 1, page, dim, code, cuda_device)
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=cuda_device)
+    g = torch.Generator().manual_seed(3)
+    for t in range(20):
+        k_new, v_new = ((torch.randn((1, 1, 1, dim), generator=g) * 2.0 ** (t / 2 - 4)).to(BF16).to(cuda_device) for _ in range(2))
+        _check_append([k_new, v_new, k, v, ks, vs, table, torch.tensor([t + 1], dtype=torch.int32, device=cuda_device)], None)
+
+
+@pytest.mark.parametrize("code", [E4M3, E5M2, S8])
+@pytest.mark.parametrize("value", [0.0, ref.QMAX[E4M3], 449.0, 127.0, 128.0, 57344.0, 1e-40, 3e38, math.inf, -math.inf, math.nan])
+def test_append_values_at_the_borders(cuda_device, code, value):
+    k_new = torch.full((1, 2, 1, 16), 0.75, dtype=BF16, device=cuda_device)
+    k_new[0, 0, 0, 3] = value
+    v_new = torch.full_like(k_new, value)
+    k, v, ks, vs = ref.make_cache(2, 1, 16, 16, code, cuda_device)
+    args = [k_new, v_new, k, v, ks, vs, torch.tensor([[1]], dtype=torch.int32, device=cuda_device), torch.tensor([2], dtype=torch.int32, device=cuda_device)]
+    _check_append(args, None)
+
+
+def test_append_to_pages_with_other_scales(cuda_device):
+    """Scales that are no powers of two, as another quantiser leaves them."""
+    args, _ = _append_inputs(cuda_device, 3, 2, 2, 64, 16, [9, 20, 34], E4M3, BF16)
+    args[4].mul_(1.3)
+    args[5].mul_(0.7)
+    _check_append(args, None)
+
+
+def test_append_reports_pages_outside_of_the_cache(cuda_device):
+    args, _ = _append_inputs(cuda_device, 2, 2, 1, 32, 16, [17, 20], E4M3, BF16)
+    args[6][0, 1] = 10 ** 6                    # the second token of sequence 0 has no page
+    args[7][1] = 100                           # sequence 1 is longer than its table
+    _check_append(args, None)
+    assert _status() == 64 and _status() == 0
+
+
+# ---- attention ---------------------------------------------------------------------------------
+def _attention_inputs(dev, heads, kv_heads, dim, page, lens, new, code, dtype, seed=0, sharp=2.0):
+    pages = sum(max(0, -(-n // page)) for n in lens) + 2
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn((len(lens), new, heads, dim), generator=g) * sharp).to(dtype).to(dev)
+    cache = ref.make_cache(pages, kv_heads, page, dim, code, dev, seed)
+    return [q, *cache, ref.make_table(lens, page, pages, dev, seed), torch.tensor(lens, dtype=torch.int32, device=dev)]
+
+
+def _attention_tolerance(want, size, slack, dtype):
+    # A weight is off by its rounding to 11 bits (relative 2^-11), by the error of its score (slack, twice: it is in the
+    # weight and in the sum) and by a few steps of exp2 and of the rescalings; the output is rounded once.
+    return size * (2.0 ** -11 * (1 + 2.0 ** -6) + 2 * slack[..., None] + 2.0 ** -18) + HALF_STEP[dtype] * (1 + 2.0 ** -7) * want.abs() + 2.0 ** -25
+
+
+def _check_attention(args, new_lens=None, window=0, scale=None, out=None):
+    new_lens = None if new_lens is None else torch.tensor(new_lens, dtype=torch.int32, device=args[0].device)
+    got, lse = out if out is not None else xla_b200.paged_attention_kv8(*args, new_lens=new_lens, window=window, softmax_scale=scale, return_lse=True)
+    want, want_lse, size, slack = ref.attention(*args, new_lens, scale, window)
+    tolerance = _attention_tolerance(want, size, slack, got.dtype)
+    off = (got.double() - want).abs()
+    assert bool((off <= tolerance).all()), float((off - tolerance).max())
+    empty = want_lse == -math.inf
+    assert torch.equal(lse == -math.inf, empty) and bool((got[empty] == 0).all())
+    close = (lse.double() - want_lse)[~empty].abs() <= (slack + 2.0 ** -18 + want_lse.abs() * 2.0 ** -22)[~empty]
+    assert bool(close.all())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,lens,new,code,dtype,new_lens,window", [
+    (1, 1, 16, 16, [1], 1, E4M3, BF16, None, 0),
+    (8, 2, 64, 16, [37], 1, E4M3, F16, None, 0),
+    (8, 1, 128, 16, [0, 1, 15, 16, 17, 63, 64, 65], 1, E4M3, BF16, None, 0),
+    (32, 8, 128, 64, [300, 5, 64], 1, E4M3, BF16, None, 0),
+    (4, 4, 80, 32, [129, 31], 1, E5M2, BF16, None, 0),
+    (5, 1, 96, 16, [100], 1, S8, F16, None, 0),
+    (16, 1, 112, 16, [77, 200], 1, E5M2, F16, None, 0),
+    (6, 2, 256, 16, [130, 47], 1, E4M3, F16, None, 0),
+    (40, 1, 192, 64, [190], 1, S8, BF16, None, 0),
+    (16, 4, 128, 32, [5, 40, 130], 5, S8, BF16, None, 0),
+    (8, 2, 64, 16, [8, 3, 100], 8, E4M3, F16, [8, 3, 2], 0),
+    (64, 8, 128, 128, [1000, 129], 3, E4M3, BF16, [0, 3], 0),
+    (8, 2, 128, 16, [500, 20, 1], 1, E4M3, BF16, None, 33),
+    (8, 2, 64, 64, [300, 65], 7, E5M2, BF16, None, 1),
+    (4, 2, 128, 32, [200], 64, E4M3, BF16, None, 100),
+    (2, 1, 32, 16, [64], 64, S8, F16, None, 0),
+    (8, 8, 256, 128, [700], 2, E5M2, BF16, None, 0),
+])
+def test_attention(cuda_device, heads, kv_heads, dim, page, lens, new, code, dtype, new_lens, window):
+    args = _attention_inputs(cuda_device, heads, kv_heads, dim, page, lens, new, code, dtype, seed=sum(lens) + dim)
+    _check_attention(args, new_lens, window)
+    assert _status() == 0
+
+
+def test_attention_of_long_and_short_sequences_together(cuda_device):
+    """One sequence far longer than the others: its work is split over the card and joined."""
+    for dtype, new in ((BF16, 1), (F16, 2)):
+        args = _attention_inputs(cuda_device, 4, 1, 128, 64, [3, 20000, 64, 0, 7001], new, E4M3, dtype)
+        _check_attention(args, [min(n, new) for n in (3, 20000, 64, 0, 7001)])
+    _check_attention(_attention_inputs(cuda_device, 6, 3, 64, 16, [9000], 1, S8, BF16), window=5000)
+    _check_attention(_attention_inputs(cuda_device, 2, 1, 256, 128, [6000, 1], 1, E4M3, BF16))
+
+
+def test_attention_scales_and_sharp_rows(cuda_device):
+    """Very sharp softmax, tiny and huge queries, page scales far apart, a negative and a zero softmax scale."""
+    args = _attention_inputs(cuda_device, 8, 2, 64, 16, [150, 90], 1, E4M3, BF16, sharp=8.0)
+    _check_attention(args)
+    _check_attention(args, scale=0.0)
+    _check_attention(args, scale=-0.1)
+    args[0][0, 0, 0] *= 2.0 ** -90
+    args[0][0, 0, 1] *= 2.0 ** -20
+    _check_attention(args)
+    args[4][:] *= torch.exp2(torch.arange(args[4].shape[0], device=cuda_device) % 7 * 5.0 - 15)[:, None]
+    args[4][3] = 0
+    _check_attention(args)
+    args[0] = args[0] * 2.0 ** 60
+    args[3].mul_(2.0 ** -60)
+    _check_attention(args)
+
+
+@pytest.mark.parametrize("code,bits", [(E4M3, 0x7F), (E5M2, 0x7F), (E5M2, 0x7C)])
+def test_attention_ignores_what_it_does_not_see(cuda_device, code, bits):
+    """NaN and infinity codes behind a sequence's end, in front of a window, and in later tokens of the same call."""
+    args = _attention_inputs(cuda_device, 8, 2, 128, 16, [35, 50], 3, code, BF16)
+    table = args[5]
+    for pages in (args[1], args[2]):
+        raw = pages.view(torch.uint8)
+        raw[int(table[0, 2]), :, 3:] = bits            # behind the end of sequence 0
+        raw[int(table[1, 0])] = bits                   # in front of the window of sequence 1
+        raw[int(table[1, 1]), :, :4] = bits
+    for scales in args[3:5]:
+        scales[int(table[1, 0])] = math.nan
+    # A window of 30 from positions 47, 48, 49 reaches back to 18: of page 1, slots 0 and 1 are not seen ...
+    for pages in (args[1], args[2]):
+        pages.view(torch.uint8)[int(table[1, 1]), :, 2:4] = 0         # ... and 2, 3 are seen by some rows
+    _check_attention(args, window=30)
+
+
+def test_attention_keeps_a_bad_value_to_the_rows_that_see_it(cuda_device):
+    """A NaN in the values of the last drafted token reaches that token's rows only."""
+    for code, bits in ((E4M3, 0x7F), (E5M2, 0x7D), (E5M2, 0x7C)):
+        args = _attention_inputs(cuda_device, 4, 2, 128, 16, [40], 3, code, BF16)
+        want, _, size, slack = ref.attention(*args)
+        args[2].view(torch.uint8)[int(args[5][0, 2]), :, 7, 5] = bits          # position 39, column 5
+        got = xla_b200.paged_attention_kv8(*args)
+        inside = (got.double() - want).abs() <= _attention_tolerance(want, size, slack, got.dtype)
+        assert bool(inside[0, :2].all())
+        assert bool((~torch.isfinite(got[0, 2, :, 5])).all())
+        others = torch.arange(128, device=cuda_device) != 5
+        assert bool(inside[0, 2][:, others].all())
+
+
+def test_attention_reports_pages_outside_of_the_cache(cuda_device):
+    args = _attention_inputs(cuda_device, 4, 2, 64, 16, [60, 33], 1, E4M3, BF16)
+    args[5][0, 1] = -5
+    args[5][1, 1] = 1 << 30
+    _check_attention(args)
+    assert _status() == 64 and _status() == 0
+    args = _attention_inputs(cuda_device, 4, 2, 64, 16, [60, 33], 1, E4M3, BF16)
+    args[6][0] = 1000                                     # a length behind the end of the table
+    _check_attention(args)
+    assert _status() == 64 and _status() == 0
+
+
+def test_attention_over_a_cache_of_more_than_4_gib(cuda_device):
+    pages, kv_heads, page, dim = 70000, 4, 128, 128        # 4.6 GB each for keys and values
+    k, v = (torch.zeros((pages, kv_heads, page, dim), dtype=torch.uint8, device=cuda_device).view(E4M3) for _ in range(2))
+    small = ref.make_cache(3, kv_heads, page, dim, E4M3, cuda_device)
+    where = torch.tensor([69999, 33000, 66000], device=cuda_device)
+    ks, vs = (torch.ones((pages, kv_heads), device=cuda_device) for _ in range(2))
+    for big, part in ((k, small[0]), (v, small[1])):
+        big.view(torch.uint8)[where] = part.view(torch.uint8)
+    ks[where], vs[where] = small[2], small[3]
+    q = torch.randn((1, 1, 8, dim), device=cuda_device).to(BF16)
+    lens = torch.tensor([300], dtype=torch.int32, device=cuda_device)
+    fresh = torch.randn((2, 1, 1, kv_heads, dim), device=cuda_device).to(BF16)
+    table = where.to(torch.int32).reshape(1, 3)
+    near = [*small, torch.arange(3, dtype=torch.int32, device=cuda_device).reshape(1, 3), lens]
+    xla_b200.kv_cache_append(fresh[0], fresh[1], *near)
+    xla_b200.kv_cache_append(fresh[0], fresh[1], k, v, ks, vs, table, lens)
+    assert torch.equal(k.view(torch.uint8)[where], small[0].view(torch.uint8)) and torch.equal(vs[where], small[3])
+    _check_attention([q, *near], out=xla_b200.paged_attention_kv8(q, k, v, ks, vs, table, lens, return_lse=True))
+
+
+def test_attention_of_nothing(cuda_device):
+    args = _attention_inputs(cuda_device, 4, 2, 64, 16, [0, 0], 1, E4M3, BF16)
+    out, lse = xla_b200.paged_attention_kv8(*args, return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all()) and _status() == 0
+    none = [args[0][:0], *args[1:5], args[5][:0], args[6][:0]]
+    assert xla_b200.paged_attention_kv8(*none).shape == (0, 1, 4, 64)
+    assert xla_b200.paged_attention_kv8(args[0][:, :0], *args[1:]).shape == (2, 0, 4, 64)
+
+
+# ---- together, on streams and in graphs ---------------------------------------------------------
+def test_a_decode_step(cuda_device):
+    """Projection, append and attention one after the other, for a few steps, against the 64-bit forms."""
+    heads, kv_heads, dim, page, hidden = 8, 2, 64, 16, 256
+    g = torch.Generator().manual_seed(1)
+    w = torch.randint(0, 256, ((heads + 2 * kv_heads) * dim, hidden // 2), generator=g).to(torch.uint8).to(cuda_device)
+    scale = ((torch.rand((w.shape[0], hidden // 64), generator=g) + 0.5) * 0.01).to(BF16).to(cuda_device)
+    cache = list(ref.make_cache(8, kv_heads, page, dim, E4M3, cuda_device))
+    table = torch.tensor([[3, 1, 7], [6, 0, 2]], dtype=torch.int32, device=cuda_device)
+    for step in range(4):
+        x = torch.randn((2, hidden), generator=g).to(BF16).to(cuda_device)
+        lens = torch.tensor([15 + step, 30 + step], dtype=torch.int32, device=cuda_device)
+        qkv = xla_b200.dot_w4(x, w, scale)
+        _check_dot(qkv, [x, w, scale, None, None], hidden)
+        q, k_new, v_new = (t.reshape(2, 1, -1, dim).contiguous() for t in qkv.split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+        _check_append([k_new, v_new, *cache, table, lens], None)
+        _check_attention([q, *cache, table, lens])
+
+
+def test_calls_on_a_side_stream_and_in_two_graphs(cuda_device):
+    """Two captured steps share the workspace and the cache and are replayed with other lengths and inputs."""
+    args = _attention_inputs(cuda_device, 8, 2, 128, 16, [400, 90], 1, E4M3, BF16)
+    longest = args[6].clone()
+    work = torch.empty(xla_b200.paged_attention_workspace_bytes(2, 1, 8, 2, 128), dtype=torch.int8, device=cuda_device)
+    x, w, scale, _, _ = _dot_inputs(cuda_device, 2, 64, 256, 64, BF16, False, False)
+    new = torch.randn((2, 1, 2, 128), device=cuda_device).to(BF16)
+    sites, graphs, outs = [], [], []
+    for _ in range(2):
+        out, y = torch.empty_like(args[0]), torch.empty((2, 64), dtype=BF16, device=cuda_device)
+        lse = torch.empty(out.shape[:3], device=cuda_device)
+        calls = [xla_b200.DotW4Call([x, w, scale], [y]), xla_b200.KvCacheAppendCall([new, new, *args[1:]], args[1:5]),
+                 xla_b200.PagedAttentionKv8Call(args, [out, lse, work], softmax_scale=128 ** -0.5, emit_lse=True)]
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            for call in calls:
+                call.run(stream.cuda_stream, 0)
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for call in calls:
+                call.execute(torch.cuda.current_stream().cuda_stream, 0)
+        sites.append(calls)
+        graphs.append(graph)
+        outs.append((out, lse, y))
+    for lens in ([400, 90], [1, 17], [33, 0], [399, 64]):
+        args[6].copy_(torch.minimum(torch.tensor(lens, dtype=torch.int32, device=cuda_device), longest))
+        args[0].normal_()
+        x.normal_()
+        new.normal_()
+        want = [t.clone() for t in args[1:5]]
+        fresh = torch.clamp(args[6], max=1)
+        want = ref.append(new, new, *want, args[5], args[6], fresh)
+        for graph, (out, lse, y) in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(args[1:5], want))
+            _check_attention(args, [min(n, 1) for n in args[6].tolist()], out=(out, lse))
+            _check_dot(y, [x, w, scale, None, None], 256)
+    xla_b200.device_status()          # a length of 0 with one new token is reported
+
+
+def test_calls_side_by_side_on_two_streams(cuda_device):
+    """Two attentions with their own workspaces at the same time give what each gives alone."""
+    a = _attention_inputs(cuda_device, 16, 2, 128, 64, [9000, 300], 1, E4M3, BF16, seed=1)
+    b = _attention_inputs(cuda_device, 8, 8, 64, 16, [5000], 2, S8, F16, seed=2)
+    alone = [xla_b200.paged_attention_kv8(*t) for t in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, (stream, t) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(stream):
+                got[i].append(xla_b200.paged_attention_kv8(*t))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(alone[i], t) for t in got[i])

@@ -106,6 +106,49 @@ class PeerReduceArgs(C.Structure):
     ]
 
 
+class DotW4Args(C.Structure):
+    """B200SD_DotW4 of include/b200_scaled_dot.h."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("x", C.c_void_p), ("w", C.c_void_p), ("scale", C.c_void_p), ("zero", C.c_void_p), ("bias", C.c_void_p),
+        ("d", C.c_void_p),
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("group", C.c_int64),
+        ("x_dtype", C.c_int32), ("weight_type", C.c_int32), ("scale_dtype", C.c_int32), ("bias_dtype", C.c_int32),
+        ("d_dtype", C.c_int32), ("epilogue", C.c_int32),
+    ]
+
+
+class KvCacheAppendArgs(C.Structure):
+    """B200SD_KvCacheAppend of include/b200_scaled_dot.h."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("k_new", C.c_void_p), ("v_new", C.c_void_p),
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("new_lens", C.c_void_p),
+        ("batch", C.c_int64), ("new_tokens", C.c_int64), ("kv_heads", C.c_int64), ("head_dim", C.c_int64),
+        ("num_pages", C.c_int64), ("page_tokens", C.c_int64), ("table_width", C.c_int64),
+        ("new_dtype", C.c_int32), ("cache_dtype", C.c_int32),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    """B200SD_PagedAttention of include/b200_scaled_dot.h."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("q", C.c_void_p),
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("new_lens", C.c_void_p),
+        ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("batch", C.c_int64), ("new_tokens", C.c_int64), ("heads", C.c_int64), ("kv_heads", C.c_int64),
+        ("head_dim", C.c_int64), ("num_pages", C.c_int64), ("page_tokens", C.c_int64), ("table_width", C.c_int64),
+        ("window", C.c_int64),
+        ("q_dtype", C.c_int32), ("cache_dtype", C.c_int32), ("softmax_scale", C.c_float),
+    ]
+
+
 product = _load(PRODUCT_LIB)
 mock = _load(MOCK_LIB)
 
@@ -117,6 +160,11 @@ product.b200sd_check_scaled_dot_f8.argtypes = [C.POINTER(ScaledDotF8Args), *_ERR
 product.b200sd_check_dot_s8.argtypes = [C.POINTER(DotS8Args), *_ERR]
 product.b200sd_block_scaled_dot_mx.argtypes = [C.POINTER(BlockScaledDotMxArgs), C.c_void_p, *_ERR]
 product.b200sd_check_block_scaled_dot_mx.argtypes = [C.POINTER(BlockScaledDotMxArgs), *_ERR]
+for _name, _args in (("dot_w4", DotW4Args), ("kv_cache_append", KvCacheAppendArgs), ("paged_attention", PagedAttentionArgs)):
+    getattr(product, "b200sd_" + _name).argtypes = [C.POINTER(_args), C.c_void_p, *_ERR]
+    getattr(product, "b200sd_check_" + _name).argtypes = [C.POINTER(_args), *_ERR]
+product.b200sd_paged_attention_workspace_bytes.argtypes = [C.c_int64] * 5
+product.b200sd_paged_attention_workspace_bytes.restype = C.c_size_t
 product.b200sd_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int64]
 product.b200sd_workspace_bytes.restype = C.c_size_t
 product.b200sd_select_kernel.argtypes = [C.c_int64, C.c_int64, C.c_int64]

@@ -356,6 +356,51 @@ int b200sd_block_scaled_dot_mx(const B200SD_BlockScaledDotMx* args, void* cuda_s
   return CopyStatus(st, err, err_len);
 }
 
+int b200sd_check_dot_w4(const B200SD_DotW4* args, char* err, size_t err_len) {
+  if (args == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args is null"), err, err_len);
+  return CopyStatus(ValidateDotW4(*args, /*check_pointers=*/false), err, err_len);
+}
+int b200sd_check_kv_cache_append(const B200SD_KvCacheAppend* args, char* err, size_t err_len) {
+  if (args == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args is null"), err, err_len);
+  return CopyStatus(ValidateKvCacheAppend(*args, /*check_pointers=*/false), err, err_len);
+}
+int b200sd_check_paged_attention(const B200SD_PagedAttention* args, char* err, size_t err_len) {
+  if (args == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args is null"), err, err_len);
+  return CopyStatus(ValidatePagedAttention(*args, /*check_pointers=*/false), err, err_len);
+}
+
+}  // extern "C"
+namespace {
+// Checks, sets the device up and launches one operator of a decode step.
+template <typename Args>
+int RunDecodeOp(const Args* args, void* cuda_stream, Status (*validate)(const Args&, bool),
+                Status (*launch)(const Args&, cudaStream_t, LaunchStats*), char* err, size_t err_len) {
+  if (args == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args is null"), err, err_len);
+  Status st = validate(*args, /*check_pointers=*/true);
+  int device = 0;
+  if (st.ok() && cudaGetDevice(&device) != cudaSuccess) st = Status::Error(kInternal, "cudaGetDevice failed");
+  if (st.ok()) st = InitDevice(device);
+  LaunchStats stats;
+  if (st.ok()) st = launch(*args, static_cast<cudaStream_t>(cuda_stream), &stats);
+  if (st.ok()) g_launches.fetch_add(stats.launches, std::memory_order_relaxed);
+  return CopyStatus(st, err, err_len);
+}
+}  // namespace
+extern "C" {
+
+int b200sd_dot_w4(const B200SD_DotW4* args, void* cuda_stream, char* err, size_t err_len) {
+  return RunDecodeOp(args, cuda_stream, ValidateDotW4, LaunchDotW4, err, err_len);
+}
+int b200sd_kv_cache_append(const B200SD_KvCacheAppend* args, void* cuda_stream, char* err, size_t err_len) {
+  return RunDecodeOp(args, cuda_stream, ValidateKvCacheAppend, LaunchKvCacheAppend, err, err_len);
+}
+int b200sd_paged_attention(const B200SD_PagedAttention* args, void* cuda_stream, char* err, size_t err_len) {
+  return RunDecodeOp(args, cuda_stream, ValidatePagedAttention, LaunchPagedAttention, err, err_len);
+}
+size_t b200sd_paged_attention_workspace_bytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  return PagedAttentionWorkspaceBytes(batch, new_tokens, heads, kv_heads, head_dim);
+}
+
 int b200sd_scaled_dot_f8_progress(const B200SD_ScaledDotF8* args, B200SD_Progress* progress, void* cuda_stream, char* err,
                                   size_t err_len) {
   if (args == nullptr || progress == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args or progress is null"), err, err_len);

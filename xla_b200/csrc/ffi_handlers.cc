@@ -23,7 +23,10 @@
 // command-buffer compatible (xla/ffi/api/api.h:251-268).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <cstdio>
+#include <initializer_list>
 #include <optional>
 #include <string>
 
@@ -421,6 +424,224 @@ ffi::Error BlockScaledDotMxExecute(cudaStream_t stream, ffi::RemainingArgs opera
   return FromCode(b200sd_block_scaled_dot_mx(&a, stream, msg, sizeof(msg)), msg);
 }
 
+// ---- b200$dot$w4 ---------------------------------------------------------------------------
+// Operands (x, w, scale, [zero iff weight_type is U4], [bias iff the epilogue adds one]), results (D, [workspace]).
+// The group size is the ratio of the minor extents of x and scale.
+bool HasDims(const ffi::AnyBuffer& b, std::initializer_list<int64_t> want) {
+  if (b.dimensions().size() != want.size()) return false;
+  return std::equal(want.begin(), want.end(), b.dimensions().begin());
+}
+ffi::Error DecodeDotW4(ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary attrs, B200SD_DotW4* out) {
+  B200SD_DotW4 a{};
+  a.struct_size = sizeof(a);
+  a.weight_type = static_cast<int32_t>(GetInt(attrs, "weight_type").value_or(B200SD_S4));
+  a.epilogue = static_cast<int32_t>(GetInt(attrs, "epilogue").value_or(B200SD_EPILOGUE_DEFAULT));
+  const bool has_zero = a.weight_type == B200SD_U4, has_bias = EpilogueAddsVectorBias(a.epilogue);
+  const size_t want = 3 + (has_zero ? 1 : 0) + (has_bias ? 1 : 0);
+  if (operands.size() != want)
+    return MakeError(3, "expected " + std::to_string(want) + " operands (x, w, scale, [zero], [bias]) for this weight_type and epilogue, got " + std::to_string(operands.size()));
+  if (results.size() < 1 || results.size() > 2) return MakeError(3, "expected results (D, [workspace]), got " + std::to_string(results.size()));
+  auto x = operands.get<ffi::AnyBuffer>(0);
+  auto w = operands.get<ffi::AnyBuffer>(1);
+  auto scale = operands.get<ffi::AnyBuffer>(2);
+  auto d = results.get<ffi::AnyBuffer>(0);
+  if (!x.has_value()) return x.error();
+  if (!w.has_value()) return w.error();
+  if (!scale.has_value()) return scale.error();
+  if (!d.has_value()) return d.error();
+  if (x->dimensions().size() != 2 || w->dimensions().size() != 2 || scale->dimensions().size() != 2)
+    return MakeError(12, "x, w and scale must have rank 2");
+  if (w->element_type() != ffi::DataType::U8 && w->element_type() != ffi::DataType::S8) return MakeError(3, "w must be bytes of two weights (U8 or S8)");
+  a.m = x->dimensions()[0];
+  a.k = x->dimensions()[1];
+  a.n = w->dimensions()[0];
+  if (a.k % 2 != 0 || w->dimensions()[1] != a.k / 2) return MakeError(3, "w must be [n, k / 2] for x [m, k]");
+  const int64_t groups = scale->dimensions()[1];
+  if (scale->dimensions()[0] != a.n || groups < 1 || a.k % groups != 0) return MakeError(3, "scale must be [n, k / group]");
+  a.group = a.k / groups;
+  if (!HasDims(**d, {a.m, a.n})) return MakeError(3, "result shape is not [m, n]");
+  a.x_dtype = static_cast<int32_t>(x->element_type());
+  a.scale_dtype = static_cast<int32_t>(scale->element_type());
+  a.d_dtype = static_cast<int32_t>((*d)->element_type());
+  a.x = x->untyped_data();
+  a.w = w->untyped_data();
+  a.scale = scale->untyped_data();
+  a.d = (*d)->untyped_data();
+  size_t at = 3;
+  if (has_zero) {
+    auto zero = operands.get<ffi::AnyBuffer>(at++);
+    if (!zero.has_value()) return zero.error();
+    if (zero->element_type() != ffi::DataType::U8 || !HasDims(*zero, {a.n, groups})) return MakeError(3, "zero must be U8 [n, k / group]");
+    a.zero = zero->untyped_data();
+  }
+  if (has_bias) {
+    auto bias = operands.get<ffi::AnyBuffer>(at++);
+    if (!bias.has_value()) return bias.error();
+    if (!HasDims(*bias, {a.n})) return MakeError(3, "vector bias must have n elements");
+    a.bias = bias->untyped_data();
+    a.bias_dtype = static_cast<int32_t>(bias->element_type());
+  }
+  *out = a;
+  return ffi::Error::Success();
+}
+ffi::Error DotW4Instantiate(ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary attrs) {
+  B200SD_DotW4 a;
+  ffi::Error e = DecodeDotW4(operands, results, attrs, &a);
+  if (e.failure()) return e;
+  char msg[512];
+  return FromCode(b200sd_check_dot_w4(&a, msg, sizeof(msg)), msg);
+}
+ffi::Error DotW4Execute(cudaStream_t stream, ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary attrs) {
+  B200SD_DotW4 a;
+  ffi::Error e = DecodeDotW4(operands, results, attrs, &a);
+  if (e.failure()) return e;
+  char msg[512];
+  return FromCode(b200sd_dot_w4(&a, stream, msg, sizeof(msg)), msg);
+}
+
+// ---- b200$kv_cache$append and b200$paged_attention$kv8 -------------------------------------
+// The operands that both calls share, from `at` on: k_pages, v_pages, k_scale, v_scale, page_table, seq_lens, [new_lens].
+template <typename Args>
+ffi::Error DecodeCache(ffi::RemainingArgs operands, size_t at, Args* a) {
+  if (operands.size() != at + 6 && operands.size() != at + 7)
+    return MakeError(3, "expected " + std::to_string(at + 6) + " operands, or one more with new_lens, got " + std::to_string(operands.size()));
+  auto k = operands.get<ffi::AnyBuffer>(at), v = operands.get<ffi::AnyBuffer>(at + 1);
+  auto ks = operands.get<ffi::AnyBuffer>(at + 2), vs = operands.get<ffi::AnyBuffer>(at + 3);
+  auto table = operands.get<ffi::AnyBuffer>(at + 4), lens = operands.get<ffi::AnyBuffer>(at + 5);
+  for (const auto* b : {&k, &v, &ks, &vs, &table, &lens})
+    if (!b->has_value()) return b->error();
+  if (k->dimensions().size() != 4) return MakeError(3, "k_pages must be [num_pages, kv_heads, page_tokens, head_dim]");
+  a->num_pages = k->dimensions()[0];
+  a->page_tokens = k->dimensions()[2];
+  if (k->dimensions()[1] != a->kv_heads || k->dimensions()[3] != a->head_dim) return MakeError(3, "k_pages does not have this call's kv_heads and head_dim");
+  if (!HasDims(*v, {a->num_pages, a->kv_heads, a->page_tokens, a->head_dim}) || v->element_type() != k->element_type())
+    return MakeError(3, "v_pages must have the shape and type of k_pages");
+  for (const auto* s : {&ks, &vs})
+    if ((*s)->element_type() != ffi::DataType::F32 || !HasDims(**s, {a->num_pages, a->kv_heads})) return MakeError(3, "k_scale and v_scale must be F32 [num_pages, kv_heads]");
+  if (table->element_type() != ffi::DataType::S32 || table->dimensions().size() != 2 || table->dimensions()[0] != a->batch)
+    return MakeError(3, "page_table must be S32 [batch, pages of the longest sequence]");
+  if (lens->element_type() != ffi::DataType::S32 || !HasDims(*lens, {a->batch})) return MakeError(3, "seq_lens must be S32 [batch]");
+  a->table_width = table->dimensions()[1];
+  a->cache_dtype = static_cast<int32_t>(k->element_type());
+  a->page_table = static_cast<const int32_t*>(table->untyped_data());
+  a->seq_lens = static_cast<const int32_t*>(lens->untyped_data());
+  if (operands.size() == at + 7) {
+    auto fresh = operands.get<ffi::AnyBuffer>(at + 6);
+    if (!fresh.has_value()) return fresh.error();
+    if (fresh->element_type() != ffi::DataType::S32 || !HasDims(*fresh, {a->batch})) return MakeError(3, "new_lens must be S32 [batch]");
+    a->new_lens = static_cast<const int32_t*>(fresh->untyped_data());
+  }
+  return ffi::Error::Success();
+}
+
+ffi::Error DecodeAppend(ffi::RemainingArgs operands, ffi::RemainingRets results, B200SD_KvCacheAppend* out) {
+  B200SD_KvCacheAppend a{};
+  a.struct_size = sizeof(a);
+  if (operands.size() < 2) return MakeError(3, "expected operands (k_new, v_new, k_pages, v_pages, k_scale, v_scale, page_table, seq_lens, [new_lens])");
+  if (results.size() != 4 && results.size() != 5) return MakeError(3, "expected results (k_pages, v_pages, k_scale, v_scale, [workspace]), got " + std::to_string(results.size()));
+  auto k_new = operands.get<ffi::AnyBuffer>(0), v_new = operands.get<ffi::AnyBuffer>(1);
+  if (!k_new.has_value()) return k_new.error();
+  if (!v_new.has_value()) return v_new.error();
+  if (k_new->dimensions().size() != 4) return MakeError(3, "k_new must be [batch, new_tokens, kv_heads, head_dim]");
+  a.batch = k_new->dimensions()[0];
+  a.new_tokens = k_new->dimensions()[1];
+  a.kv_heads = k_new->dimensions()[2];
+  a.head_dim = k_new->dimensions()[3];
+  if (!HasDims(*v_new, {a.batch, a.new_tokens, a.kv_heads, a.head_dim}) || v_new->element_type() != k_new->element_type())
+    return MakeError(3, "v_new must have the shape and type of k_new");
+  a.new_dtype = static_cast<int32_t>(k_new->element_type());
+  a.k_new = k_new->untyped_data();
+  a.v_new = v_new->untyped_data();
+  if (ffi::Error e = DecodeCache(operands, 2, &a); e.failure()) return e;
+  // The cache is updated in place: each result is its operand's buffer.
+  for (size_t i = 0; i < 4; ++i) {
+    auto op = operands.get<ffi::AnyBuffer>(2 + i);
+    auto res = results.get<ffi::AnyBuffer>(i);
+    if (!res.has_value()) return res.error();
+    if ((*res)->element_type() != op->element_type() || (*res)->dimensions().size() != op->dimensions().size() ||
+        !std::equal(op->dimensions().begin(), op->dimensions().end(), (*res)->dimensions().begin()) || (*res)->untyped_data() != op->untyped_data())
+      return MakeError(3, "result " + std::to_string(i) + " must be operand " + std::to_string(2 + i) + "'s buffer (output_to_operand_aliasing)");
+  }
+  a.k_pages = (*results.get<ffi::AnyBuffer>(0))->untyped_data();
+  a.v_pages = (*results.get<ffi::AnyBuffer>(1))->untyped_data();
+  a.k_scale = static_cast<float*>((*results.get<ffi::AnyBuffer>(2))->untyped_data());
+  a.v_scale = static_cast<float*>((*results.get<ffi::AnyBuffer>(3))->untyped_data());
+  *out = a;
+  return ffi::Error::Success();
+}
+ffi::Error KvCacheAppendInstantiate(ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary) {
+  B200SD_KvCacheAppend a;
+  ffi::Error e = DecodeAppend(operands, results, &a);
+  if (e.failure()) return e;
+  char msg[512];
+  return FromCode(b200sd_check_kv_cache_append(&a, msg, sizeof(msg)), msg);
+}
+ffi::Error KvCacheAppendExecute(cudaStream_t stream, ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary) {
+  B200SD_KvCacheAppend a;
+  ffi::Error e = DecodeAppend(operands, results, &a);
+  if (e.failure()) return e;
+  char msg[512];
+  return FromCode(b200sd_kv_cache_append(&a, stream, msg, sizeof(msg)), msg);
+}
+
+ffi::Error DecodeAttention(ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary attrs, B200SD_PagedAttention* out) {
+  B200SD_PagedAttention a{};
+  a.struct_size = sizeof(a);
+  const bool emit_lse = GetBool(attrs, "emit_lse", false);
+  const auto scale = GetFloat(attrs, "softmax_scale");
+  if (!scale.has_value()) return MakeError(3, "softmax_scale is required");
+  a.softmax_scale = static_cast<float>(*scale);
+  a.window = GetInt(attrs, "window").value_or(0);
+  if (operands.size() < 2) return MakeError(3, "expected operands (q, k_pages, v_pages, k_scale, v_scale, page_table, seq_lens, [new_lens])");
+  const size_t want = emit_lse ? 3 : 2;
+  if (results.size() != want) return MakeError(3, std::string("expected results (out, ") + (emit_lse ? "lse, " : "") + "workspace), got " + std::to_string(results.size()));
+  auto q = operands.get<ffi::AnyBuffer>(0), k = operands.get<ffi::AnyBuffer>(1);
+  auto o = results.get<ffi::AnyBuffer>(0), ws = results.get<ffi::AnyBuffer>(want - 1);
+  if (!q.has_value()) return q.error();
+  if (!k.has_value()) return k.error();
+  if (!o.has_value()) return o.error();
+  if (!ws.has_value()) return ws.error();
+  if (q->dimensions().size() != 4 || k->dimensions().size() != 4) return MakeError(3, "q must be [batch, new_tokens, heads, head_dim] and k_pages [num_pages, kv_heads, page_tokens, head_dim]");
+  a.batch = q->dimensions()[0];
+  a.new_tokens = q->dimensions()[1];
+  a.heads = q->dimensions()[2];
+  a.head_dim = q->dimensions()[3];
+  a.kv_heads = k->dimensions()[1];
+  if (ffi::Error e = DecodeCache(operands, 1, &a); e.failure()) return e;
+  if (!HasDims(**o, {a.batch, a.new_tokens, a.heads, a.head_dim}) || (*o)->element_type() != q->element_type()) return MakeError(3, "the result must have the shape and type of q");
+  a.q_dtype = static_cast<int32_t>(q->element_type());
+  a.q = q->untyped_data();
+  a.k_pages = operands.get<ffi::AnyBuffer>(1)->untyped_data();
+  a.v_pages = operands.get<ffi::AnyBuffer>(2)->untyped_data();
+  a.k_scale = static_cast<const float*>(operands.get<ffi::AnyBuffer>(3)->untyped_data());
+  a.v_scale = static_cast<const float*>(operands.get<ffi::AnyBuffer>(4)->untyped_data());
+  a.out = (*o)->untyped_data();
+  if (emit_lse) {
+    auto lse = results.get<ffi::AnyBuffer>(1);
+    if (!lse.has_value()) return lse.error();
+    if ((*lse)->element_type() != ffi::DataType::F32 || !HasDims(**lse, {a.batch, a.new_tokens, a.heads})) return MakeError(3, "lse must be F32 [batch, new_tokens, heads]");
+    a.lse = static_cast<float*>((*lse)->untyped_data());
+  }
+  a.workspace = (*ws)->untyped_data();
+  a.workspace_bytes = (*ws)->size_bytes();
+  *out = a;
+  return ffi::Error::Success();
+}
+ffi::Error PagedAttentionInstantiate(ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary attrs) {
+  B200SD_PagedAttention a;
+  ffi::Error e = DecodeAttention(operands, results, attrs, &a);
+  if (e.failure()) return e;
+  char msg[512];
+  return FromCode(b200sd_check_paged_attention(&a, msg, sizeof(msg)), msg);
+}
+ffi::Error PagedAttentionExecute(cudaStream_t stream, ffi::RemainingArgs operands, ffi::RemainingRets results, ffi::Dictionary attrs) {
+  B200SD_PagedAttention a;
+  ffi::Error e = DecodeAttention(operands, results, attrs, &a);
+  if (e.failure()) return e;
+  char msg[512];
+  return FromCode(b200sd_paged_attention(&a, stream, msg, sizeof(msg)), msg);
+}
+
 }  // namespace
 
 XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_block_scaled_dot_mx_instantiate, BlockScaledDotMxInstantiate,
@@ -456,6 +677,39 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_s8, DotS8Execute,
                                   .Attrs(),
                               {ffi::Traits::kCmdBufferCompatible});
 
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4_instantiate, DotW4Instantiate,
+                              ffi::Ffi::BindInstantiate().RemainingArgs().RemainingRets().Attrs());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4_initialize, InitializeDevice, ffi::Ffi::BindInitialize());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4, DotW4Execute,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .RemainingArgs()
+                                  .RemainingRets()
+                                  .Attrs(),
+                              {ffi::Traits::kCmdBufferCompatible});
+
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_kv_cache_append_instantiate, KvCacheAppendInstantiate,
+                              ffi::Ffi::BindInstantiate().RemainingArgs().RemainingRets().Attrs());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_kv_cache_append_initialize, InitializeDevice, ffi::Ffi::BindInitialize());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_kv_cache_append, KvCacheAppendExecute,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .RemainingArgs()
+                                  .RemainingRets()
+                                  .Attrs(),
+                              {ffi::Traits::kCmdBufferCompatible});
+
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention_instantiate, PagedAttentionInstantiate,
+                              ffi::Ffi::BindInstantiate().RemainingArgs().RemainingRets().Attrs());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention_initialize, InitializeDevice, ffi::Ffi::BindInitialize());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention, PagedAttentionExecute,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .RemainingArgs()
+                                  .RemainingRets()
+                                  .Attrs(),
+                              {ffi::Traits::kCmdBufferCompatible});
+
 extern "C" int b200sd_ffi_register(const void* xla_ffi_api, char* err, size_t err_len) {
   const XLA_FFI_Api* api = static_cast<const XLA_FFI_Api*>(xla_ffi_api);
   if (api == nullptr) {
@@ -478,6 +732,11 @@ extern "C" int b200sd_ffi_register(const void* xla_ffi_api, char* err, size_t er
       {"b200$block_scaled_dot$mx",
        {b200sd_ffi_block_scaled_dot_mx_instantiate, nullptr, b200sd_ffi_block_scaled_dot_mx_initialize,
         b200sd_ffi_block_scaled_dot_mx}},
+      {"b200$dot$w4", {b200sd_ffi_dot_w4_instantiate, nullptr, b200sd_ffi_dot_w4_initialize, b200sd_ffi_dot_w4}},
+      {"b200$kv_cache$append",
+       {b200sd_ffi_kv_cache_append_instantiate, nullptr, b200sd_ffi_kv_cache_append_initialize, b200sd_ffi_kv_cache_append}},
+      {"b200$paged_attention$kv8",
+       {b200sd_ffi_paged_attention_instantiate, nullptr, b200sd_ffi_paged_attention_initialize, b200sd_ffi_paged_attention}},
   };
   for (const Target& t : targets) {
     XLA_FFI_Error* e = ffi::Ffi::RegisterStaticHandler(api, t.name, "CUDA", t.bundle,

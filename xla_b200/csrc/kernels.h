@@ -7,6 +7,11 @@
 #include <cstdlib>
 #include <string>
 
+#ifndef B200SD_NO_FFI_DECLS
+#define B200SD_NO_FFI_DECLS 1
+#endif
+#include "../../include/b200_scaled_dot.h"
+
 struct CUtensorMap_st;   // CUtensorMap of <cuda.h>
 
 // B200SD_TUNING=1 (make TUNING=1 -> libb200_scaled_dot_tuning.so) compiles in what the product
@@ -37,11 +42,14 @@ enum PrimitiveType : int32_t {
   kInvalidType = 0,
   kS8 = 2,
   kS32 = 4,
+  kU8 = 6,
   kF16 = 10,
   kF32 = 11,
   kBF16 = 16,
   kF8E5M2 = 19,
   kF8E4M3FN = 20,
+  kS4 = 21,
+  kU4 = 22,
   kF8E8M0FNU = 33,
 };
 
@@ -181,6 +189,15 @@ struct MxProblem {
 int TunedMxKernel(int64_t m, int64_t n, int64_t k);      // the tuned table's tile form for this shape, or kKernelAuto
 Status ValidateMx(const MxProblem& g);      // everything but the pointers
 Status LaunchMx(const MxProblem& g, cudaStream_t stream, LaunchStats* stats);
+
+// The operators of a decode step take the C structs as they are, once these checks have passed.
+Status ValidateDotW4(const B200SD_DotW4& a, bool check_pointers);
+Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stats);
+Status ValidateKvCacheAppend(const B200SD_KvCacheAppend& a, bool check_pointers);
+Status LaunchKvCacheAppend(const B200SD_KvCacheAppend& a, cudaStream_t stream, LaunchStats* stats);
+Status ValidatePagedAttention(const B200SD_PagedAttention& a, bool check_pointers);
+Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream, LaunchStats* stats);
+size_t PagedAttentionWorkspaceBytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim);
 
 // Reads (and clears) the device status word the kernels OR their error bits into.  Synchronises
 // the device.

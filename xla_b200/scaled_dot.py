@@ -22,6 +22,7 @@ from . import _native
 
 # XLA PrimitiveType / XLA_FFI_DataType numbers (xla/ffi/api/c_api.h:233-266).
 PRED, S8, S32, S64, F16, F32, F64, BF16, F8E5M2, F8E4M3FN = 1, 2, 4, 5, 10, 11, 12, 16, 19, 20
+U8, S4, U4 = 6, 21, 22
 F8E8M0FNU = 33
 
 TARGET_F8 = "b200$scaled_dot$f8"
@@ -99,7 +100,7 @@ def _torch():
 def _dtype_code(t) -> int:
     torch = _torch()
     table = {
-        torch.float8_e4m3fn: F8E4M3FN, torch.float8_e5m2: F8E5M2, torch.int8: S8, torch.int32: S32,
+        torch.float8_e4m3fn: F8E4M3FN, torch.float8_e5m2: F8E5M2, torch.int8: S8, torch.int32: S32, torch.uint8: U8,
         torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16,
     }
     if hasattr(torch, "float8_e8m0fnu"):
