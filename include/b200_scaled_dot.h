@@ -204,7 +204,8 @@ typedef struct B200SD_DotW4 {
  * head_dim], a value is its code times the scale of its (page, head).  Position t of sequence b is slot
  * t % page_tokens of page page_table[b, t / page_tokens].  seq_lens[b] counts the sequence's tokens
  * INCLUDING the new ones of the call; new_lens[b] (NULL: new_tokens for all) of the new_tokens rows given
- * for a sequence are in use, at positions seq_lens[b] - new_lens[b] onwards.  Entries of the table behind a
+ * for a sequence are in use, at positions seq_lens[b] - new_lens[b] onwards; what would stand below position
+ * 0 is padding, is not stored and sees nothing (so a length of 0 is an idle slot).  Entries of the table behind a
  * sequence's last page are not read.  An entry or a length that points outside of the cache is skipped
  * and reported as bit 64 of b200sd_device_status().
  *

@@ -183,6 +183,13 @@ def test_append_to_pages_with_other_scales(cuda_device):
     _check_append(args, None)
 
 
+def test_append_with_padding_in_front(cuda_device):
+    """Sequences shorter than their new tokens: the first of them are padding."""
+    args, _ = _append_inputs(cuda_device, 4, 20, 2, 32, 16, [0, 1, 17, 20], E4M3, BF16)
+    _check_append(args, None)
+    assert _status() == 0
+
+
 def test_append_reports_pages_outside_of_the_cache(cuda_device):
     args, _ = _append_inputs(cuda_device, 2, 2, 1, 32, 16, [17, 20], E4M3, BF16)
     args[6][0, 1] = 10 ** 6                    # the second token of sequence 0 has no page
@@ -308,6 +315,8 @@ def test_attention_reports_pages_outside_of_the_cache(cuda_device):
     args[5][1, 1] = 1 << 30
     _check_attention(args)
     assert _status() == 64 and _status() == 0
+    args[6][0] = -7                                       # a length below 0 is an idle slot, and reported
+    assert bool((xla_b200.paged_attention_kv8(*args)[0] == 0).all()) and _status() == 64
     args = _attention_inputs(cuda_device, 4, 2, 64, 16, [60, 33], 1, E4M3, BF16)
     args[6][0] = 1000                                     # a length behind the end of the table
     _check_attention(args)
@@ -402,7 +411,7 @@ def test_calls_on_a_side_stream_and_in_two_graphs(cuda_device):
             assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(args[1:5], want))
             _check_attention(args, [min(n, 1) for n in args[6].tolist()], out=(out, lse))
             _check_dot(y, [x, w, scale, None, None], 256)
-    xla_b200.device_status()          # a length of 0 with one new token is reported
+    assert _status() == 0
 
 
 def test_calls_side_by_side_on_two_streams(cuda_device):

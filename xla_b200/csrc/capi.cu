@@ -25,6 +25,7 @@ __device__ uint32_t g_device_status;
 Status InitDenseKernels();
 Status InitSkinnyKernels();
 Status InitMxKernels();
+Status InitAttentionKernels();
 
 namespace {
 
@@ -89,6 +90,7 @@ Status InitDevice(int device) {
     st.init_status = InitDenseKernels();
     if (st.init_status.ok()) st.init_status = InitSkinnyKernels();
     if (st.init_status.ok()) st.init_status = InitMxKernels();
+    if (st.init_status.ok()) st.init_status = InitAttentionKernels();
     // A persisted tuning result named by the environment is loaded with the first device (a file
     // that cannot be read or parsed makes the first call fail loudly instead of being ignored).
     static std::once_flag table_once;

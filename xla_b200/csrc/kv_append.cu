@@ -73,15 +73,16 @@ template <int kCode, typename T>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a) {
   __shared__ uint32_t warp_max[kThreads / 32];
   const int b = blockIdx.z >> 1, which = blockIdx.z & 1, head = blockIdx.y;
-  const int64_t len = a.seq_lens[b];
+  const int32_t length = a.seq_lens[b];
+  const int64_t len = length > 0 ? length : 0;
   const int64_t count = a.new_lens != nullptr ? min(max(a.new_lens[b], 0), a.new_tokens) : a.new_tokens;
-  const int64_t start = len - count;                       // position of the first new token; below 0 for a bad length
+  const int64_t start = len - count;                       // position of the first new token; below 0 where the first ones are padding
   const int64_t first = start > 0 ? start : 0;
   const int64_t index = first / a.page_tokens + blockIdx.x;
   const int64_t base = index * a.page_tokens;              // position of the page's first slot
   const int64_t lo = first > base ? first : base;
   const int64_t hi = len < base + a.page_tokens ? len : base + a.page_tokens;
-  if (start < 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
+  if (length < 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
   if (lo >= hi) return;
   const int64_t page = index < a.table_width ? a.page_table[b * a.table_width + index] : -1;
   if (page < 0 || page >= a.num_pages) {

@@ -1,4 +1,34 @@
 // Attention of each sequence's last tokens over the paged 8-bit cache.
+//
+// For one key head the queries of a sequence -- the heads that share the key head, times the new tokens -- are the rows of
+// one product, so the cache is read once for all of them: 8 or 16 rows per pass.  A step is bound by reading the codes:
+// one byte of keys or values is used for 2 * rows operations.
+//
+// Work.  An item is (sequence, key head, block of rows); a unit is kUnit tokens of an item.  The units of all items, in
+// one line, are dealt out to the CTAs in equal consecutive shares, whatever the lengths are; an item that a share's end
+// cuts leaves its pieces (maximum, sum, weighted values) in the workspace, and a second kernel joins them in order, so
+// that the result does not depend on timing.
+//
+// A CTA is four warps, and each warp works on its own 16 tokens of every 64: they come through a ring in shared
+// memory that only this warp fills (cp.async, 16 bytes per lane) and reads, so no barrier stands between loading and
+// computing until an item ends.  The 16-byte pieces of a row are stored at piece ^ (row & 7), which leaves both kinds of
+// reads below without bank conflicts.
+//
+// Arithmetic, on mma.m16n8k16 with f16 operands and f32 sums; codes of all three cache types are f16 numbers, exactly.
+// Queries are f16 too: bf16 rows are multiplied by a power of two that brings their largest value to 2^13, so nothing is
+// rounded but what lies 2^27 below it.
+//   scores^T [16 tokens, 8 rows] = keys [16, d] queries^T [d, 8]: the order of the products along d is free, so a
+//     lane takes 16 consecutive bytes of a key and feeds them to four products.
+//   values^T [d, 16 tokens] weights^T [16, 8]: a lane takes 16 bytes at the same place of four tokens, pairs the bytes of
+//     two tokens with prmt and decodes the pairs; the weights turn from score layout to operand layout with movmatrix.
+// Token m of the 16 is row m ^ ((m & 1) << 2) of the tile in both products.
+//
+// Softmax.  A page has one scale for its values, so the weight of a token that enters the product is
+// exp2(score + log2(value scale) - M) with one running M per row: the largest weight stays the same even if the scales of
+// pages lie far apart, and the 11 bits of f16 (chosen over bf16's 8, at the same speed) are relative to what matters.
+// M lies 9 below the largest score when it is set, so that weights keep all their bits down to 2^-23 of the largest.  The
+// sum takes the weight times the inverse scale, in f32.  M moves only when a new score passes the one that set it by
+// more than 6, so most tiles rescale nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -6,6 +36,14 @@
 
 namespace b200sd {
 namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = 16;                       // tokens of a warp's step
+constexpr int kStep = kTile * kWarps;           // tokens of a CTA's step
+constexpr int kMaxCtas = 148 * 5;               // of one launch; bounds the workspace
+constexpr float kLift = 9.0f;                   // binary digits that a row's largest weight is lifted by ...
+constexpr float kSlack = 6.0f;                  // ... and that a later one may pass it by: together below f16's 2^15.99
 
 struct AttentionArgs {
   const void* q;
@@ -18,74 +56,665 @@ struct AttentionArgs {
   const int32_t* new_lens;
   void* out;
   float* lse;
-  int32_t batch, new_tokens, heads, kv_heads, head_dim, page_tokens;
-  int64_t num_pages, table_width, window;
-  float softmax_scale;
-  int32_t is_bf16, cache_dtype;
+  float* work;
+  int32_t batch, new_tokens, heads, kv_heads, head_dim, page_shift;
+  int32_t rows, blocks;                         // rows of a (sequence, key head), and blocks of them
+  int32_t num_pages, table_width, window;       // window: 0 none
+  int32_t unit;                                 // tokens of a unit, a multiple of kStep
+  int32_t min_units;                            // a CTA's share is not smaller
+  float scale;                                  // softmax_scale * log2(e)
+  int32_t is_bf16;
   uint32_t* status;
 };
 
-__device__ __forceinline__ float Decode(uint8_t code, int32_t type) {
-  if (type == kS8) return static_cast<float>(static_cast<int8_t>(code));
-  uint32_t h;
-  const uint16_t c = code;
-  if (type == kF8E4M3FN) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-  else asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"(c));
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
+// The positions of one sequence that some row sees, from a multiple of kTile on.
+struct Span {
+  int32_t base;                                 // position of the first new token
+  int32_t count;                                // new tokens
+  int32_t lo, hi;
+  int32_t units;
+};
+
+__device__ __forceinline__ Span SpanOf(const AttentionArgs& a, int b) {
+  Span s;
+  const int32_t len = a.seq_lens[b];
+  s.count = a.new_lens != nullptr ? min(max(a.new_lens[b], 0), a.new_tokens) : a.new_tokens;
+  s.base = max(len, 0) - s.count;               // below 0 for a length that does not hold the new tokens
+  const int32_t capacity = a.table_width << a.page_shift;
+  s.hi = s.count > 0 ? min(max(len, 0), capacity) : 0;
+  s.lo = a.window > 0 ? max(0, s.base + 1 - a.window) & ~(kTile - 1) : 0;
+  s.units = s.hi > s.lo ? (s.hi - s.lo + a.unit - 1) / a.unit : 1;        // an item without tokens still has rows to write
+  return s;
 }
 
-// One warp per row: running maximum, sum and weighted values, token by token.
-__global__ void __launch_bounds__(32) kv_attention_kernel(const AttentionArgs a) {
-  const int lane = threadIdx.x, h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
-  const int64_t row = (static_cast<int64_t>(b) * a.new_tokens + i) * a.heads + h;
-  const int64_t len = a.seq_lens[b];
-  const int64_t count = a.new_lens != nullptr ? min(max(a.new_lens[b], 0), a.new_tokens) : a.new_tokens;
-  int64_t end = i < count ? len - count + i + 1 : 0;             // one behind the last position that the row sees
-  const int64_t first = a.window > 0 && end > a.window ? end - a.window : 0;
-  const int64_t capacity = a.table_width * a.page_tokens;
-  if (end > capacity) {
-    if (lane == 0) atomicOr(a.status, kStatusBadPage);
-    end = capacity;
+// The share of one CTA: `left` units from unit `offset` of item `item` of sequence `b` on.
+struct Share {
+  int32_t b, item, offset;
+  int64_t left;
+  int64_t begin, total, ctas;
+};
+
+// The share of CTA `cta`, with b, item and offset of its first or of its last unit.  Every thread of the block calls it.
+template <int kBlock>
+__device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit) {
+  __shared__ int64_t warp_sum[kBlock / 32];
+  __shared__ Share found;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int per = (a.batch + kBlock - 1) / kBlock, first = min(tid * per, a.batch), end = min(first + per, a.batch);
+  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.blocks;
+  int64_t mine = 0;
+  for (int b = first; b < end; ++b) mine += SpanOf(a, b).units * items;
+  int64_t before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
   }
-  float q[8], o[8] = {};
-  for (int j = 0; j < 8; ++j) {
-    const int d = j * 32 + lane;
-    q[j] = d >= a.head_dim ? 0.0f
-           : a.is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[row * a.head_dim + d])
-                       : __half2float(static_cast<const __half*>(a.q)[row * a.head_dim + d]);
+  if (lane == 31) warp_sum[warp] = before;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kBlock / 32; ++w) {
+    if (w == warp) before += total;
+    total += warp_sum[w];
   }
-  float top = -INFINITY, sum = 0.0f;
-  const int kv = h / (a.heads / a.kv_heads);
-  for (int64_t t = first; t < end; ++t) {
-    const int64_t page = a.page_table[b * a.table_width + t / a.page_tokens];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) atomicOr(a.status, kStatusBadPage);
-      continue;
+  before -= mine;
+  const int64_t ctas = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / a.min_units));
+  const int64_t u0 = cta < ctas ? cta * total / ctas : total, u1 = cta < ctas ? (cta + 1) * total / ctas : total;
+  const int64_t u = last_unit ? u1 - 1 : u0;
+  if (u0 < u1 && u >= before && u < before + mine) {
+    for (int b = first; b < end; ++b) {
+      const int64_t units = SpanOf(a, b).units;
+      if (u < before + units * items) {
+        const int64_t at = u - before;
+        found = {b, static_cast<int32_t>(at / units), static_cast<int32_t>(at % units), u1 - u0, u0, total, ctas};
+        break;
+      }
+      before += units * items;
     }
-    const int64_t at = ((page * a.kv_heads + kv) * a.page_tokens + t % a.page_tokens) * a.head_dim;
-    float s = 0.0f;
-    for (int j = 0; j < 8; ++j)
-      if (j * 32 + lane < a.head_dim) s += q[j] * Decode(a.k_pages[at + j * 32 + lane], a.cache_dtype);
-    for (int w = 16; w > 0; w /= 2) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= a.softmax_scale * a.k_scale[page * a.kv_heads + kv];
-    if (s == -INFINITY) continue;
-    const float next = fmaxf(top, s), fade = expf(top - next), p = expf(s - next), vs = a.v_scale[page * a.kv_heads + kv];
-    sum = sum * fade + p;
-    for (int j = 0; j < 8; ++j)
-      if (j * 32 + lane < a.head_dim) o[j] = o[j] * fade + p * (vs * Decode(a.v_pages[at + j * 32 + lane], a.cache_dtype));
-    top = next;
   }
-  for (int j = 0; j < 8; ++j) {
-    const int d = j * 32 + lane;
-    if (d >= a.head_dim) continue;
-    const float y = sum == 0.0f ? 0.0f : o[j] / sum;
-    if (a.is_bf16) static_cast<__nv_bfloat16*>(a.out)[row * a.head_dim + d] = __float2bfloat16_rn(y);
-    else static_cast<__half*>(a.out)[row * a.head_dim + d] = __float2half_rn(y);
+  __syncthreads();
+  if (u0 >= u1) return {0, 0, 0, 0, 0, total, ctas};
+  return found;
+}
+
+// Steps through the pieces of items that make up a share.
+struct Walk {
+  int32_t b, item, offset;
+  int64_t left;
+  Span span;
+
+  __device__ Walk(const AttentionArgs& a, const Share& s) : b(s.b), item(s.item), offset(s.offset), left(s.left) {
+    if (left > 0) span = SpanOf(a, b);
   }
-  if (a.lse != nullptr && lane == 0) a.lse[row] = top + logf(sum);
+  __device__ int32_t Units() const { return static_cast<int32_t>(min(left, static_cast<int64_t>(span.units - offset))); }
+  __device__ int32_t Begin(const AttentionArgs& a) const { return span.lo + offset * a.unit; }
+  __device__ int32_t End(const AttentionArgs& a) const {
+    return static_cast<int32_t>(min(static_cast<int64_t>(span.hi), static_cast<int64_t>(Begin(a)) + static_cast<int64_t>(Units()) * a.unit));
+  }
+  __device__ void Next(const AttentionArgs& a) {
+    const int32_t n = Units();
+    left -= n;
+    offset += n;
+    if (offset == span.units) {
+      offset = 0;
+      if (++item == a.kv_heads * a.blocks) {
+        item = 0;
+        ++b;
+        if (left > 0) span = SpanOf(a, b);
+      }
+    }
+  }
+};
+
+// Four codes, two by two, to f16 pairs.
+template <int kCode>
+__device__ __forceinline__ void Decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (kCode == kF8E4M3FN) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else if constexpr (kCode == kF8E5M2) {      // the upper half of an f16
+    lo = __byte_perm(w, 0, 0x1404);
+    hi = __byte_perm(w, 0, 0x3424);
+  } else {                                      // 1024 + (code + 128) has the code's bits, offset, in its low byte
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+    uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 lv = __hsub2(*reinterpret_cast<__half2*>(&l), bias), hv = __hsub2(*reinterpret_cast<__half2*>(&h), bias);
+    lo = *reinterpret_cast<const uint32_t*>(&lv);
+    hi = *reinterpret_cast<const uint32_t*>(&hv);
+  }
+}
+template <int kCode>
+__device__ __forceinline__ float Decode1(uint32_t code) {
+  uint32_t lo, hi;
+  Decode4<kCode>(code & 255u, lo, hi);
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(lo)));
+}
+// Whether one of four codes is NaN or infinite.
+template <int kCode>
+__device__ __forceinline__ bool NotFinite4(uint32_t w) {
+  if constexpr (kCode == kS8) return false;
+  const uint32_t bits = kCode == kF8E4M3FN ? 0x7f7f7f7fu : 0x7c7c7c7cu;
+  const uint32_t left = (w & bits) ^ bits;                                  // a zero byte is such a code
+  return ((left - 0x01010101u) & ~left & 0x80808080u) != 0;
+}
+
+__device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t Transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float Exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Ring, exchange buffer and per-tile numbers of one instantiation.
+template <int kDim, int kRowTiles>
+struct Layout {
+  static constexpr int kStages = kDim == 64 ? 4 : kDim == 128 ? 3 : 2;
+  static constexpr int kTileBytes = kTile * kDim;                           // of keys, and again of values
+  static constexpr int kRows = 8 * kRowTiles;
+  static constexpr int kStride = kDim + 4;                                  // floats of a row in the exchange buffer
+  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;
+  static constexpr int kNumbers = kWarps * kStages * 16;
+  static constexpr int kExchange = kWarps * kRows * (kStride + 2) * 4;
+  static constexpr int kBytes = kRing + kNumbers + kExchange;
+  static constexpr int kSlot = kRows * (kDim + 2);                          // floats of a piece in the workspace
+};
+
+// Byte of 16-byte piece `c` of row `r` in a tile.
+template <int kDim>
+__device__ __forceinline__ int PieceAt(int r, int c) {
+  if constexpr (kDim == 64) return (r >> 1) * 128 + ((((r & 1) << 2) | c) ^ (r >> 1)) * 16;
+  return r * kDim + (c >> 3) * 128 + ((c & 7) ^ (r & 7)) * 16;
+}
+// Column of the values' product that m-tile `mt` of lane group `g` holds (its row g; row g + 8 is the next column).
+template <int kDim>
+__device__ __forceinline__ int Column(int g, int mt) {
+  if constexpr (kDim == 64) return 8 * g + 2 * mt;
+  return (mt / 8) * 128 + 16 * g + 2 * (mt % 8);
+}
+
+// One row of the result from its weighted values `o` (4 columns at `d`), its sum and its running maximum.
+__device__ __forceinline__ void StoreRow(const AttentionArgs& a, int b, int head, int row, int count, int d, float4 o, float m, float sum) {
+  const int share = a.heads / a.kv_heads, i = row / share;
+  const int64_t at = (static_cast<int64_t>(b) * a.new_tokens + i) * a.heads + head * share + row % share;
+  const bool empty = i >= count || (m == -INFINITY && sum == 0.0f);
+  if (a.lse != nullptr && d == 0) a.lse[at] = empty ? -INFINITY : 0.69314718055994531f * (m + log2f(sum));
+  if (d >= a.head_dim) return;
+  const float inv = 1.0f / sum;
+  const float4 y = empty ? make_float4(0, 0, 0, 0) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  uint2 packed;
+  if (a.is_bf16) {
+    const __nv_bfloat162 l = __floats2bfloat162_rn(y.x, y.y), h = __floats2bfloat162_rn(y.z, y.w);
+    packed = make_uint2(*reinterpret_cast<const uint32_t*>(&l), *reinterpret_cast<const uint32_t*>(&h));
+  } else {
+    const __half2 l = __floats2half2_rn(y.x, y.y), h = __floats2half2_rn(y.z, y.w);
+    packed = make_uint2(*reinterpret_cast<const uint32_t*>(&l), *reinterpret_cast<const uint32_t*>(&h));
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * a.head_dim + d) = packed;
+}
+
+template <int kCode, int kDim, int kRowTiles>
+__global__ void __launch_bounds__(kThreads) kv_attention_kernel(const AttentionArgs a) {
+  using L = Layout<kDim, kRowTiles>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  if (threadIdx.x == 0) griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const Share share = Locate<kThreads>(a, blockIdx.x, false);
+  if (share.left == 0) return;
+
+  uint8_t* ring = smem + warp * L::kStages * 2 * L::kTileBytes;
+  float4* numbers = reinterpret_cast<float4*>(smem + L::kRing) + warp * L::kStages;
+  float* exchange = reinterpret_cast<float*>(smem + L::kRing + L::kNumbers);
+  float* exchange_max = exchange + kWarps * L::kRows * L::kStride;
+  float* exchange_sum = exchange_max + kWarps * L::kRows;
+
+  // ---- loading: this warp's tiles of the whole share, one after the other -----------------------
+  const int pieces = a.head_dim / 16;
+  const int64_t head_bytes = static_cast<int64_t>(a.head_dim) << a.page_shift;
+  Walk ahead(a, share);
+  int32_t load_pos, load_end, batch_at = 32;               // batch_at: tile of the batch below that comes next
+  int32_t page_of = -1;                                    // lane j: page of tile j of the batch ...
+  float4 numbers_of = {};                                  // ... key scale, log2 of the value scale, its inverse, its sign
+  bool loading = true;
+  load_pos = ahead.Begin(a) + warp * kTile;
+  load_end = ahead.End(a);
+  auto load_tile = [&](int stage) {
+    while (loading && load_pos >= load_end) {
+      ahead.Next(a);
+      batch_at = 32;
+      if (ahead.left == 0) { loading = false; break; }
+      load_pos = ahead.Begin(a) + warp * kTile;
+      load_end = ahead.End(a);
+    }
+    if (loading) {
+      const int head = ahead.item / a.blocks;
+      if (batch_at == 32) {
+        // Pages and scales of the next 32 tiles, one per lane.
+        const int64_t pos = static_cast<int64_t>(load_pos) + static_cast<int64_t>(lane) * kStep;
+        page_of = -1;
+        numbers_of = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+        if (pos < load_end) {
+          const int32_t page = a.page_table[static_cast<int64_t>(ahead.b) * a.table_width + (pos >> a.page_shift)];
+          if (page >= 0 && page < a.num_pages) {
+            page_of = page;
+            const int64_t at = static_cast<int64_t>(page) * a.kv_heads + head;
+            const float vs = a.v_scale[at], size = fminf(fmaxf(fabsf(vs), 0x1p-100f), 0x1p100f);
+            numbers_of = make_float4(a.k_scale[at], log2f(size), 1.0f / size, vs / size);
+          } else {
+            atomicOr(a.status, kStatusBadPage);            // its tokens count as not seen
+          }
+        }
+        batch_at = 0;
+      }
+      const int32_t page = __shfl_sync(0xffffffffu, page_of, batch_at);
+      if (lane == batch_at) numbers[stage] = numbers_of;
+      const int64_t slot = load_pos & ((1 << a.page_shift) - 1);
+      const int64_t at = (static_cast<int64_t>(max(page, 0)) * a.kv_heads + head) * head_bytes + slot * a.head_dim;
+      const uint8_t *k = a.k_pages + at, *v = a.v_pages + at;
+      const uint32_t dst = smem_u32(ring + stage * 2 * L::kTileBytes);
+#pragma unroll
+      for (int i = 0; i < kDim / 32; ++i) {
+        const int piece = i * 32 + lane, r = piece / (kDim / 16), c = piece % (kDim / 16);
+        const bool in = c < pieces && page >= 0;           // what is not there reads as zero
+        const int off = r * a.head_dim + c * 16;
+        CopyAsync16(dst + PieceAt<kDim>(r, c), in ? k + off : a.q, in ? 16 : 0);
+        CopyAsync16(dst + L::kTileBytes + PieceAt<kDim>(r, c), in ? v + off : a.q, in ? 16 : 0);
+      }
+      ++batch_at;
+      load_pos += kStep;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < L::kStages - 1; ++s) load_tile(s);
+
+  // ---- computing, piece by piece ---------------------------------------------------------------
+  int stage = 0;
+  const int group = a.heads / a.kv_heads;
+  for (Walk walk(a, share); walk.left > 0; walk.Next(a)) {
+    const int head = walk.item / a.blocks, row0 = (walk.item % a.blocks) * L::kRows;
+    const Span& span = walk.span;
+    const int32_t begin = walk.Begin(a), end = walk.End(a);
+    if (threadIdx.x == 0 && span.count > 0) {
+      const int32_t len = a.seq_lens[walk.b];
+      if (len < 0 || len > static_cast<int64_t>(a.table_width) << a.page_shift) atomicOr(a.status, kStatusBadPage);
+    }
+
+    // Queries as the products want them, and what turns a product into a score, for the rows 2t and 2t + 1 of each 8.
+    uint32_t q[kRowTiles][kDim / 64][4][2];
+    float factor[kRowTiles][2];
+    int32_t row_end[kRowTiles][2], row_begin[kRowTiles][2];
+#pragma unroll
+    for (int n = 0; n < kRowTiles; ++n) {
+      const int row = row0 + n * 8 + g;
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) +
+          ((static_cast<int64_t>(walk.b) * a.new_tokens + row / group) * a.heads + head * group + row % group) * a.head_dim;
+#pragma unroll
+      for (int hf = 0; hf < kDim / 64; ++hf) {
+        uint4 v[2] = {};
+        if (row < a.rows && 4 * hf + t < pieces) {
+          v[0] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t);
+          v[1] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t + 8);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          q[n][hf][j][0] = j < 2 ? (j == 0 ? v[0].x : v[0].z) : (j == 2 ? v[1].x : v[1].z);
+          q[n][hf][j][1] = j < 2 ? (j == 0 ? v[0].y : v[0].w) : (j == 2 ? v[1].y : v[1].w);
+        }
+      }
+      float mine = 1.0f;
+      if (a.is_bf16) {
+        uint32_t top = 0;                                  // exponent of the row's largest value
+#pragma unroll
+        for (int hf = 0; hf < kDim / 64; ++hf)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t w = q[n][hf][j / 2][j % 2];
+            top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+          }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int power = top >= 0x7f80u || top == 0 ? 0 : min(126, 13 - (static_cast<int>(top >> 7) - 127));
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+        mine = 1.0f / up;
+#pragma unroll
+        for (int hf = 0; hf < kDim / 64; ++hf)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t& w = q[n][hf][j / 2][j % 2];
+            const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+            w = *reinterpret_cast<const uint32_t*>(&h);
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        factor[n][e] = a.scale * __shfl_sync(0xffffffffu, mine, (2 * t + e) * 4);
+        const int r = row0 + n * 8 + 2 * t + e, i = r / group;
+        row_end[n][e] = r < a.rows && i < span.count ? span.base + i + 1 : INT32_MIN;
+        row_begin[n][e] = a.window > 0 ? row_end[n][e] - (row_end[n][e] == INT32_MIN ? 0 : a.window) : 0;
+      }
+    }
+    // Tiles inside [all_begin, all_end) are seen by every row of the block that sees anything, tiles outside of
+    // [any_begin, any_end) by none.
+    const int first_i = min(row0 / group, span.count - 1), last_i = min((min(row0 + L::kRows, a.rows) - 1) / group, span.count - 1);
+    const int32_t all_end = span.base + first_i + 1, any_end = span.base + last_i + 1;
+    const int32_t all_begin = a.window > 0 ? any_end - a.window : 0, any_begin = a.window > 0 ? all_end - a.window : 0;
+
+    float o[kRowTiles][kDim / 16][4] = {};
+    float top[kRowTiles][2], sum[kRowTiles][2];
+#pragma unroll
+    for (int n = 0; n < kRowTiles; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
+
+    for (int32_t pos = begin + warp * kTile; pos < end; pos += kStep) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+      __syncwarp();
+      load_tile(stage == 0 ? L::kStages - 1 : stage - 1);
+      const uint8_t* keys = ring + stage * 2 * L::kTileBytes;
+      const uint8_t* values = keys + L::kTileBytes;
+      const float4 num = numbers[stage];
+      stage = stage + 1 == L::kStages ? 0 : stage + 1;
+
+      const int kr = g ^ ((g & 1) << 2);
+      float s[kRowTiles][4] = {};
+#pragma unroll
+      for (int hf = 0; hf < kDim / 64; ++hf) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(keys + PieceAt<kDim>(kr, 4 * hf + t));
+        const uint4 kb = *reinterpret_cast<const uint4*>(keys + PieceAt<kDim>(kr + 8, 4 * hf + t));
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0, a1, a2, a3;
+          Decode4<kCode>(wa[j], a0, a2);
+          Decode4<kCode>(wb[j], a1, a3);
+#pragma unroll
+          for (int n = 0; n < kRowTiles; ++n) Mma(s[n], a0, a1, a2, a3, q[n][hf][j][0], q[n][hf][j][1]);
+        }
+      }
+      const bool whole = pos >= all_begin && pos + kTile <= all_end;
+      bool move = false;
+      float high[kRowTiles][2];
+#pragma unroll
+      for (int n = 0; n < kRowTiles; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], factor[n][e % 2] * num.x, num.y);
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int32_t at = pos + kr + (e / 2) * 8;
+            if (at >= row_end[n][e % 2] || at < row_begin[n][e % 2]) s[n][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float h = fmaxf(s[n][e], s[n][e + 2]);
+          h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, 4));
+          h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, 8));
+          h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, 16));
+          high[n][e] = h;
+          move |= h > top[n][e] + (kLift + kSlack);
+        }
+      }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int n = 0; n < kRowTiles; ++n) {
+          float fade[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float next = fmaxf(top[n][e], high[n][e] - kLift);
+            fade[e] = next == -INFINITY ? 1.0f : Exp2(top[n][e] - next);
+            top[n][e] = next;
+            sum[n][e] *= fade[e];
+          }
+#pragma unroll
+          for (int mt = 0; mt < kDim / 16; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][mt][e] *= fade[e % 2];
+        }
+      }
+      uint32_t p[kRowTiles][2];
+#pragma unroll
+      for (int n = 0; n < kRowTiles; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] = Exp2(s[n][e] - (top[n][e % 2] == -INFINITY ? 0.0f : top[n][e % 2]));
+          sum[n][e % 2] = fmaf(s[n][e], num.z, sum[n][e % 2]);
+          s[n][e] *= num.w;
+        }
+        const __half2 l = __floats2half2_rn(s[n][0], s[n][1]), h = __floats2half2_rn(s[n][2], s[n][3]);
+        p[n][0] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&l));
+        p[n][1] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+      }
+      // Values: the pieces at this lane's columns of tokens 2t, 2t + 1, 2t + 8 and 2t + 9.
+      const int r0 = (2 * t) ^ 0, r1 = (2 * t + 1) ^ 4;
+      bool scalar = false;
+#pragma unroll
+      for (int part = 0; part < (kDim == 256 ? 2 : 1); ++part) {
+        constexpr int kWords = kDim == 64 ? 2 : 4;
+        uint32_t w[4][kWords];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = (r & 1 ? r1 : r0) + (r & 2 ? 8 : 0);
+          if constexpr (kDim == 64) {
+            const uint2 v = *reinterpret_cast<const uint2*>(values + PieceAt<kDim>(row, g >> 1) + (g & 1) * 8);
+            w[r][0] = v.x, w[r][1] = v.y;
+          } else {
+            const uint4 v = *reinterpret_cast<const uint4*>(values + PieceAt<kDim>(row, part * 8 + g));
+            w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
+          }
+          if (!whole) {
+            // Weight 0 does not silence a NaN: codes that no row sees are taken out, and where some rows see one that
+            // is not finite, the products of the tile are formed one by one.
+            const int32_t at = pos + row;
+            const bool unseen = at >= any_end || at < any_begin;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              if (unseen) w[r][i] = 0;
+              scalar |= NotFinite4<kCode>(w[r][i]);
+            }
+          }
+        }
+        if (!whole && all_end != any_end && __any_sync(0xffffffffu, scalar)) {
+#pragma unroll 1
+          for (int token = 0; token < kTile; ++token) {
+            const int row = token ^ ((token & 1) << 2);
+#pragma unroll
+            for (int n = 0; n < kRowTiles; ++n) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float low = __shfl_sync(0xffffffffu, s[n][e], (token & 7) * 4 + t), upper = __shfl_sync(0xffffffffu, s[n][e + 2], (token & 7) * 4 + t);
+                const float weight = token < 8 ? low : upper;
+                if (pos + row < row_end[n][e] && pos + row >= row_begin[n][e]) {
+#pragma unroll
+                  for (int m = 0; m < 2 * kWords; ++m) {
+                    const int column = Column<kDim>(g, part * 8 + m);
+                    const uint8_t* codes = values + PieceAt<kDim>(row, column / 16) + column % 16;
+                    o[n][part * 8 + m][e] += weight * Decode1<kCode>(codes[0]);
+                    o[n][part * 8 + m][e + 2] += weight * Decode1<kCode>(codes[1]);
+                  }
+                }
+              }
+            }
+          }
+          continue;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            Decode4<kCode>(__byte_perm(w[0][i], w[1][i], h == 0 ? 0x5140 : 0x7362), a0, a1);
+            Decode4<kCode>(__byte_perm(w[2][i], w[3][i], h == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+            for (int n = 0; n < kRowTiles; ++n) Mma(o[n][part * 8 + 2 * i + h], a0, a1, a2, a3, p[n][0], p[n][1]);
+          }
+        }
+      }
+    }
+
+    // ---- the piece's end: the four warps' parts become one ------------------------------------
+    __syncthreads();                                       // the previous piece has been read
+#pragma unroll
+    for (int n = 0; n < kRowTiles; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = sum[n][e];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        const int row = warp * L::kRows + n * 8 + 2 * t + e;
+        if (g == 0) {
+          exchange_max[row] = top[n][e];
+          exchange_sum[row] = v;
+        }
+#pragma unroll
+        for (int mt = 0; mt < kDim / 16; ++mt)
+          *reinterpret_cast<float2*>(exchange + row * L::kStride + Column<kDim>(g, mt)) = make_float2(o[n][mt][e], o[n][mt][e + 2]);
+      }
+    }
+    __syncthreads();
+    const bool complete = walk.offset == 0 && walk.Units() == span.units;
+    float* slot = a.work + (static_cast<int64_t>(blockIdx.x) * 2 + (walk.offset == 0 ? 1 : 0)) * L::kSlot;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < L::kRows * kDim / 4; i += kThreads) {
+      const int row = i / (kDim / 4), d = i % (kDim / 4) * 4;
+      float m = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, exchange_max[w * L::kRows + row]);
+      float4 y = {};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = exchange_max[w * L::kRows + row], fade = mw == -INFINITY ? 0.0f : Exp2(mw - m);
+        // A part with no score is left out rather than multiplied by 0 -- its sum may hold the NaN of a row that has one.
+        if (fade == 0.0f && exchange_sum[w * L::kRows + row] == 0.0f) continue;
+        const float4 v = *reinterpret_cast<const float4*>(exchange + (w * L::kRows + row) * L::kStride + d);
+        total = fmaf(exchange_sum[w * L::kRows + row], fade, total);
+        y.x = fmaf(v.x, fade, y.x), y.y = fmaf(v.y, fade, y.y), y.z = fmaf(v.z, fade, y.z), y.w = fmaf(v.w, fade, y.w);
+      }
+      if (complete) {
+        if (row0 + row < a.rows) StoreRow(a, walk.b, head, row0 + row, span.count, d, y, m, total);
+      } else {
+        *reinterpret_cast<float4*>(slot + row * kDim + d) = y;
+        if (d == 0) {
+          slot[L::kRows * kDim + row] = m;
+          slot[L::kRows * kDim + L::kRows + row] = total;
+        }
+      }
+    }
+  }
+}
+
+// Joins the pieces of the item that the end of CTA blockIdx.x's share cuts first: maximum over the pieces, then the
+// pieces' sums and values times exp2(their maximum - it), in the order of the pieces.
+constexpr int kJoinThreads = 512;
+
+template <int kDim, int kRowTiles>
+__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const AttentionArgs a) {
+  using L = Layout<kDim, kRowTiles>;
+  constexpr int kParts = kJoinThreads / 32 / L::kRows;      // warps of a row
+  constexpr int kVectors = kDim == 256 ? 2 : 1;             // of four columns, per lane
+  __shared__ float4 part_values[kParts][L::kRows][kDim / 4];
+  __shared__ float part_sum[kParts][L::kRows];
+  if (threadIdx.x == 0) griddep_launch_dependents();
+  griddep_wait();
+  const int c = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = warp % L::kRows, part = warp / L::kRows;
+  const Share at = Locate<kJoinThreads>(a, c, true);
+  if (at.left == 0) return;
+  const Span span = SpanOf(a, at.b);
+  const int64_t first = at.begin + at.left - 1 - at.offset;              // the item's first unit
+  if (at.offset + 1 == span.units || first < at.begin) return;
+  const int last_cta = static_cast<int>(((first + span.units) * at.ctas - 1) / at.total);
+  const int pieces = last_cta - c + 1;
+  auto slot_of = [&](int p) { return a.work + (static_cast<int64_t>(c + p) * 2 + (p == 0 ? 1 : 0)) * L::kSlot; };
+  float m = -INFINITY;
+  for (int p = lane; p < pieces; p += 32) m = fmaxf(m, slot_of(p)[L::kRows * kDim + row]);
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float total = 0.0f;
+  float4 y[kVectors] = {};
+  const bool mine = lane * 4 < kDim;
+#pragma unroll 4
+  for (int p = part; p < pieces; p += kParts) {
+    const float* slot = slot_of(p);
+    const float mp = slot[L::kRows * kDim + row], sp = slot[L::kRows * kDim + L::kRows + row];
+    float4 v[kVectors] = {};
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (mine) v[i] = *reinterpret_cast<const float4*>(slot + row * kDim + i * 128 + lane * 4);
+    const float fade = mp == -INFINITY ? 0.0f : Exp2(mp - m);
+    total = fmaf(sp, fade, total);
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) y[i].x = fmaf(v[i].x, fade, y[i].x), y[i].y = fmaf(v[i].y, fade, y[i].y), y[i].z = fmaf(v[i].z, fade, y[i].z), y[i].w = fmaf(v[i].w, fade, y[i].w);
+  }
+  if (part > 0) {
+    if (lane == 0) part_sum[part][row] = total;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (mine) part_values[part][row][i * 32 + lane] = y[i];
+  }
+  __syncthreads();
+  const int item_row = (at.item % a.blocks) * L::kRows + row;
+  if (part > 0 || item_row >= a.rows) return;
+  for (int p = 1; p < kParts; ++p) {
+    total += part_sum[p][row];
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (mine) {
+        const float4 v = part_values[p][row][i * 32 + lane];
+        y[i].x += v.x, y[i].y += v.y, y[i].z += v.z, y[i].w += v.w;
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+    if (mine) StoreRow(a, at.b, at.item / a.blocks, item_row, span.count, i * 128 + lane * 4, y[i], m, total);
+}
+
+struct Variant {
+  void (*main)(AttentionArgs);
+  void (*join)(AttentionArgs);
+  int dim, row_tiles, bytes, slot;
+};
+template <int kCode, int kDim, int kRowTiles>
+constexpr Variant MakeVariant() {
+  using L = Layout<kDim, kRowTiles>;
+  return {kv_attention_kernel<kCode, kDim, kRowTiles>, kv_attention_join_kernel<kDim, kRowTiles>, kDim, kRowTiles, L::kBytes, L::kSlot};
+}
+// Per cache type: heads up to 64, 128 and 256 wide, 8 or 16 rows at a time.  16 rows of 256 columns do not fit the registers.
+constexpr int kShapes = 5;
+#define B200SD_ATTENTION_VARIANTS(code) MakeVariant<code, 64, 1>(), MakeVariant<code, 64, 2>(), MakeVariant<code, 128, 1>(), MakeVariant<code, 128, 2>(), MakeVariant<code, 256, 1>()
+const Variant kVariants[3][kShapes] = {{B200SD_ATTENTION_VARIANTS(kF8E4M3FN)}, {B200SD_ATTENTION_VARIANTS(kF8E5M2)}, {B200SD_ATTENTION_VARIANTS(kS8)}};
+#undef B200SD_ATTENTION_VARIANTS
+int g_ctas_per_sm[3][kShapes];                  // the same on every B200; set by InitAttentionKernels
+
+int ShapeIndex(int64_t head_dim, int64_t rows) {
+  if (head_dim > 128) return 4;
+  return (head_dim > 64 ? 2 : 0) + (rows > 8 ? 1 : 0);
 }
 
 }  // namespace
+
+Status InitAttentionKernels() {
+  for (int c = 0; c < 3; ++c)
+    for (int s = 0; s < kShapes; ++s) {
+      const Variant& v = kVariants[c][s];
+      cudaError_t e = cudaFuncSetAttribute(v.main, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes);
+      int n = 0;
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, v.main, kThreads, v.bytes);
+      if (e != cudaSuccess) return Status::Error(kInternal, std::string("kv_attention_kernel set-up: ") + cudaGetErrorString(e));
+      g_ctas_per_sm[c][s] = n > 0 ? n : 1;
+    }
+  return Status::Ok();
+}
 
 Status ValidatePagedAttention(const B200SD_PagedAttention& a, bool check_pointers) {
   auto bad = [](const std::string& m) { return Status::Error(kInvalidArgument, m); };
@@ -107,21 +736,52 @@ Status ValidatePagedAttention(const B200SD_PagedAttention& a, bool check_pointer
 }
 
 size_t PagedAttentionWorkspaceBytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-  if (batch < 1 || new_tokens < 1 || kv_heads < 1 || heads < kv_heads || head_dim < 16) return 0;
-  return 16;
+  if (batch < 1 || new_tokens < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || head_dim < 16 || head_dim > 256) return 0;
+  const Variant& v = kVariants[0][ShapeIndex(head_dim, new_tokens * (heads / kv_heads))];
+  return static_cast<size_t>(kMaxCtas) * 2 * v.slot * sizeof(float);
 }
 
 Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream, LaunchStats* stats) {
   if (a.batch == 0 || a.new_tokens == 0) return Status::Ok();
-  const AttentionArgs args{a.q, static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages), a.k_scale, a.v_scale,
-                           a.page_table, a.seq_lens, a.new_lens, a.out, a.lse,
-                           static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
-                           static_cast<int32_t>(a.head_dim), static_cast<int32_t>(a.page_tokens),
-                           a.num_pages, a.table_width, a.window, a.softmax_scale, a.q_dtype == kBF16, a.cache_dtype, StatusWordPtr()};
-  kv_attention_kernel<<<dim3(static_cast<unsigned>(a.heads), static_cast<unsigned>(a.new_tokens), static_cast<unsigned>(a.batch)), 32, 0, stream>>>(args);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return Status::Error(kInternal, std::string("kv_attention_kernel launch: ") + cudaGetErrorString(e));
+  const int code = a.cache_dtype == kF8E4M3FN ? 0 : a.cache_dtype == kF8E5M2 ? 1 : 2;
+  const int64_t rows = a.new_tokens * (a.heads / a.kv_heads);
+  const int shape = ShapeIndex(a.head_dim, rows);
+  const Variant& v = kVariants[code][shape];
+  const int64_t block = 8 * v.row_tiles, blocks = (rows + block - 1) / block;
+  int shift = 4;
+  while ((1 << shift) < a.page_tokens) ++shift;
+  const int64_t capacity = a.table_width * a.page_tokens;
+  // A sequence that the table cannot make longer than this is not cut: the second kernel would cost more than it saves.
+  const bool cut = capacity > 512;
+  AttentionArgs args{a.q, static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages), a.k_scale, a.v_scale,
+                     a.page_table, a.seq_lens, a.new_lens, a.out, a.lse, static_cast<float*>(a.workspace),
+                     static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
+                     static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
+                     static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
+                     cut ? kStep : 1 << 30, cut ? 4 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
+  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + kStep - 1) / kStep : 1);
+  int64_t grid = static_cast<int64_t>(DeviceSmCount()) * g_ctas_per_sm[code][shape];
+  grid = grid < kMaxCtas ? grid : kMaxCtas;
+  grid = grid < most ? grid : most;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // see griddep_wait() in the kernels
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = v.bytes;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, v.main, args);
   stats->launches = 1;
+  if (e == cudaSuccess && cut) {
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, v.join, args);
+    stats->launches = 2;
+  }
+  if (e != cudaSuccess) return Status::Error(kInternal, std::string("kv_attention_kernel launch: ") + cudaGetErrorString(e));
   return Status::Ok();
 }
 
