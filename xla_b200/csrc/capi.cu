@@ -26,6 +26,7 @@ Status InitDenseKernels();
 Status InitSkinnyKernels();
 Status InitMxKernels();
 Status InitAttentionKernels();
+Status InitW4Kernels();
 
 namespace {
 
@@ -91,6 +92,7 @@ Status InitDevice(int device) {
     if (st.init_status.ok()) st.init_status = InitSkinnyKernels();
     if (st.init_status.ok()) st.init_status = InitMxKernels();
     if (st.init_status.ok()) st.init_status = InitAttentionKernels();
+    if (st.init_status.ok()) st.init_status = InitW4Kernels();
     // A persisted tuning result named by the environment is loaded with the first device (a file
     // that cannot be read or parsed makes the first call fail loudly instead of being ignored).
     static std::once_flag table_once;
