@@ -5,14 +5,22 @@
 //
 // Products run on mma.m16n8k16 with 16 weight rows on the large side and 8 rows of x on the other: A is the weights as
 // they lie in memory, B is x.  The order along k inside a product is free, so a lane feeds two products from one
-// 32-bit word of 8 weights: the pairs (i, i + 4) of its nibbles are one mask away from being f16 or bf16 numbers with a
-// constant offset (1024 + w, 128 + w), and one subtraction takes the offset and the zero point away -- exactly, the
-// operands are the integers w - z.  x is paired the same way.  A lane's word, half or whole 16-byte piece is chosen so
-// that one product never mixes two groups; a group's f32 sum is multiplied by its scale in f32 and added up.
+// 32-bit word of 8 weights, in the pairs (0, 4), (1, 5), (2, 6), (3, 7) of its nibbles, and x is paired the same way.  A
+// lane's word, half or whole 16-byte piece is chosen so that one product never mixes two groups; a group's f32 sum is
+// multiplied by its scale in f32 and added up.
 //
-// A CTA owns n / CTAs consecutive rows, whole rows of bytes with none read twice or by two CTAs whatever n is; its warps
-// split k among them in steps of 128 (and, where k is short, also the rows), each with its own cp.async ring for its
-// weights and the matching part of x, and add their sums through shared memory once per block of rows, in a fixed order.
+// Where x fits shared memory beside the rings it is put there once, paired, as f16 whatever its type, each row multiplied
+// by the power of two that brings its largest value to 2^13 (what lies 2^23 below that is rounded, to 2^-34 of it).  A
+// nibble under a mask then is an f16 operand as it stands: the subnormal n * 2^-24, or 16 n * 2^-24 for the nibbles one
+// place higher, whose x is stored divided by 16.  That is 5 instructions for 8 weights; the zero point (8 for two's
+// complement) is taken off a group's sum as z times the sum of x over the group, which is formed once in f32.  The sum
+// before that is not much larger than after, so this costs at most a few bits of f32's 24.
+// Otherwise x comes through the rings with the weights and the products have x's type: a masked nibble plus an offset is
+// an f16 or bf16 number (1024 + n, 128 + n), and one subtraction leaves w - z, exactly; 9 and 11 instructions for 8.
+//
+// A CTA owns n / CTAs consecutive rows, whole rows of bytes with none read twice or by two CTAs whatever n is.  A block of
+// its rows and 128 of k are a unit; the warps take the units in turn, each through its own cp.async ring, and leave their
+// sums of each block in shared memory, where they are added in the order of the warps, as many blocks at a time as fit.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,60 +44,99 @@ struct W4Args {
   int32_t m, n, k, groups;
   int32_t group_shift;                          // log2 of the 128-blocks of k in a group (groups of 128 and more) ...
   int32_t blocks_per_group;                     // ... or their number where it is no power of two
-  int32_t k_warps;                              // warps that share a block of rows
-  int32_t scale_dtype, bias_dtype, d_dtype, is_signed;
+  int32_t rows, rows_left;                      // of a CTA: `rows`, and one more for the first `rows_left`
+  int32_t steps, per_round;                     // 128-blocks of k; blocks of rows whose sums fit shared memory
+  uint32_t piece_inverse;                       // 2^32 / (16 * steps), rounded up
+  int32_t x_is_bf16, scale_dtype, bias_dtype, d_dtype, is_signed;
 };
 
-__device__ __forceinline__ float ScaleValue(uint32_t raw, int32_t dtype) {
-  if (dtype == kBF16) return __uint_as_float(raw << 16);
-  if (dtype == kF16) return __half2float(__ushort_as_half(static_cast<unsigned short>(raw)));
-  return __uint_as_float(raw);
+// Scales and bias: their bits, loaded ahead, and what they stand for.  kType 0 takes the type from the arguments.
+template <int kType>
+__device__ __forceinline__ uint32_t LoadBits(const void* p, int64_t i, int32_t dtype) {
+  if (kType == kF32 || (kType == 0 && dtype == kF32)) return static_cast<const uint32_t*>(p)[i];
+  return static_cast<const uint16_t*>(p)[i];
 }
-__device__ __forceinline__ uint32_t LoadRaw(const void* p, int64_t i, int32_t dtype) {
-  if (dtype == kF32) return __ldg(static_cast<const uint32_t*>(p) + i);
-  return __ldg(static_cast<const unsigned short*>(p) + i);
+template <int kType>
+__device__ __forceinline__ float ValueOf(uint32_t bits, int32_t dtype) {
+  if (kType == kF32 || (kType == 0 && dtype == kF32)) return __uint_as_float(bits);
+  if (kType == kBF16 || (kType == 0 && dtype == kBF16)) return __uint_as_float(bits << 16);
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
-__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void CopyAsync16If(bool wanted, uint32_t dst, const void* src) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"(static_cast<int>(wanted)) : "memory");
+}
+// Loads that stay whole (a compiler short of registers takes a vector apart), from addresses that stay in registers.
+__device__ __forceinline__ uint4 LoadShared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void StoreShared16(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint2 LoadShared8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t LoadShared4(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t Kept(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+__device__ __forceinline__ void CopyAsync16OrZero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// (w & mask) ^ magic in one instruction; written out because the compiler splits it where a part of `magic` is not constant.
+__device__ __forceinline__ uint32_t MaskXor(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(v) : "r"(w), "r"(mask), "r"(magic));
+  return v;
 }
 
-// What turns masked nibbles into operands: offset + zero point of one weight row and group, for both halves.
-template <typename T> struct Offsets;
-template <> struct Offsets<__half> {
-  __half2 low, high;
-  __device__ explicit Offsets(int z) {
-    low = __half2half2(__int2half_rn(-1024 - z));
-    high = __half2half2(__int2half_rn(-64 - z));
+// How a word's nibbles become operands.  Subnormal: as they are, see above; `flip` (8 for two's complement) turns -8 .. 7
+// into 0 .. 15 with zero point 8.
+struct Subnormal {
+  using Operand = __half;
+  __device__ void Set(uint32_t) {}
+  __device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, uint32_t (&v)[4]) const {
+    v[0] = MaskXor(w, 0x000f000fu, flip), v[1] = MaskXor(w, 0x00f000f0u, flip << 4);
+    v[2] = MaskXor(w >> 8, 0x000f000fu, flip), v[3] = MaskXor(w >> 8, 0x00f000f0u, flip << 4);
   }
 };
-template <> struct Offsets<__nv_bfloat16> {
-  __nv_bfloat162 low;
-  __device__ explicit Offsets(int z) { low = __bfloat162bfloat162(__int2bfloat16_rn(-128 - z)); }
-};
-
-// The pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's nibbles, w - z each; `flip` is 8 for two's complement.
-__device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, const Offsets<__half>& o, uint32_t (&v)[4]) {
-  const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
-  const uint32_t low = 0x64006400u | flip, high = 0x64006400u | flip << 4;
+// w - z exactly.  The offsets -(1024 + z), -(64 + z) and -(128 + z) of one weight row and group have z in their low bits,
+// so they are put together, not converted.
+template <typename T> struct Offset;
+template <> struct Offset<__half> {
+  using Operand = __half;
+  uint32_t low, high;
+  __device__ void Set(uint32_t z) { low = 0xe400e400u | z * 0x00010001u, high = 0xd400d400u | z * 0x00100010u; }
+  __device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, uint32_t (&v)[4]) const {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t shifted = w >> (8 * i);
-    const uint32_t a = (shifted & 0x000f000fu) ^ low, b = (shifted & 0x00f000f0u) ^ high;       // 1024 + n, 1024 + 16 n
-    const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&a), o.low);
-    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, o.high);
-    v[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
-    v[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t a = MaskXor(w >> (8 * i), 0x000f000fu, 0x64006400u ^ flip);                  // 1024 + n
+      const uint32_t b = MaskXor(w >> (8 * i), 0x00f000f0u, 0x64006400u ^ flip << 4);             // 1024 + 16 n
+      asm("add.f16x2 %0, %1, %2;" : "=r"(v[2 * i]) : "r"(a), "r"(low));
+      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[2 * i + 1]) : "r"(b), "r"(0x2c002c00u), "r"(high));   // times 1 / 16
+    }
   }
-}
-__device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, const Offsets<__nv_bfloat16>& o, uint32_t (&v)[4]) {
-  const uint32_t low = 0x43004300u | flip;
+};
+template <> struct Offset<__nv_bfloat16> {
+  using Operand = __nv_bfloat16;
+  uint32_t low;
+  __device__ void Set(uint32_t z) { low = 0xc300c300u | z * 0x00010001u; }
+  __device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, uint32_t (&v)[4]) const {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t a = ((w >> (4 * i)) & 0x000f000fu) ^ low;                                    // 128 + n
-    const __nv_bfloat162 x = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), o.low);
-    v[i] = *reinterpret_cast<const uint32_t*>(&x);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = MaskXor(w >> (4 * i), 0x000f000fu, 0x43004300u ^ flip);                  // 128 + n
+      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v[i]) : "r"(a), "r"(0x3f803f80u), "r"(low));     // times 1
+    }
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -101,18 +148,25 @@ __device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// kGroup: 32, 64 or 128 (which stands for its multiples too); kTiles: weight row tiles of 16 of a warp; kCols: tiles of 8
-// rows of x.
-template <int kTiles_, int kCols_, int kWarps_, int kStages_>
+// Weight row tiles of 16 of a unit, tiles of 8 rows of x, warps of a CTA, stages of a ring; T is the type of x in the
+// rings, void where x is resident.
+template <int kTiles_, int kCols_, int kWarps_, int kStages_, typename T_>
 struct Shape {
+  using T = T_;
   static constexpr int kTiles = kTiles_, kCols = kCols_, kWarps = kWarps_, kStages = kStages_;
-  static constexpr int kRows = 16 * kTiles;                 // weight rows of a warp's block
+  static constexpr bool kResident = std::is_void_v<T>;
+  static constexpr int kRows = 16 * kTiles;                 // weight rows of a unit
   static constexpr int kStride = kRows + 4;                 // floats between two rows of x in the sums
-  static constexpr int kSums = kWarps * 8 * kCols * kStride * 4;
-  static int Bytes(int m) { return kSums + kWarps * kStages * (kTiles * 1024 + m * 256); }
+  static constexpr int kSums = kWarps * 8 * kCols * kStride;            // floats: one block for the most rows of x, more for fewer
+  static constexpr int kFactors = 16 * kCols;               // floats: the inverse of each resident row's power of two, its largest value
+  static int64_t Bytes(int64_t m, int64_t steps, int64_t group) {
+    const int64_t ring = kWarps * kStages * (kTiles * 1024 + (kResident ? 0 : m * 256));
+    const int64_t resident = kResident ? steps * m * 256 + steps * (128 / group) * ((m + 1) / 2 * 2) * 4 : 0;
+    return (kSums + kFactors) * 4 + ring + resident;
+  }
 };
 
-// Where 16-byte piece `c` of weight row `r` (64 bytes of a step) and piece `c` of row `r` of x (256 bytes) lie: so that the
+// Where 16-byte piece `c` of weight row `r` (64 bytes of a unit) and piece `c` of row `r` of x (256 bytes) lie: so that the
 // reads below have no bank conflicts.
 __device__ __forceinline__ int WeightPiece(int r, int c) { return r * 64 + (c ^ ((r & 2) | ((r >> 2) & 1))) * 16; }
 template <int kGroup>
@@ -121,235 +175,429 @@ __device__ __forceinline__ int InputPiece(int r, int c) {
   return r * 256 + (at ^ ((r & 1) << 2)) * 16;
 }
 
-template <typename T, int kGroup, typename S>
-__global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const W4Args a) {
+// Eight values of x in the order of the weights' pairs.
+__device__ __forceinline__ uint4 Paired(uint4 v) {
+  return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+}
+
+// The two values of a word of x, in f32.
+__device__ __forceinline__ float2 Unpack(uint32_t w, bool is_bf16) {
+  if (is_bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// All of x to shared memory: `inputs` as paired, scaled f16, `factors` the inverse powers of two (0 for a row that is not
+// finite), `sums` [group][row] the sums of the scaled values over each group (each 128 of k for groups longer than that).
+// The copies are under way before the weights', so that they do not queue behind them; a thread works on the pieces that
+// it has copied itself, in place.  The loops are not unrolled: this code runs once, and its instructions are fetched cold.
+template <int kGroup, int kThreads>
+struct Staging {
+  const W4Args& a;
+  int all, total;                               // pieces of 16 bytes of a row, with its padding to whole steps, and of all rows
+  uint32_t inverse, inputs;
+  __device__ Staging(const W4Args& args, uint32_t to) : a(args), all(args.steps * 16), total(all * args.m), inverse(args.piece_inverse), inputs(to) {}
+  __device__ __forceinline__ void Place(int i, int& r, int& c, uint32_t& at) const {
+    r = all == total ? 0 : static_cast<int>(__umulhi(i, inverse));       // i / all, for i < total and total * all < 2^32
+    c = i - r * all;
+    at = inputs + (c / 16 * a.m) * 256 + InputPiece<kGroup>(r, c % 16);
+  }
+  __device__ __forceinline__ void Copy() const {
+    int r, c;
+    uint32_t at;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      Place(i, r, c, at);
+      const bool there = c < a.k / 8;
+      CopyAsync16OrZero(at, there ? static_cast<const uint16_t*>(a.x) + (r * a.k + c * 8) : a.x, there);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // `top` [row] holds zeros on entry.
+  __device__ __forceinline__ void Convert(float* factors, uint32_t* top, float* sums) const {
+    const uint32_t lanes = threadIdx.x % 32 < 16 ? 0x0000ffffu : 0xffff0000u;       // 16 lanes in a row share r and the step
+    const int columns = (a.m + 1) / 2 * 2;
+    int r, c;
+    uint32_t at;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      Place(i, r, c, at);
+      const uint4 v = LoadShared16(at);
+      const uint32_t both = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+      const uint32_t most = __reduce_max_sync(lanes, max(both & 0xffffu, both >> 16));
+      if (threadIdx.x % 16 == 0 && most > 0) atomicMax(top + r, __float_as_uint(Unpack(most, a.x_is_bf16).x));
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      Place(i, r, c, at);
+      const uint4 v = LoadShared16(at);
+      const uint32_t bits = top[r];
+      const int power = bits >= 0x7f800000u || bits == 0 ? 0 : min(126, 13 - (static_cast<int>(bits >> 23) - 127));
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23), up16 = up * 0.0625f;
+      const float2 x01 = Unpack(v.x, a.x_is_bf16), x23 = Unpack(v.y, a.x_is_bf16), x45 = Unpack(v.z, a.x_is_bf16), x67 = Unpack(v.w, a.x_is_bf16);
+      const __half2 p0 = __floats2half2_rn(x01.x * up, x45.x * up), p1 = __floats2half2_rn(x01.y * up16, x45.y * up16);
+      const __half2 p2 = __floats2half2_rn(x23.x * up, x67.x * up), p3 = __floats2half2_rn(x23.y * up16, x67.y * up16);
+      StoreShared16(at, make_uint4(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1), *reinterpret_cast<const uint32_t*>(&p2), *reinterpret_cast<const uint32_t*>(&p3)));
+      const float2 f0 = __half22float2(p0), f1 = __half22float2(p1), f2 = __half22float2(p2), f3 = __half22float2(p3);
+      float sum = ((f0.x + f0.y) + (f2.x + f2.y)) + 16.0f * ((f1.x + f1.y) + (f3.x + f3.y));
+#pragma unroll
+      for (int o = kGroup / 16; o > 0; o /= 2) sum += __shfl_xor_sync(lanes, sum, o);
+      if (c % (kGroup / 8) == 0) sums[c / (kGroup / 8) * columns + r] = sum;
+      if (c == 0) factors[r] = bits >= 0x7f800000u ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
+    }
+    __syncthreads();
+  }
+};
+
+// One result from its definition, for a row of x with an infinity or a NaN: there the sums above would take one from another.
+__device__ __noinline__ float PlainDot(const W4Args& a, int x_row, int row) {
+  float y = 0.0f;
+  const int group = a.k / a.groups;
+  for (int k = 0; k < a.k; ++k) {
+    const int64_t at = static_cast<int64_t>(row) * a.groups + k / group;
+    const int n = a.w[static_cast<int64_t>(row) * (a.k / 2) + k / 2] >> (k % 2 * 4) & 15;
+    const int w = a.is_signed ? (n ^ 8) - 8 : n - (a.zero[at] & 15);
+    const uint32_t raw = static_cast<const uint16_t*>(a.x)[static_cast<int64_t>(x_row) * a.k + k];
+    y += static_cast<float>(w) * Unpack(raw, a.x_is_bf16).x * ValueOf<0>(LoadBits<0>(a.scale, at, a.scale_dtype), a.scale_dtype);
+  }
+  return y;
+}
+
+// kGroup: 32, 64 or 128 (which stands for its multiples too).  kScale: the scales' type, kSign: 1 for two's complement, 0
+// for zero points; ring variants have 0 and 2 there and go by the arguments.
+template <int kGroup, int kScale, int kSign, typename S>
+__global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
+  using Decoder = std::conditional_t<S::kResident, Subnormal, Offset<std::conditional_t<S::kResident, __half, typename S::T>>>;
+  using Operand = typename Decoder::Operand;
   constexpr int kPerStep = 128 / kGroup;                    // groups of a step
   constexpr int kWords = kGroup / 32;                       // words of a lane in a group
+  constexpr int kTiles = S::kTiles, kCols = S::kCols, kWarps = S::kWarps;
+  const bool is_signed = kSign == 2 ? a.is_signed != 0 : kSign == 1;
   extern __shared__ __align__(128) uint8_t smem[];
   if (threadIdx.x == 0) griddep_launch_dependents();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int wk = warp % a.k_warps, wn = warp / a.k_warps, row_step = S::kRows * (S::kWarps / a.k_warps);
-  const int first = static_cast<int>(static_cast<int64_t>(blockIdx.x) * a.n / gridDim.x);
-  const int last = static_cast<int>(static_cast<int64_t>(blockIdx.x + 1) * a.n / gridDim.x);
-  const int steps = (a.k + 127) / 128, row_bytes = a.k / 2;
-  const int stage_bytes = S::kTiles * 1024 + a.m * 256;
+  const int cta = blockIdx.x, first = cta * a.rows + min(cta, a.rows_left), last = first + a.rows + (cta < a.rows_left ? 1 : 0);
+  const int steps = a.steps, row_bytes = a.k / 2, blocks = (last - first + S::kRows - 1) / S::kRows, per_round = a.per_round;
+  const int stage_bytes = kTiles * 1024 + (S::kResident ? 0 : a.m * 256);
   float* sums = reinterpret_cast<float*>(smem);
-  uint8_t* ring = smem + S::kSums + warp * S::kStages * stage_bytes;
-  const uint32_t flip = a.is_signed ? 0x00080008u : 0u;
+  float* factors = sums + S::kSums;
+  uint8_t* ring = smem + (S::kSums + S::kFactors) * 4 + warp * S::kStages * stage_bytes;
+  uint8_t* resident = smem + (S::kSums + S::kFactors) * 4 + kWarps * S::kStages * stage_bytes;
+  float* group_sums = reinterpret_cast<float*>(resident + steps * a.m * 256);
+  const int columns = (a.m + 1) / 2 * 2;
+  const uint32_t flip = is_signed ? 0x00080008u : 0u;
+  // A CTA's rows of the weights and of the scales span less than 4 GiB, so 32-bit offsets from its first row do.
+  const uint8_t* w_base = a.w + static_cast<int64_t>(first) * row_bytes;
+  const uint8_t* scale_base = static_cast<const uint8_t*>(a.scale) + static_cast<int64_t>(first) * a.groups * ((kScale == 0 ? a.scale_dtype : kScale) == kF32 ? 4 : 2);
+  const uint8_t* zero_base = a.zero + static_cast<int64_t>(first) * a.groups;
 
-  int load_row = first + wn * S::kRows, load_step = wk;
-  auto load = [&](int stage) {
-    if (load_row < last && load_step < steps) {
-      const uint32_t dst = smem_u32(ring + stage * stage_bytes);
+  // A warp's units of a round of blocks are the warp-th, the (warp + warps)-th ... of the line (block, step): within a block
+  // every kWarps-th step, and what is left over carries into the next block.
+  //
+  // Loading: each lane brings piece `t` of rows g, g + 8, ... of a unit.  What lies behind the last row or the end of k is
+  // not loaded: old bytes there are finite weights too, of rows that are not stored or against a 0 of x.
+  const uint32_t eight_rows = 8 * row_bytes, next_block = S::kRows * row_bytes - steps * 64;
+  int load_step = warp, load_block = 0, load_round = per_round, load_rows = last - first - g;
+  uint32_t load_from = static_cast<uint32_t>(g) * row_bytes + warp * 64 + t * 16, load_to = Kept(smem_u32(ring) + WeightPiece(g, t));
+  auto to_next_block = [&] {
+    while (load_step >= steps && load_block < blocks) {
+      ++load_block;
+      load_rows -= S::kRows;
+      load_step -= steps;
+      load_from += next_block;
+      if (load_block == load_round) {                       // every round starts with the warp-th unit
+        load_round += per_round;
+        load_from += (warp - load_step) * 64;
+        load_step = warp;
+      }
+    }
+  };
+  if (load_step >= steps) to_next_block();
+  auto load = [&](uint32_t stage) {                         // `stage`: its place in the ring, in bytes
+    if (load_block < blocks) {
+      const uint32_t dst = load_to + stage;
+      const int rows = load_step * 64 + t * 16 < row_bytes ? load_rows : 0;
 #pragma unroll
-      for (int i = 0; i < 2 * S::kTiles; ++i) {
-        const int piece = i * 32 + lane, r = piece / 4, c = piece % 4, at = load_step * 64 + c * 16;
-        const bool in = load_row + r < last && at < row_bytes;
-        CopyAsync16(dst + WeightPiece(r, c), in ? a.w + static_cast<int64_t>(load_row + r) * row_bytes + at : a.w, in ? 16 : 0);
+      for (int i = 0; i < 2 * kTiles; ++i)
+        CopyAsync16If(8 * i < rows, dst + i * 512, w_base + (load_from + i * eight_rows));
+      if constexpr (!S::kResident) {
+#pragma unroll
+        for (int i = 0; i < 4 * kCols; ++i) {
+          const int r = i * 2 + lane / 16, c = lane % 16, at = load_step * 128 + c * 8;
+          if (r < a.m)
+            CopyAsync16OrZero(smem_u32(ring) + stage + kTiles * 1024 + InputPiece<kGroup>(r, c), at < a.k ? static_cast<const uint16_t*>(a.x) + (r * a.k + at) : a.x, at < a.k);
+        }
       }
-      for (int piece = lane; piece < a.m * 16; piece += 32) {
-        const int r = piece / 16, c = piece % 16, at = load_step * 128 + c * 8;
-        const bool in = at < a.k;
-        CopyAsync16(dst + S::kTiles * 1024 + InputPiece<kGroup>(r, c), in ? static_cast<const T*>(a.x) + static_cast<int64_t>(r) * a.k + at : a.x, in ? 16 : 0);
-      }
-      load_step += a.k_warps;
-      if (load_step >= steps) {
-        load_step = wk;
-        load_row += row_step;
-      }
+      load_step += kWarps;
+      load_from += kWarps * 64;
+      if (load_step >= steps) to_next_block();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // Scales (as they are stored) and zero points of a step for this lane's rows; with several groups in a step the four lanes
-  // of a row hold one each.
-  auto load_scales = [&](int row, int step, uint32_t (&scale)[S::kTiles][2], int (&zero)[S::kTiles][2]) {
-    const int group = kGroup == 128 ? (a.group_shift >= 0 ? step >> a.group_shift : step / a.blocks_per_group) : step * kPerStep + t;
+  // Scales and zero points of a unit for this lane's rows; with several groups in a step the four lanes of a row hold one
+  // each.  Rows behind the last take its numbers, groups behind the end of k a scale of 0.  They are loaded a unit ahead,
+  // into the registers that the unit before has just used; in front of a block, its first unit's.
+  uint32_t scale[kTiles][2], zero[kTiles][2], row_at[kTiles][2];
+  auto load_numbers = [&](int step) {
+    const uint32_t group = kGroup == 128 ? (a.group_shift >= 0 ? step >> a.group_shift : step / a.blocks_per_group) : step * kPerStep + t % kPerStep;
+    const bool there = kGroup == 128 || group < a.groups;
 #pragma unroll
-    for (int r = 0; r < S::kTiles; ++r)
+    for (int r = 0; r < kTiles; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int at = row + r * 16 + h * 8 + g;
-        scale[r][h] = 0;
-        zero[r][h] = 8;
-        if (at < last && step < steps && group < a.groups && (kGroup == 128 || t < kPerStep)) {
-          const int64_t i = static_cast<int64_t>(at) * a.groups + group;
-          scale[r][h] = LoadRaw(a.scale, i, a.scale_dtype);
-          if (!a.is_signed) zero[r][h] = __ldg(a.zero + i) & 15;
-        }
+        const uint32_t at = row_at[r][h] + (there ? group : 0);
+        scale[r][h] = LoadBits<kScale>(scale_base, at, a.scale_dtype);
+        if (!there) scale[r][h] = 0;
+        if (!is_signed) zero[r][h] = zero_base[at] & 15u;
+        else if (!S::kResident) zero[r][h] = 8;
       }
   };
-
-  griddep_wait();
+  auto set_rows = [&](int block) {
+    const int row = min(block, blocks - 1) * S::kRows + g, most = last - first - 1;
 #pragma unroll
-  for (int s = 0; s < S::kStages - 1; ++s) load(s);
-  uint32_t next_scale[S::kTiles][2];
-  int next_zero[S::kTiles][2];
-  load_scales(first + wn * S::kRows, wk, next_scale, next_zero);
+    for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(row + r * 16 + h * 8, most)) * a.groups;
+  };
 
-  int stage = 0;
-  for (int block = first; block < last; block += row_step) {
-    const int row = block + wn * S::kRows;
-    float acc[S::kTiles][S::kCols][4] = {};
-    if (row < last) {
-      for (int step = wk; step < steps; step += a.k_warps) {
+  uint32_t* top = reinterpret_cast<uint32_t*>(factors + 8 * kCols);
+  if (S::kResident && threadIdx.x < 8 * kCols) top[threadIdx.x] = 0;
+  __syncthreads();
+  griddep_wait();
+  const Staging<kGroup, kWarps * 32> staging(a, smem_u32(resident));
+  if constexpr (S::kResident) staging.Copy();
+#pragma unroll 1
+  for (int s = 0; s < S::kStages - 1; ++s) load(s * stage_bytes);
+  set_rows(0);
+  load_numbers(min(warp, steps - 1));
+  if constexpr (S::kResident) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");       // this thread's part of x has come
+    staging.Convert(factors, top, group_sums);
+  }
+
+  // Places of this lane's words and of its pieces of x, of the sums that belong to them; behind the last row of x any will
+  // do, its column is not stored.
+  uint32_t weight_at[kPerStep], input_at[kCols][4], sums_at[kCols];
+#pragma unroll
+  for (int i = 0; i < kPerStep; ++i)
+    weight_at[i] = Kept(smem_u32(ring) + (kGroup == 128 ? WeightPiece(g, t) : kGroup == 64 ? WeightPiece(g, i * 2 + t / 2) + t % 2 * 8 : WeightPiece(g, i) + t * 4));
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? i / 2 * 8 + t * 2 + i % 2 : i * 4 + t;
+      input_at[c][i] = Kept((S::kResident ? smem_u32(resident) : smem_u32(ring) + kTiles * 1024) + InputPiece<kGroup>(min(c * 8 + g, a.m - 1), piece));
+    }
+    sums_at[c] = Kept(smem_u32(group_sums) + min(c * 8 + 2 * t, columns - 2) * 4);
+  }
+
+  uint32_t stage = 0, load_stage = (S::kStages - 1) * stage_bytes;
+  for (int round = 0; round < blocks; round += per_round) {
+    const int round_end = min(round + per_round, blocks);
+    int step = warp;
+    for (int block = round; block < round_end; ++block) {
+      float acc[kTiles][kCols][4] = {};
+      for (; step < steps; step += kWarps) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
         __syncwarp();
-        load(stage == 0 ? S::kStages - 1 : stage - 1);
-        const uint8_t* weights = ring + stage * stage_bytes;
-        const uint8_t* inputs = weights + S::kTiles * 1024;
-        stage = stage + 1 == S::kStages ? 0 : stage + 1;
-        uint32_t scale[S::kTiles][2];
-        int zero[S::kTiles][2];
+        load(load_stage);
+        load_stage = stage;
+        const uint32_t inputs = S::kResident ? step * (a.m * 256) : stage, sums_step = step * (kPerStep * columns * 4);
+        Decoder decoder[kTiles][2];
+        if (kGroup == 128) {
 #pragma unroll
-        for (int r = 0; r < S::kTiles; ++r)
+          for (int r = 0; r < kTiles; ++r)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) scale[r][h] = next_scale[r][h], zero[r][h] = next_zero[r][h];
-        const bool more = step + a.k_warps < steps;
-        load_scales(more ? row : row + row_step, more ? step + a.k_warps : wk, next_scale, next_zero);
-
+            for (int h = 0; h < 2; ++h) decoder[r][h].Set(zero[r][h]);
+        }
 #pragma unroll
         for (int group = 0; group < kPerStep; ++group) {
-          // The words of this group, of rows g and g + 8 of each tile.
-          uint32_t w[S::kTiles][2][kWords];
+          const int holder = (lane & ~3) | group;           // the lane with this group's numbers
+          if (kGroup < 128 && !S::kResident) {
 #pragma unroll
-          for (int r = 0; r < S::kTiles; ++r)
+            for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) decoder[r][h].Set(__shfl_sync(0xffffffffu, zero[r][h], holder));
+          }
+          float part[kTiles][kCols][4] = {};
+          // The words of this group, of rows g and g + 8 of each tile.
+          uint32_t w[kTiles][2][kWords];
+#pragma unroll
+          for (int r = 0; r < kTiles; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int at = r * 16 + h * 8 + g;
+              const uint32_t at = weight_at[group] + stage + (r * 16 + h * 8) * 64;
               if constexpr (kGroup == 128) {
-                const uint4 v = *reinterpret_cast<const uint4*>(weights + WeightPiece(at, t));
+                const uint4 v = LoadShared16(at);
                 w[r][h][0] = v.x, w[r][h][1] = v.y, w[r][h][2] = v.z, w[r][h][3] = v.w;
               } else if constexpr (kGroup == 64) {
-                const uint2 v = *reinterpret_cast<const uint2*>(weights + WeightPiece(at, group * 2 + t / 2) + t % 2 * 8);
+                const uint2 v = LoadShared8(at);
                 w[r][h][0] = v.x, w[r][h][1] = v.y;
               } else {
-                w[r][h][0] = *reinterpret_cast<const uint32_t*>(weights + WeightPiece(at, group) + t * 4);
+                w[r][h][0] = LoadShared4(at);
               }
             }
-          float part[S::kTiles][S::kCols][4] = {};
 #pragma unroll
           for (int i = 0; i < kWords; ++i) {
-            uint32_t b[S::kCols][4];
+            uint4 b[kCols];
 #pragma unroll
-            for (int c = 0; c < S::kCols; ++c) {
-              const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? group * 8 + t * 2 + i : group * 4 + t;
-              uint4 v = {};
-              if (c * 8 + g < a.m) v = *reinterpret_cast<const uint4*>(inputs + InputPiece<kGroup>(c * 8 + g, piece));
-              b[c][0] = __byte_perm(v.x, v.z, 0x5410), b[c][1] = __byte_perm(v.x, v.z, 0x7632);
-              b[c][2] = __byte_perm(v.y, v.w, 0x5410), b[c][3] = __byte_perm(v.y, v.w, 0x7632);
+            for (int c = 0; c < kCols; ++c) {
+              b[c] = LoadShared16(input_at[c][group * kWords + i] + inputs);
+              if constexpr (!S::kResident) b[c] = Paired(b[c]);
             }
 #pragma unroll
-            for (int r = 0; r < S::kTiles; ++r) {
+            for (int r = 0; r < kTiles; ++r) {
               uint32_t low[4], high[4];
-              const int from = kGroup == 128 ? lane : (lane & ~3) | group;
-              const int z0 = kGroup == 128 ? zero[r][0] : __shfl_sync(0xffffffffu, zero[r][0], from);
-              const int z1 = kGroup == 128 ? zero[r][1] : __shfl_sync(0xffffffffu, zero[r][1], from);
-              Decode8(w[r][0][i], flip, Offsets<T>(z0), low);
-              Decode8(w[r][1][i], flip, Offsets<T>(z1), high);
+              decoder[r][0].Decode8(w[r][0][i], flip, low);
+              decoder[r][1].Decode8(w[r][1][i], flip, high);
 #pragma unroll
-              for (int c = 0; c < S::kCols; ++c) {
-                Mma<T>(part[r][c], low[0], high[0], low[1], high[1], b[c][0], b[c][1]);
-                Mma<T>(part[r][c], low[2], high[2], low[3], high[3], b[c][2], b[c][3]);
+              for (int c = 0; c < kCols; ++c) {
+                Mma<Operand>(part[r][c], low[0], high[0], low[1], high[1], b[c].x, b[c].y);
+                Mma<Operand>(part[r][c], low[2], high[2], low[3], high[3], b[c].z, b[c].w);
+              }
+            }
+          }
+          if constexpr (S::kResident) {                     // the zero points' share
+            float2 sum[kCols];
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              const uint2 v = LoadShared8(sums_at[c] + sums_step + group * (columns * 4));
+              sum[c] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+            }
+#pragma unroll
+            for (int r = 0; r < kTiles; ++r) {
+              float z0 = -0x1p-21f, z1 = -0x1p-21f;          // -8 * 2^-24
+              if (!is_signed) {
+                z0 = -0x1p-24f * static_cast<float>(kGroup == 128 ? zero[r][0] : __shfl_sync(0xffffffffu, zero[r][0], holder));
+                z1 = -0x1p-24f * static_cast<float>(kGroup == 128 ? zero[r][1] : __shfl_sync(0xffffffffu, zero[r][1], holder));
+              }
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) {
+                part[r][c][0] = fmaf(z0, sum[c].x, part[r][c][0]), part[r][c][1] = fmaf(z0, sum[c].y, part[r][c][1]);
+                part[r][c][2] = fmaf(z1, sum[c].x, part[r][c][2]), part[r][c][3] = fmaf(z1, sum[c].y, part[r][c][3]);
               }
             }
           }
 #pragma unroll
-          for (int r = 0; r < S::kTiles; ++r) {
-            const int from = (lane & ~3) | group;
-            const float s0 = ScaleValue(kGroup == 128 ? scale[r][0] : __shfl_sync(0xffffffffu, scale[r][0], from), a.scale_dtype);
-            const float s1 = ScaleValue(kGroup == 128 ? scale[r][1] : __shfl_sync(0xffffffffu, scale[r][1], from), a.scale_dtype);
+          for (int r = 0; r < kTiles; ++r) {
+            float s0 = ValueOf<kScale>(scale[r][0], a.scale_dtype), s1 = ValueOf<kScale>(scale[r][1], a.scale_dtype);
+            if (kGroup < 128) s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
 #pragma unroll
-            for (int c = 0; c < S::kCols; ++c) {
-              acc[r][c][0] = fmaf(part[r][c][0], s0, acc[r][c][0]);
-              acc[r][c][1] = fmaf(part[r][c][1], s0, acc[r][c][1]);
-              acc[r][c][2] = fmaf(part[r][c][2], s1, acc[r][c][2]);
-              acc[r][c][3] = fmaf(part[r][c][3], s1, acc[r][c][3]);
+            for (int c = 0; c < kCols; ++c) {
+              acc[r][c][0] = fmaf(part[r][c][0], s0, acc[r][c][0]), acc[r][c][1] = fmaf(part[r][c][1], s0, acc[r][c][1]);
+              acc[r][c][2] = fmaf(part[r][c][2], s1, acc[r][c][2]), acc[r][c][3] = fmaf(part[r][c][3], s1, acc[r][c][3]);
             }
           }
         }
+        stage = stage == (S::kStages - 1) * stage_bytes ? 0 : stage + stage_bytes;
+        if (step + kWarps < steps) load_numbers(step + kWarps);
+      }
+      step -= steps;
+      if (block + 1 == round_end) step = warp;
+      set_rows(block + 1);
+      if (step < steps) load_numbers(step);
+      // This warp's sums of the block, zeros where it had no unit of it.
+      float* mine = sums + ((block - round) * kWarps + warp) * a.m * S::kStride;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (c * 8 + 2 * t + e < a.m) {
+#pragma unroll
+            for (int r = 0; r < kTiles; ++r) {
+              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + g] = acc[r][c][e];
+              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + 8 + g] = acc[r][c][e + 2];
+            }
+          }
+    }
+    __syncthreads();
+    const int rows = min(round_end * S::kRows, last - first) - round * S::kRows;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < rows; i += kWarps * 32) {
+      const int at = first + round * S::kRows + i;
+      const float bias = a.bias != nullptr ? ValueOf<0>(LoadBits<0>(a.bias, at, a.bias_dtype), a.bias_dtype) : 0.0f;
+#pragma unroll 1
+      for (int x_row = 0; x_row < a.m; ++x_row) {
+        const float* part = sums + (i / S::kRows * kWarps * a.m + x_row) * S::kStride + i % S::kRows;
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) y += part[w * a.m * S::kStride];
+        if constexpr (S::kResident) y = factors[x_row] != 0.0f ? y * 0x1p24f * factors[x_row] : PlainDot(a, x_row, at);
+        y += bias;
+        const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
+        if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
+        else if (a.d_dtype == kF16) static_cast<__half*>(a.d)[place] = __float2half_rn(y);
+        else static_cast<float*>(a.d)[place] = y;
       }
     }
-    // The warps' sums of this block of rows, added in the order of the warps.
-    __syncthreads();                                        // those of the block before have been read
-    float* mine = sums + warp * 8 * S::kCols * S::kStride;
-#pragma unroll
-    for (int r = 0; r < S::kTiles; ++r)
-#pragma unroll
-      for (int c = 0; c < S::kCols; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mine[(c * 8 + 2 * t + e % 2) * S::kStride + r * 16 + e / 2 * 8 + g] = acc[r][c][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.m * row_step; i += S::kWarps * 32) {
-      const int x_row = i / row_step, in_block = i % row_step, at = block + in_block;
-      if (at >= last) continue;
-      const float* from = sums + (in_block / S::kRows * a.k_warps * 8 * S::kCols + x_row) * S::kStride + in_block % S::kRows;
-      float y = 0.0f;
-      for (int w = 0; w < a.k_warps; ++w) y += from[w * 8 * S::kCols * S::kStride];
-      if (a.bias != nullptr) y += ScaleValue(LoadRaw(a.bias, at, a.bias_dtype), a.bias_dtype);
-      const int64_t to = static_cast<int64_t>(x_row) * a.n + at;
-      if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[to] = __float2bfloat16_rn(y);
-      else if (a.d_dtype == kF16) static_cast<__half*>(a.d)[to] = __float2half_rn(y);
-      else static_cast<float*>(a.d)[to] = y;
-    }
+    __syncthreads();                                        // the sums have been read
   }
 }
-
-// Per tile count of x: how many weight rows share a piece of x, the warps, and the stages of a ring.  A CTA reads x once
-// per block of rows, m / (4 * tiles) bytes of it for a byte of weights.
-using Shape8 = Shape<2, 1, 8, 4>;
-using Shape16 = Shape<4, 2, 4, 4>;
-using Shape32 = Shape<4, 4, 4, 4>;
-using Shape64 = Shape<2, 8, 4, 2>;
 
 struct Variant {
   void (*kernel)(W4Args);
-  int rows, warps, registers;
+  int64_t (*bytes)(int64_t m, int64_t steps, int64_t group);
+  int most, rows, warps, sums, registers;        // most: rows of x; sums: floats for those of a round
 };
-constexpr int kShapes = 4;
-template <typename T, int kGroup>
-void Fill(Variant* v) {
-  v[0] = {w4_dot_kernel<T, kGroup, Shape8>, Shape8::kRows, Shape8::kWarps, 0};
-  v[1] = {w4_dot_kernel<T, kGroup, Shape16>, Shape16::kRows, Shape16::kWarps, 0};
-  v[2] = {w4_dot_kernel<T, kGroup, Shape32>, Shape32::kRows, Shape32::kWarps, 0};
-  v[3] = {w4_dot_kernel<T, kGroup, Shape64>, Shape64::kRows, Shape64::kWarps, 0};
+constexpr int64_t kSmemPerSm = 228 * 1024, kSmemPerCta = 227 * 1024, kSmemReserved = 1024;
+template <int kGroup, int kScale, int kSign, typename S>
+Variant Make() {
+  return {w4_dot_kernel<kGroup, kScale, kSign, S>, S::Bytes, 8 * S::kCols, S::kRows, S::kWarps, S::kSums / (S::kWarps * S::kStride), 0};
 }
-int SmemBytes(int shape, int m) {
-  switch (shape) {
-    case 0: return Shape8::Bytes(m);
-    case 1: return Shape16::Bytes(m);
-    case 2: return Shape32::Bytes(m);
-    default: return Shape64::Bytes(m);
-  }
-}
+// In order of preference: the first that takes m rows of x and fits shared memory.  Without a resident x a CTA reads it once
+// per block of rows, m / (4 * tiles) bytes of it for a byte of weights.
+constexpr int kResidentShapes = 4, kRingShapes = 4;
 struct Variants {
-  Variant v[2][3][kShapes];
+  Variant resident[3][3][2][kResidentShapes];    // group, type of the scales, sign
+  Variant ring[2][3][kRingShapes];               // type of x, group
+  template <int kGroup, int kScale, int kSign>
+  void Fill(Variant* to) {
+    to[0] = Make<kGroup, kScale, kSign, Shape<2, 1, 24, 3, void>>();
+    to[1] = Make<kGroup, kScale, kSign, Shape<2, 1, 16, 3, void>>();
+    to[2] = Make<kGroup, kScale, kSign, Shape<2, 1, 16, 2, void>>();
+    to[3] = Make<kGroup, kScale, kSign, Shape<2, 2, 16, 3, void>>();
+  }
+  template <int kGroup>
+  void FillGroup(int at) {
+    Fill<kGroup, kF16, 0>(resident[at][0][0]);
+    Fill<kGroup, kF16, 1>(resident[at][0][1]);
+    Fill<kGroup, kBF16, 0>(resident[at][1][0]);
+    Fill<kGroup, kBF16, 1>(resident[at][1][1]);
+    Fill<kGroup, kF32, 0>(resident[at][2][0]);
+    Fill<kGroup, kF32, 1>(resident[at][2][1]);
+    FillRing<kGroup, __half>(ring[0][at]);
+    FillRing<kGroup, __nv_bfloat16>(ring[1][at]);
+  }
+  template <int kGroup, typename T>
+  void FillRing(Variant* to) {
+    to[0] = Make<kGroup, 0, 2, Shape<2, 1, 8, 4, T>>();
+    to[1] = Make<kGroup, 0, 2, Shape<4, 2, 4, 4, T>>();
+    to[2] = Make<kGroup, 0, 2, Shape<4, 4, 4, 4, T>>();
+    to[3] = Make<kGroup, 0, 2, Shape<2, 8, 4, 2, T>>();
+  }
   Variants() {
-    Fill<__half, 32>(v[0][0]);
-    Fill<__half, 64>(v[0][1]);
-    Fill<__half, 128>(v[0][2]);
-    Fill<__nv_bfloat16, 32>(v[1][0]);
-    Fill<__nv_bfloat16, 64>(v[1][1]);
-    Fill<__nv_bfloat16, 128>(v[1][2]);
+    FillGroup<32>(0);
+    FillGroup<64>(1);
+    FillGroup<128>(2);
   }
 };
 Variants& TheVariants() {
   static Variants v;
   return v;
 }
-constexpr int kSmemPerSm = 227 * 1024;
 
 }  // namespace
 
 Status InitW4Kernels() {
-  for (auto& types : TheVariants().v)
-    for (auto& groups : types)
-      for (int s = 0; s < kShapes; ++s) {
-        cudaFuncAttributes attr{};
-        cudaError_t e = cudaFuncSetAttribute(groups[s].kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SmemBytes(s, 8 << s));
-        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, groups[s].kernel);
-        if (e != cudaSuccess) return Status::Error(kInternal, std::string("w4_dot_kernel set-up: ") + cudaGetErrorString(e));
-        groups[s].registers = attr.numRegs;
-      }
+  static_assert(std::is_standard_layout_v<Variants>);
+  Variant* v = reinterpret_cast<Variant*>(&TheVariants());
+  for (size_t i = 0; i < sizeof(Variants) / sizeof(Variant); ++i) {
+    cudaFuncAttributes attr{};
+    cudaError_t e = cudaFuncSetAttribute(v[i].kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerCta);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, v[i].kernel);
+    if (e != cudaSuccess) return Status::Error(kInternal, std::string("w4_dot_kernel set-up: ") + cudaGetErrorString(e));
+    v[i].registers = attr.numRegs;
+  }
   return Status::Ok();
 }
 
@@ -380,24 +628,28 @@ Status ValidateDotW4(const B200SD_DotW4& a, bool check_pointers) {
 
 Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stats) {
   if (a.m == 0) return Status::Ok();
-  const int shape = a.m <= 8 ? 0 : a.m <= 16 ? 1 : a.m <= 32 ? 2 : 3;
-  const Variant& v = TheVariants().v[a.x_dtype == kBF16][a.group == 32 ? 0 : a.group == 64 ? 1 : 2][shape];
-  const int bytes = SmemBytes(shape, static_cast<int>(a.m)), threads = v.warps * 32;
-  const int by_registers = 65536 / (threads * ((v.registers + 7) / 8 * 8)), by_smem = kSmemPerSm / (bytes + 1024);
+  const int64_t steps = (a.k + 127) / 128, step_group = std::min<int64_t>(a.group, 128);
+  const int group_at = a.group == 32 ? 0 : a.group == 64 ? 1 : 2, scale_at = a.scale_dtype == kF16 ? 0 : a.scale_dtype == kBF16 ? 1 : 2;
+  const auto& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
+  const auto& ring = TheVariants().ring[a.x_dtype == kBF16][group_at];
+  int pick = 0;
+  auto shape = [&](int i) -> const Variant& { return i < kResidentShapes ? resident[i] : ring[i - kResidentShapes]; };
+  while (a.m > shape(pick).most || shape(pick).bytes(a.m, steps, step_group) > kSmemPerCta) ++pick;       // the last one always fits
+  const Variant& v = shape(pick);
+  const int bytes = static_cast<int>(v.bytes(a.m, steps, step_group)), threads = v.warps * 32;
+  const int by_registers = 65536 / (threads * ((v.registers + 7) / 8 * 8)), by_smem = static_cast<int>(kSmemPerSm / (bytes + kSmemReserved));
   const int per_sm = std::max(1, std::min({by_registers, by_smem, 2048 / threads}));
   // One CTA per resident slot, each with its even share of the rows, but no more CTAs than tiles of 8 rows.
   const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(DeviceSmCount()) * per_sm, (a.n + 7) / 8);
-  // All warps split k where that leaves each at least 8 steps of it; otherwise some take other rows, if the CTA has them.
-  const int64_t steps = (a.k + 127) / 128, rows = (a.n + ctas - 1) / ctas;
-  int k_warps = v.warps;
-  while (k_warps > 1 && steps / k_warps < 8 && rows >= static_cast<int64_t>(v.rows) * (v.warps / k_warps) * 2) k_warps /= 2;
   const int64_t blocks_per_group = a.group >= 128 ? a.group / 128 : 1;
   int group_shift = 0;
   while ((int64_t{1} << group_shift) < blocks_per_group) ++group_shift;
   if ((int64_t{1} << group_shift) != blocks_per_group) group_shift = -1;
   const W4Args args{a.x, static_cast<const uint8_t*>(a.w), a.scale, static_cast<const uint8_t*>(a.zero), a.epilogue == B200SD_EPILOGUE_BIAS ? a.bias : nullptr, a.d,
                     static_cast<int32_t>(a.m), static_cast<int32_t>(a.n), static_cast<int32_t>(a.k), static_cast<int32_t>(a.k / a.group),
-                    group_shift, static_cast<int32_t>(blocks_per_group), k_warps, a.scale_dtype, a.bias_dtype, a.d_dtype, a.weight_type == kS4};
+                    group_shift, static_cast<int32_t>(blocks_per_group),
+                    static_cast<int32_t>(a.n / ctas), static_cast<int32_t>(a.n % ctas), static_cast<int32_t>(steps), v.sums / static_cast<int32_t>(a.m),
+                    0xffffffffu / static_cast<uint32_t>(steps * 16) + 1, a.x_dtype == kBF16, a.scale_dtype, a.bias_dtype, a.d_dtype, a.weight_type == kS4};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // see griddep_wait() in the kernel
   attr.val.programmaticStreamSerializationAllowed = 1;
