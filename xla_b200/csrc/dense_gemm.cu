@@ -1478,6 +1478,22 @@ Status MakeBatchedByteMatrixMap(CUtensorMap* map, const void* base, int64_t batc
   return Status::Ok();
 }
 
+// `count` row-major [rows, cols] byte matrices, 16 rows of box_cols (64 or 128, which may exceed cols) bytes at a time,
+// swizzled by as many bytes; out-of-range elements read as zero.
+Status MakeTileMap(CUtensorMap* map, const void* base, int64_t count, int64_t rows, int64_t cols, uint32_t box_cols) {
+  EncodeTiledFn encode = GetEncodeTiled();
+  if (encode == nullptr) return Status::Error(kInternal, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(count)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows) * static_cast<cuuint64_t>(cols)};
+  const cuuint32_t box[3] = {box_cols, 16, 1};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return Status::Error(kInternal, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(int(r)));
+  return Status::Ok();
+}
+
 // A 3-D byte view [batch, rows, cols] without a shared-memory swizzle: the box lands row after row, box_cols bytes
 // each.  Rows are row_stride bytes apart and batches batch_stride (both multiples of 16); cols itself may be anything,
 // bytes past it read as zero.

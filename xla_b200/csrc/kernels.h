@@ -227,6 +227,9 @@ inline bool StreamIsCapturing(cudaStream_t stream) {
 Status MakeByteMatrixMap(::CUtensorMap_st* map, const void* base, int64_t rows, int64_t cols, uint32_t box_cols,
                          uint32_t box_rows, int l2_promotion = 3);
 
+// Tensor map of `count` row-major [rows, cols] byte matrices in tiles of 16 rows by box_cols (64 or 128) bytes.
+Status MakeTileMap(::CUtensorMap_st* map, const void* base, int64_t count, int64_t rows, int64_t cols, uint32_t box_cols);
+
 // Device address of the current device's status word (valid after InitDevice).
 uint32_t* StatusWordPtr();
 

@@ -9,10 +9,10 @@
 // cuts leaves its pieces (maximum, sum, weighted values) in the workspace, and a second kernel joins them in order, so
 // that the result does not depend on timing.
 //
-// A CTA is four warps, and each warp works on its own 16 tokens of every 64: they come through a ring in shared
-// memory that only this warp fills (cp.async, 16 bytes per lane) and reads, so no barrier stands between loading and
-// computing until an item ends.  The 16-byte pieces of a row are stored at piece ^ (row & 7), which leaves both kinds of
-// reads below without bank conflicts.
+// A CTA is four warps, and each warp works on its own tokens, two tiles of 16 of every 128: they come through a ring in
+// shared memory that only this warp fills (TMA, one box per tile of keys or values) and reads, so no barrier stands
+// between loading and computing until an item ends.  TMA's swizzle puts the 16-byte pieces of a row at piece ^ (row & 7),
+// which leaves both kinds of reads below without bank conflicts.
 //
 // Arithmetic, on mma.m16n8k16 with f16 operands and f32 sums; codes of all three cache types are f16 numbers, exactly.
 // Queries are f16 too: bf16 rows are multiplied by a power of two that brings their largest value to 2^13, so nothing is
@@ -40,7 +40,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                       // tokens of a warp's step
-constexpr int kStep = kTile * kWarps;           // tokens of a CTA's step
 constexpr int kMaxCtas = 148 * 5;               // of one launch; bounds the workspace
 constexpr float kLift = 9.0f;                   // binary digits that a row's largest weight is lifted by ...
 constexpr float kSlack = 6.0f;                  // ... and that a later one may pass it by: together below f16's 2^15.99
@@ -60,7 +59,7 @@ struct AttentionArgs {
   int32_t batch, new_tokens, heads, kv_heads, head_dim, page_shift;
   int32_t rows, blocks;                         // rows of a (sequence, key head), and blocks of them
   int32_t num_pages, table_width, window;       // window: 0 none
-  int32_t unit;                                 // tokens of a unit, a multiple of kStep
+  int32_t unit;                                 // tokens of a unit, a multiple of the CTA's step
   int32_t min_units;                            // a CTA's share is not smaller
   float scale;                                  // softmax_scale * log2(e)
   int32_t is_bf16;
@@ -91,18 +90,34 @@ __device__ __forceinline__ Span SpanOf(const AttentionArgs& a, int b) {
 struct Share {
   int32_t b, item, offset;
   int64_t left;
-  int64_t begin, total, ctas;
+  int64_t begin;
+};
+
+__device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {           // of numbers that mostly fit 32 bits, above 0
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The line of units of `total`, dealt out to `ctas`: `per` to each, and one more to the first `more` of them.
+struct Deal {
+  int64_t total, ctas, per, more;
+  __device__ int64_t Begin(int64_t cta) const { return cta * per + min(cta, more); }
+  __device__ int64_t CtaOf(int64_t u) const {
+    const int64_t large = more * (per + 1);
+    return u < large ? Divide(u, per + 1) : more + Divide(u - large, per);
+  }
 };
 
 // The share of CTA `cta`, with b, item and offset of its first or of its last unit.  Every thread of the block calls it.
 template <int kBlock>
-__device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit) {
+__device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit, Deal* deal) {
   __shared__ int64_t warp_sum[kBlock / 32];
   __shared__ Share found;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int per = (a.batch + kBlock - 1) / kBlock, first = min(tid * per, a.batch), end = min(first + per, a.batch);
   const int64_t items = static_cast<int64_t>(a.kv_heads) * a.blocks;
   int64_t mine = 0;
+#pragma unroll 1
   for (int b = first; b < end; ++b) mine += SpanOf(a, b).units * items;
   int64_t before = mine;
 #pragma unroll
@@ -113,27 +128,32 @@ __device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit) {
   if (lane == 31) warp_sum[warp] = before;
   __syncthreads();
   int64_t total = 0;
+#pragma unroll
   for (int w = 0; w < kBlock / 32; ++w) {
     if (w == warp) before += total;
     total += warp_sum[w];
   }
   before -= mine;
-  const int64_t ctas = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / a.min_units));
-  const int64_t u0 = cta < ctas ? cta * total / ctas : total, u1 = cta < ctas ? (cta + 1) * total / ctas : total;
+  deal->total = total;
+  deal->ctas = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), Divide(total, a.min_units)));
+  deal->per = Divide(total, deal->ctas);
+  deal->more = total - deal->per * deal->ctas;
+  const int64_t u0 = cta < deal->ctas ? deal->Begin(cta) : total, u1 = cta < deal->ctas ? deal->Begin(cta + 1) : total;
   const int64_t u = last_unit ? u1 - 1 : u0;
   if (u0 < u1 && u >= before && u < before + mine) {
+#pragma unroll 1
     for (int b = first; b < end; ++b) {
       const int64_t units = SpanOf(a, b).units;
       if (u < before + units * items) {
-        const int64_t at = u - before;
-        found = {b, static_cast<int32_t>(at / units), static_cast<int32_t>(at % units), u1 - u0, u0, total, ctas};
+        const int64_t at = u - before, item = Divide(at, units);
+        found = {b, static_cast<int32_t>(item), static_cast<int32_t>(at - item * units), u1 - u0, u0};
         break;
       }
       before += units * items;
     }
   }
   __syncthreads();
-  if (u0 >= u1) return {0, 0, 0, 0, 0, total, ctas};
+  if (u0 >= u1) return {0, 0, 0, 0, 0};
   return found;
 }
 
@@ -212,29 +232,26 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
-// Ring, exchange buffer and per-tile numbers of one instantiation.
+// Rings, exchange buffers and per-tile numbers of one instantiation.
 template <int kDim, int kRowTiles>
 struct Layout {
-  static constexpr int kStages = kDim == 64 ? 4 : kDim == 128 ? 3 : 2;
+  static constexpr int kPair = kDim == 256 ? 1 : 2;                         // tiles of a stage
+  static constexpr int kStages = kDim == 64 ? 3 : 2;
+  static constexpr int kStep = kTile * kPair * kWarps;                      // tokens of a CTA's step
   static constexpr int kTileBytes = kTile * kDim;                           // of keys, and again of values
   static constexpr int kRows = 8 * kRowTiles;
-  static constexpr int kStride = kDim + 4;                                  // floats of a row in the exchange buffer
-  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;
-  static constexpr int kNumbers = kWarps * kStages * 16;
-  static constexpr int kExchange = kWarps * kRows * (kStride + 2) * 4;
-  static constexpr int kBytes = kRing + kNumbers + kExchange;
+  static constexpr int kRing = kWarps * kStages * kPair * 2 * kTileBytes;
+  static constexpr int kPart = 32 * kRowTiles * (kDim / 16 + 1);            // float4s of a warp's part of an item: values, then maxima and sums
+  static constexpr int kNumbers = kWarps * kStages * kPair;                 // float4s
+  static constexpr int kBytes = 1024 + kRing + 2 * kPart * 16 + kNumbers * 16 + kWarps * kStages * 8 + 16;
   static constexpr int kSlot = kRows * (kDim + 2);                          // floats of a piece in the workspace
 };
 
-// Byte of 16-byte piece `c` of row `r` in a tile.
+// Byte of 16-byte piece `c` of row `r` in a tile: TMA's swizzles by 64 and by 128 bytes; 256 columns are two boxes.
 template <int kDim>
 __device__ __forceinline__ int PieceAt(int r, int c) {
-  if constexpr (kDim == 64) return (r >> 1) * 128 + ((((r & 1) << 2) | c) ^ (r >> 1)) * 16;
-  return r * kDim + (c >> 3) * 128 + ((c & 7) ^ (r & 7)) * 16;
+  if constexpr (kDim == 64) return r * 64 + (c ^ ((r >> 1) & 3)) * 16;
+  return (c >> 3) * (kTile * 128) + r * 128 + ((c & 7) ^ (r & 7)) * 16;
 }
 // Column of the values' product that m-tile `mt` of lane group `g` holds (its row g; row g + 8 is the next column).
 template <int kDim>
@@ -243,104 +260,139 @@ __device__ __forceinline__ int Column(int g, int mt) {
   return (mt / 8) * 128 + 16 * g + 2 * (mt % 8);
 }
 
-// One row of the result from its weighted values `o` (4 columns at `d`), its sum and its running maximum.
-__device__ __forceinline__ void StoreRow(const AttentionArgs& a, int b, int head, int row, int count, int d, float4 o, float m, float sum) {
+// Part of a row of the result from its weighted values `o` (kCount columns at `d`), its sum and its running maximum.
+template <int kCount>
+__device__ __forceinline__ void StoreRow(const AttentionArgs& a, int b, int head, int row, int count, int d, const float (&o)[kCount], float m, float sum) {
   const int share = a.heads / a.kv_heads, i = row / share;
   const int64_t at = (static_cast<int64_t>(b) * a.new_tokens + i) * a.heads + head * share + row % share;
   const bool empty = i >= count || (m == -INFINITY && sum == 0.0f);
   if (a.lse != nullptr && d == 0) a.lse[at] = empty ? -INFINITY : 0.69314718055994531f * (m + log2f(sum));
   if (d >= a.head_dim) return;
-  const float inv = 1.0f / sum;
-  const float4 y = empty ? make_float4(0, 0, 0, 0) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-  uint2 packed;
-  if (a.is_bf16) {
-    const __nv_bfloat162 l = __floats2bfloat162_rn(y.x, y.y), h = __floats2bfloat162_rn(y.z, y.w);
-    packed = make_uint2(*reinterpret_cast<const uint32_t*>(&l), *reinterpret_cast<const uint32_t*>(&h));
-  } else {
-    const __half2 l = __floats2half2_rn(y.x, y.y), h = __floats2half2_rn(y.z, y.w);
-    packed = make_uint2(*reinterpret_cast<const uint32_t*>(&l), *reinterpret_cast<const uint32_t*>(&h));
+  const float inv = empty ? 0.0f : 1.0f / sum;
+  uint32_t packed[kCount / 2];
+#pragma unroll
+  for (int j = 0; j < kCount / 2; ++j) {
+    const float x = empty ? 0.0f : o[2 * j] * inv, y = empty ? 0.0f : o[2 * j + 1] * inv;
+    if (a.is_bf16) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+      packed[j] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      const __half2 v = __floats2half2_rn(x, y);
+      packed[j] = *reinterpret_cast<const uint32_t*>(&v);
+    }
   }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * a.head_dim + d) = packed;
+  uint16_t* to = static_cast<uint16_t*>(a.out) + at * a.head_dim + d;
+  if constexpr (kCount == 4) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(packed[0], packed[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kCount / 8; ++j) *reinterpret_cast<uint4*>(to + 8 * j) = make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
+  }
 }
 
 template <int kCode, int kDim, int kRowTiles>
-__global__ void __launch_bounds__(kThreads) kv_attention_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ CUtensorMap key_map,
+                                                                const __grid_constant__ CUtensorMap value_map) {
   using L = Layout<kDim, kRowTiles>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  if (threadIdx.x == 0) griddep_launch_dependents();
-  griddep_wait();
+  constexpr int kPair = L::kPair, kStages = L::kStages, kStep = L::kStep, kStageBytes = kPair * 2 * L::kTileBytes;
+  constexpr int kBoxes = kDim == 256 ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;       // the swizzle goes by the address
+  __shared__ int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const Share share = Locate<kThreads>(a, blockIdx.x, false);
+  uint8_t* ring = smem + warp * kStages * kStageBytes;
+  float4* exchange = reinterpret_cast<float4*>(smem + L::kRing);
+  float4* numbers = exchange + 2 * L::kPart + warp * kStages * kPair;
+  uint64_t* full = reinterpret_cast<uint64_t*>(exchange + 2 * L::kPart + L::kNumbers) + warp * kStages;
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+  }
+  griddep_wait();
+  // From here on the second kernel may start: it reads the lengths, which are final now, before it waits for this one.
+  if (threadIdx.x == 0) griddep_launch_dependents();
+  Deal deal;
+  const Share share = Locate<kThreads>(a, blockIdx.x, false, &deal);            // its barriers make the set-up above visible
   if (share.left == 0) return;
 
-  uint8_t* ring = smem + warp * L::kStages * 2 * L::kTileBytes;
-  float4* numbers = reinterpret_cast<float4*>(smem + L::kRing) + warp * L::kStages;
-  float* exchange = reinterpret_cast<float*>(smem + L::kRing + L::kNumbers);
-  float* exchange_max = exchange + kWarps * L::kRows * L::kStride;
-  float* exchange_sum = exchange_max + kWarps * L::kRows;
-
   // ---- loading: this warp's tiles of the whole share, one after the other -----------------------
-  const int pieces = a.head_dim / 16;
-  const int64_t head_bytes = static_cast<int64_t>(a.head_dim) << a.page_shift;
+  // Pages and scales come for 32 tiles at a time, one per lane.  A tile is sent for as soon as its page is known; what the
+  // scales become is written beside the stage (`flush`) when it is about to be used.
   Walk ahead(a, share);
-  int32_t load_pos, load_end, batch_at = 32;               // batch_at: tile of the batch below that comes next
-  int32_t page_of = -1;                                    // lane j: page of tile j of the batch ...
-  float4 numbers_of = {};                                  // ... key scale, log2 of the value scale, its inverse, its sign
-  bool loading = true;
-  load_pos = ahead.Begin(a) + warp * kTile;
-  load_end = ahead.End(a);
-  auto load_tile = [&](int stage) {
-    while (loading && load_pos >= load_end) {
+  int32_t load_pos = ahead.Begin(a) + warp * (kTile * kPair), load_end = ahead.End(a), batch_at = 32;      // batch_at: tile of the batch that comes next
+  int32_t page_of = -1, load_stage = 0, pending = 0;       // lane j: page of tile j of the batch; stages whose numbers are not written
+  float key_scale = 0.0f, value_scale = 0.0f;
+  auto flush = [&] {
+    if (pending == 0) return;
+    // Key scale, log2 of the value scale, its inverse and its sign; -infinity marks a tile that is not there.
+    const float size = fminf(fmaxf(fabsf(value_scale), 0x1p-100f), 0x1p100f);
+    const float4 of_tile = page_of >= 0 ? make_float4(key_scale, log2f(size), 1.0f / size, value_scale / size) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    const int at = lane - (batch_at - pending * kPair);    // this lane's tile among the pending ones
+    if (at >= 0 && at < pending * kPair) {
+      int stage = load_stage - pending + at / kPair;
+      if (stage < 0) stage += kStages;
+      numbers[stage * kPair + at % kPair] = of_tile;
+    }
+    pending = 0;
+  };
+  auto issue = [&] {
+    while (ahead.left > 0 && load_pos >= load_end) {
       ahead.Next(a);
+      flush();
       batch_at = 32;
-      if (ahead.left == 0) { loading = false; break; }
-      load_pos = ahead.Begin(a) + warp * kTile;
+      if (ahead.left == 0) break;
+      load_pos = ahead.Begin(a) + warp * (kTile * kPair);
       load_end = ahead.End(a);
     }
-    if (loading) {
-      const int head = ahead.item / a.blocks;
-      if (batch_at == 32) {
-        // Pages and scales of the next 32 tiles, one per lane.
-        const int64_t pos = static_cast<int64_t>(load_pos) + static_cast<int64_t>(lane) * kStep;
-        page_of = -1;
-        numbers_of = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
-        if (pos < load_end) {
-          const int32_t page = a.page_table[static_cast<int64_t>(ahead.b) * a.table_width + (pos >> a.page_shift)];
-          if (page >= 0 && page < a.num_pages) {
-            page_of = page;
-            const int64_t at = static_cast<int64_t>(page) * a.kv_heads + head;
-            const float vs = a.v_scale[at], size = fminf(fmaxf(fabsf(vs), 0x1p-100f), 0x1p100f);
-            numbers_of = make_float4(a.k_scale[at], log2f(size), 1.0f / size, vs / size);
-          } else {
-            atomicOr(a.status, kStatusBadPage);            // its tokens count as not seen
-          }
+    if (ahead.left == 0) return;
+    const int head = ahead.item / a.blocks;
+    if (batch_at == 32) {
+      flush();
+      const int64_t pos = static_cast<int64_t>(load_pos) + lane / kPair * kStep + lane % kPair * kTile;
+      page_of = -1;
+      if (pos < load_end) {
+        page_of = a.page_table[static_cast<int64_t>(ahead.b) * a.table_width + (pos >> a.page_shift)];
+        if (page_of < 0 || page_of >= a.num_pages) {
+          page_of = -1;
+          atomicOr(a.status, kStatusBadPage);              // its tokens count as not seen
         }
-        batch_at = 0;
       }
-      const int32_t page = __shfl_sync(0xffffffffu, page_of, batch_at);
-      if (lane == batch_at) numbers[stage] = numbers_of;
-      const int64_t slot = load_pos & ((1 << a.page_shift) - 1);
-      const int64_t at = (static_cast<int64_t>(max(page, 0)) * a.kv_heads + head) * head_bytes + slot * a.head_dim;
-      const uint8_t *k = a.k_pages + at, *v = a.v_pages + at;
-      const uint32_t dst = smem_u32(ring + stage * 2 * L::kTileBytes);
-#pragma unroll
-      for (int i = 0; i < kDim / 32; ++i) {
-        const int piece = i * 32 + lane, r = piece / (kDim / 16), c = piece % (kDim / 16);
-        const bool in = c < pieces && page >= 0;           // what is not there reads as zero
-        const int off = r * a.head_dim + c * 16;
-        CopyAsync16(dst + PieceAt<kDim>(r, c), in ? k + off : a.q, in ? 16 : 0);
-        CopyAsync16(dst + L::kTileBytes + PieceAt<kDim>(r, c), in ? v + off : a.q, in ? 16 : 0);
-      }
-      ++batch_at;
-      load_pos += kStep;
+      const int64_t at = static_cast<int64_t>(max(page_of, 0)) * a.kv_heads + head;
+      if (page_of >= 0) key_scale = a.k_scale[at], value_scale = a.v_scale[at];
+      batch_at = 0;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
+    int32_t pages[kPair];
 #pragma unroll
-  for (int s = 0; s < L::kStages - 1; ++s) load_tile(s);
+    for (int i = 0; i < kPair; ++i) pages[i] = __shfl_sync(0xffffffffu, page_of, batch_at + i);
+    if (lane == 0) {
+      int tiles = 0;
+#pragma unroll
+      for (int i = 0; i < kPair; ++i) tiles += pages[i] >= 0 ? 1 : 0;
+      mbar_arrive_expect_tx(&full[load_stage], tiles * 2 * L::kTileBytes);
+#pragma unroll
+      for (int i = 0; i < kPair; ++i) {
+        if (pages[i] < 0) continue;
+        const int slot = (load_pos + i * kTile) & ((1 << a.page_shift) - 1), matrix = pages[i] * a.kv_heads + head;
+        uint8_t* dst = ring + load_stage * kStageBytes + i * 2 * L::kTileBytes;
+#pragma unroll
+        for (int box = 0; box < kBoxes; ++box) {
+          tma_load_3d(dst + box * (kTile * 128), &key_map, &full[load_stage], box * 128, slot, matrix);
+          tma_load_3d(dst + L::kTileBytes + box * (kTile * 128), &value_map, &full[load_stage], box * 128, slot, matrix);
+        }
+      }
+    }
+    batch_at += kPair;
+    load_pos += kStep;
+    ++pending;
+    if (++load_stage == kStages) load_stage = 0;
+  };
+#pragma unroll 1
+  for (int s = 0; s < kStages; ++s) issue();
 
   // ---- computing, piece by piece ---------------------------------------------------------------
   int stage = 0;
+  uint32_t parity = 0;
   const int group = a.heads / a.kv_heads;
   for (Walk walk(a, share); walk.left > 0; walk.Next(a)) {
     const int head = walk.item / a.blocks, row0 = (walk.item % a.blocks) * L::kRows;
@@ -363,7 +415,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const AttentionA
 #pragma unroll
       for (int hf = 0; hf < kDim / 64; ++hf) {
         uint4 v[2] = {};
-        if (row < a.rows && 4 * hf + t < pieces) {
+        if (row < a.rows && 64 * hf + 16 * t < a.head_dim) {
           v[0] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t);
           v[1] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t + 8);
         }
@@ -416,48 +468,60 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const AttentionA
 #pragma unroll
     for (int n = 0; n < kRowTiles; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
 
-    for (int32_t pos = begin + warp * kTile; pos < end; pos += kStep) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+    const int kr = g ^ ((g & 1) << 2);
+#pragma unroll 1
+    for (int32_t pos = begin + warp * (kTile * kPair); pos < end; pos += kStep) {
+      flush();
+      const uint8_t* tiles = ring + stage * kStageBytes;
+      (void)mbar_wait(&full[stage], parity, &abort_flag, a.status, kStatusTileTimeout);
       __syncwarp();
-      load_tile(stage == 0 ? L::kStages - 1 : stage - 1);
-      const uint8_t* keys = ring + stage * 2 * L::kTileBytes;
-      const uint8_t* values = keys + L::kTileBytes;
-      const float4 num = numbers[stage];
-      stage = stage + 1 == L::kStages ? 0 : stage + 1;
+      float4 num[kPair];
+#pragma unroll
+      for (int i = 0; i < kPair; ++i) num[i] = numbers[stage * kPair + i];
+      if (++stage == kStages) stage = 0, parity ^= 1;
 
-      const int kr = g ^ ((g & 1) << 2);
-      float s[kRowTiles][4] = {};
+      float s[kPair][kRowTiles][4] = {};
 #pragma unroll
-      for (int hf = 0; hf < kDim / 64; ++hf) {
-        const uint4 ka = *reinterpret_cast<const uint4*>(keys + PieceAt<kDim>(kr, 4 * hf + t));
-        const uint4 kb = *reinterpret_cast<const uint4*>(keys + PieceAt<kDim>(kr + 8, 4 * hf + t));
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      for (int hf = 0; hf < kDim / 64; ++hf)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t a0, a1, a2, a3;
-          Decode4<kCode>(wa[j], a0, a2);
-          Decode4<kCode>(wb[j], a1, a3);
+        for (int i = 0; i < kPair; ++i) {
+          const uint8_t* keys = tiles + i * 2 * L::kTileBytes;
+          const uint4 ka = *reinterpret_cast<const uint4*>(keys + PieceAt<kDim>(kr, 4 * hf + t));
+          const uint4 kb = *reinterpret_cast<const uint4*>(keys + PieceAt<kDim>(kr + 8, 4 * hf + t));
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-          for (int n = 0; n < kRowTiles; ++n) Mma(s[n], a0, a1, a2, a3, q[n][hf][j][0], q[n][hf][j][1]);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, a2, a3;
+            Decode4<kCode>(wa[j], a0, a2);
+            Decode4<kCode>(wb[j], a1, a3);
+#pragma unroll
+            for (int n = 0; n < kRowTiles; ++n) Mma(s[i][n], a0, a1, a2, a3, q[n][hf][j][0], q[n][hf][j][1]);
+          }
         }
-      }
-      const bool whole = pos >= all_begin && pos + kTile <= all_end;
+      bool whole = pos >= all_begin && pos + kTile * kPair <= all_end;
+#pragma unroll
+      for (int i = 0; i < kPair; ++i) whole = whole && num[i].y != -INFINITY;
       bool move = false;
       float high[kRowTiles][2];
 #pragma unroll
       for (int n = 0; n < kRowTiles; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], factor[n][e % 2] * num.x, num.y);
+        for (int i = 0; i < kPair; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][n][e] = fmaf(s[i][n][e], factor[n][e % 2] * num[i].x, num[i].y);
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int32_t at = pos + kr + (e / 2) * 8;
-            if (at >= row_end[n][e % 2] || at < row_begin[n][e % 2]) s[n][e] = -INFINITY;
-          }
+          for (int i = 0; i < kPair; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int32_t at = pos + i * kTile + kr + (e / 2) * 8;
+              if (num[i].y == -INFINITY || at >= row_end[n][e % 2] || at < row_begin[n][e % 2]) s[i][n][e] = -INFINITY;
+            }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float h = fmaxf(s[n][e], s[n][e + 2]);
+          float h = fmaxf(s[0][n][e], s[0][n][e + 2]);
+          if (kPair == 2) h = fmaxf(h, fmaxf(s[kPair - 1][n][e], s[kPair - 1][n][e + 2]));
           h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, 4));
           h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, 8));
           h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, 16));
@@ -482,134 +546,173 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const AttentionA
             for (int e = 0; e < 4; ++e) o[n][mt][e] *= fade[e % 2];
         }
       }
-      uint32_t p[kRowTiles][2];
+      uint32_t p[kPair][kRowTiles][2];
 #pragma unroll
       for (int n = 0; n < kRowTiles; ++n) {
+        const float from[2] = {top[n][0] == -INFINITY ? 0.0f : top[n][0], top[n][1] == -INFINITY ? 0.0f : top[n][1]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] = Exp2(s[n][e] - (top[n][e % 2] == -INFINITY ? 0.0f : top[n][e % 2]));
-          sum[n][e % 2] = fmaf(s[n][e], num.z, sum[n][e % 2]);
-          s[n][e] *= num.w;
+        for (int i = 0; i < kPair; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[i][n][e] = Exp2(s[i][n][e] - from[e % 2]);
+            sum[n][e % 2] = fmaf(s[i][n][e], num[i].z, sum[n][e % 2]);
+            s[i][n][e] *= num[i].w;
+          }
+          const __half2 l = __floats2half2_rn(s[i][n][0], s[i][n][1]), h = __floats2half2_rn(s[i][n][2], s[i][n][3]);
+          p[i][n][0] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&l));
+          p[i][n][1] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
         }
-        const __half2 l = __floats2half2_rn(s[n][0], s[n][1]), h = __floats2half2_rn(s[n][2], s[n][3]);
-        p[n][0] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&l));
-        p[n][1] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
       }
       // Values: the pieces at this lane's columns of tokens 2t, 2t + 1, 2t + 8 and 2t + 9.
-      const int r0 = (2 * t) ^ 0, r1 = (2 * t + 1) ^ 4;
-      bool scalar = false;
+      const int r0 = 2 * t, r1 = (2 * t + 1) ^ 4;
 #pragma unroll
-      for (int part = 0; part < (kDim == 256 ? 2 : 1); ++part) {
-        constexpr int kWords = kDim == 64 ? 2 : 4;
-        uint32_t w[4][kWords];
+      for (int i = 0; i < kPair; ++i) {
+        if (num[i].y == -INFINITY) continue;               // not loaded
+        const uint8_t* values = tiles + i * 2 * L::kTileBytes + L::kTileBytes;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = (r & 1 ? r1 : r0) + (r & 2 ? 8 : 0);
-          if constexpr (kDim == 64) {
-            const uint2 v = *reinterpret_cast<const uint2*>(values + PieceAt<kDim>(row, g >> 1) + (g & 1) * 8);
-            w[r][0] = v.x, w[r][1] = v.y;
-          } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(values + PieceAt<kDim>(row, part * 8 + g));
-            w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
+        for (int part = 0; part < (kDim == 256 ? 2 : 1); ++part) {
+          constexpr int kWords = kDim == 64 ? 2 : 4;
+          uint32_t w[4][kWords];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = (r & 1 ? r1 : r0) + (r & 2 ? 8 : 0);
+            if constexpr (kDim == 64) {
+              const uint2 v = *reinterpret_cast<const uint2*>(values + PieceAt<kDim>(row, g >> 1) + (g & 1) * 8);
+              w[r][0] = v.x, w[r][1] = v.y;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(values + PieceAt<kDim>(row, part * 8 + g));
+              w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
+            }
           }
           if (!whole) {
             // Weight 0 does not silence a NaN: codes that no row sees are taken out, and where some rows see one that
             // is not finite, the products of the tile are formed one by one.
-            const int32_t at = pos + row;
-            const bool unseen = at >= any_end || at < any_begin;
+            bool scalar = false;
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-              if (unseen) w[r][i] = 0;
-              scalar |= NotFinite4<kCode>(w[r][i]);
+            for (int r = 0; r < 4; ++r) {
+              const int32_t at = pos + i * kTile + (r & 1 ? r1 : r0) + (r & 2 ? 8 : 0);
+              const bool unseen = at >= any_end || at < any_begin;
+#pragma unroll
+              for (int j = 0; j < kWords; ++j) {
+                if (unseen) w[r][j] = 0;
+                scalar |= NotFinite4<kCode>(w[r][j]);
+              }
             }
-          }
-        }
-        if (!whole && all_end != any_end && __any_sync(0xffffffffu, scalar)) {
+            if (kCode != kS8 && all_end != any_end && __any_sync(0xffffffffu, scalar)) {
 #pragma unroll 1
-          for (int token = 0; token < kTile; ++token) {
-            const int row = token ^ ((token & 1) << 2);
+              for (int token = 0; token < kTile; ++token) {
+                const int row = token ^ ((token & 1) << 2), at = pos + i * kTile + row;
 #pragma unroll
-            for (int n = 0; n < kRowTiles; ++n) {
+                for (int n = 0; n < kRowTiles; ++n) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float low = __shfl_sync(0xffffffffu, s[n][e], (token & 7) * 4 + t), upper = __shfl_sync(0xffffffffu, s[n][e + 2], (token & 7) * 4 + t);
-                const float weight = token < 8 ? low : upper;
-                if (pos + row < row_end[n][e] && pos + row >= row_begin[n][e]) {
+                  for (int e = 0; e < 2; ++e) {
+                    const float low = __shfl_sync(0xffffffffu, s[i][n][e], (token & 7) * 4 + t), upper = __shfl_sync(0xffffffffu, s[i][n][e + 2], (token & 7) * 4 + t);
+                    const float weight = token < 8 ? low : upper;
+                    if (at < row_end[n][e] && at >= row_begin[n][e]) {
 #pragma unroll
-                  for (int m = 0; m < 2 * kWords; ++m) {
-                    const int column = Column<kDim>(g, part * 8 + m);
-                    const uint8_t* codes = values + PieceAt<kDim>(row, column / 16) + column % 16;
-                    o[n][part * 8 + m][e] += weight * Decode1<kCode>(codes[0]);
-                    o[n][part * 8 + m][e + 2] += weight * Decode1<kCode>(codes[1]);
+                      for (int m = 0; m < 2 * kWords; ++m) {
+                        const int column = Column<kDim>(g, part * 8 + m);
+                        const uint8_t* codes = values + PieceAt<kDim>(row, column / 16) + column % 16;
+                        o[n][part * 8 + m][e] += weight * Decode1<kCode>(codes[0]);
+                        o[n][part * 8 + m][e + 2] += weight * Decode1<kCode>(codes[1]);
+                      }
+                    }
                   }
                 }
               }
+              continue;
             }
           }
-          continue;
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t a0, a1, a2, a3;
+              Decode4<kCode>(__byte_perm(w[0][j], w[1][j], h == 0 ? 0x5140 : 0x7362), a0, a1);
+              Decode4<kCode>(__byte_perm(w[2][j], w[3][j], h == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+              for (int n = 0; n < kRowTiles; ++n) Mma(o[n][part * 8 + 2 * j + h], a0, a1, a2, a3, p[i][n][0], p[i][n][1]);
+            }
+          }
         }
+      }
+      __syncwarp();                                        // all lanes have read the stage
+      issue();
+    }
+
+    // ---- the piece's end: warps 2 and 3 hand their parts to 0 and 1, then 1 to 0; a lane's part is one of the same places ----
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
+    for (int n = 0; n < kRowTiles; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            Decode4<kCode>(__byte_perm(w[0][i], w[1][i], h == 0 ? 0x5140 : 0x7362), a0, a1);
-            Decode4<kCode>(__byte_perm(w[2][i], w[3][i], h == 0 ? 0x5140 : 0x7362), a2, a3);
+      for (int e = 0; e < 2; ++e) {
+        sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 4);
+        sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 8);
+        sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 16);
+      }
+    __syncthreads();                                       // the buffers of the piece before have been read
+#pragma unroll 1
+    for (int from = 2; from > 0; from /= 2) {
+      if (warp >= from && warp < 2 * from) {
+        float4* to = exchange + (warp & 1) * L::kPart + lane;
 #pragma unroll
-            for (int n = 0; n < kRowTiles; ++n) Mma(o[n][part * 8 + 2 * i + h], a0, a1, a2, a3, p[n][0], p[n][1]);
+        for (int n = 0; n < kRowTiles; ++n) {
+#pragma unroll
+          for (int mt = 0; mt < kDim / 16; ++mt) to[(n * (kDim / 16) + mt) * 32] = make_float4(o[n][mt][0], o[n][mt][1], o[n][mt][2], o[n][mt][3]);
+          to[(kRowTiles * (kDim / 16) + n) * 32] = make_float4(top[n][0], top[n][1], sum[n][0], sum[n][1]);
+        }
+      }
+      __syncthreads();
+      if (warp < from) {
+        const float4* with = exchange + (from == 2 ? warp : 1) * L::kPart + lane;
+#pragma unroll
+        for (int n = 0; n < kRowTiles; ++n) {
+          const float4 other = with[(kRowTiles * (kDim / 16) + n) * 32];
+          const float their_top[2] = {other.x, other.y}, their_sum[2] = {other.z, other.w};
+          float mine[2], theirs[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float m = fmaxf(top[n][e], their_top[e]);
+            mine[e] = top[n][e] == -INFINITY ? 0.0f : Exp2(top[n][e] - m);
+            theirs[e] = their_top[e] == -INFINITY ? 0.0f : Exp2(their_top[e] - m);
+            sum[n][e] = sum[n][e] * mine[e] + their_sum[e] * theirs[e];
+            top[n][e] = m;
+          }
+#pragma unroll
+          for (int mt = 0; mt < kDim / 16; ++mt) {
+            const float4 v = with[(n * (kDim / 16) + mt) * 32];
+            o[n][mt][0] = o[n][mt][0] * mine[0] + v.x * theirs[0], o[n][mt][1] = o[n][mt][1] * mine[1] + v.y * theirs[1];
+            o[n][mt][2] = o[n][mt][2] * mine[0] + v.z * theirs[0], o[n][mt][3] = o[n][mt][3] * mine[1] + v.w * theirs[1];
           }
         }
       }
     }
-
-    // ---- the piece's end: the four warps' parts become one ------------------------------------
-    __syncthreads();                                       // the previous piece has been read
+    if (warp == 0) {
+      const bool complete = walk.offset == 0 && walk.Units() == span.units;
+      float* slot = a.work + (static_cast<int64_t>(blockIdx.x) * 2 + (walk.offset == 0 ? 1 : 0)) * L::kSlot;
+      constexpr int kRun = kDim == 64 ? 8 : 16;              // columns in a row that a lane holds
 #pragma unroll
-    for (int n = 0; n < kRowTiles; ++n) {
+      for (int n = 0; n < kRowTiles; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v = sum[n][e];
-        v += __shfl_xor_sync(0xffffffffu, v, 4);
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const int row = warp * L::kRows + n * 8 + 2 * t + e;
-        if (g == 0) {
-          exchange_max[row] = top[n][e];
-          exchange_sum[row] = v;
+        for (int e = 0; e < 2; ++e) {
+          const int row = n * 8 + 2 * t + e;
+#pragma unroll
+          for (int part = 0; part < kDim / 8 / kRun; ++part) {
+            float run[kRun];
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) run[j] = o[n][part * 8 + j / 2][e + j % 2 * 2];
+            const int d = part * 128 + g * kRun;
+            if (complete) {
+              if (row0 + row < a.rows) StoreRow(a, walk.b, head, row0 + row, span.count, d, run, top[n][e], sum[n][e]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < kRun / 4; ++j) *reinterpret_cast<float4*>(slot + row * kDim + d + 4 * j) = make_float4(run[4 * j], run[4 * j + 1], run[4 * j + 2], run[4 * j + 3]);
+              if (d == 0) {
+                slot[L::kRows * kDim + row] = top[n][e];
+                slot[L::kRows * kDim + L::kRows + row] = sum[n][e];
+              }
+            }
+          }
         }
-#pragma unroll
-        for (int mt = 0; mt < kDim / 16; ++mt)
-          *reinterpret_cast<float2*>(exchange + row * L::kStride + Column<kDim>(g, mt)) = make_float2(o[n][mt][e], o[n][mt][e + 2]);
-      }
-    }
-    __syncthreads();
-    const bool complete = walk.offset == 0 && walk.Units() == span.units;
-    float* slot = a.work + (static_cast<int64_t>(blockIdx.x) * 2 + (walk.offset == 0 ? 1 : 0)) * L::kSlot;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < L::kRows * kDim / 4; i += kThreads) {
-      const int row = i / (kDim / 4), d = i % (kDim / 4) * 4;
-      float m = -INFINITY, total = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, exchange_max[w * L::kRows + row]);
-      float4 y = {};
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = exchange_max[w * L::kRows + row], fade = mw == -INFINITY ? 0.0f : Exp2(mw - m);
-        // A part with no score is left out rather than multiplied by 0 -- its sum may hold the NaN of a row that has one.
-        if (fade == 0.0f && exchange_sum[w * L::kRows + row] == 0.0f) continue;
-        const float4 v = *reinterpret_cast<const float4*>(exchange + (w * L::kRows + row) * L::kStride + d);
-        total = fmaf(exchange_sum[w * L::kRows + row], fade, total);
-        y.x = fmaf(v.x, fade, y.x), y.y = fmaf(v.y, fade, y.y), y.z = fmaf(v.z, fade, y.z), y.w = fmaf(v.w, fade, y.w);
-      }
-      if (complete) {
-        if (row0 + row < a.rows) StoreRow(a, walk.b, head, row0 + row, span.count, d, y, m, total);
-      } else {
-        *reinterpret_cast<float4*>(slot + row * kDim + d) = y;
-        if (d == 0) {
-          slot[L::kRows * kDim + row] = m;
-          slot[L::kRows * kDim + L::kRows + row] = total;
-        }
-      }
     }
   }
 }
@@ -625,15 +728,16 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   constexpr int kVectors = kDim == 256 ? 2 : 1;             // of four columns, per lane
   __shared__ float4 part_values[kParts][L::kRows][kDim / 4];
   __shared__ float part_sum[kParts][L::kRows];
-  if (threadIdx.x == 0) griddep_launch_dependents();
-  griddep_wait();
   const int c = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = warp % L::kRows, part = warp / L::kRows;
-  const Share at = Locate<kJoinThreads>(a, c, true);
+  Deal deal;
+  const Share at = Locate<kJoinThreads>(a, c, true, &deal);
+  griddep_wait();
+  if (threadIdx.x == 0) griddep_launch_dependents();
   if (at.left == 0) return;
   const Span span = SpanOf(a, at.b);
   const int64_t first = at.begin + at.left - 1 - at.offset;              // the item's first unit
   if (at.offset + 1 == span.units || first < at.begin) return;
-  const int last_cta = static_cast<int>(((first + span.units) * at.ctas - 1) / at.total);
+  const int last_cta = static_cast<int>(deal.CtaOf(first + span.units - 1));
   const int pieces = last_cta - c + 1;
   auto slot_of = [&](int p) { return a.work + (static_cast<int64_t>(c + p) * 2 + (p == 0 ? 1 : 0)) * L::kSlot; };
   float m = -INFINITY;
@@ -676,18 +780,21 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   }
 #pragma unroll
   for (int i = 0; i < kVectors; ++i)
-    if (mine) StoreRow(a, at.b, at.item / a.blocks, item_row, span.count, i * 128 + lane * 4, y[i], m, total);
+    if (mine) {
+      const float run[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+      StoreRow(a, at.b, at.item / a.blocks, item_row, span.count, i * 128 + lane * 4, run, m, total);
+    }
 }
 
 struct Variant {
-  void (*main)(AttentionArgs);
+  void (*main)(AttentionArgs, CUtensorMap, CUtensorMap);
   void (*join)(AttentionArgs);
-  int dim, row_tiles, bytes, slot;
+  int dim, row_tiles, bytes, slot, step;
 };
 template <int kCode, int kDim, int kRowTiles>
 constexpr Variant MakeVariant() {
   using L = Layout<kDim, kRowTiles>;
-  return {kv_attention_kernel<kCode, kDim, kRowTiles>, kv_attention_join_kernel<kDim, kRowTiles>, kDim, kRowTiles, L::kBytes, L::kSlot};
+  return {kv_attention_kernel<kCode, kDim, kRowTiles>, kv_attention_join_kernel<kDim, kRowTiles>, kDim, kRowTiles, L::kBytes, L::kSlot, L::kStep};
 }
 // Per cache type: heads up to 64, 128 and 256 wide, 8 or 16 rows at a time.  16 rows of 256 columns do not fit the registers.
 constexpr int kShapes = 5;
@@ -758,8 +865,14 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
                      static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
-                     cut ? kStep : 1 << 30, cut ? 4 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
-  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + kStep - 1) / kStep : 1);
+                     cut ? v.step : 1 << 30, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
+  CUtensorMap key_map, value_map;
+  const bool none = a.num_pages == 0;                                 // then no page is valid, and no tile is loaded
+  const int64_t matrices = none ? 1 : a.num_pages * a.kv_heads;
+  Status st = MakeTileMap(&key_map, none ? a.q : a.k_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
+  if (st.ok()) st = MakeTileMap(&value_map, none ? a.q : a.v_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
+  if (!st.ok()) return st;
+  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + v.step - 1) / v.step : 1);
   int64_t grid = static_cast<int64_t>(DeviceSmCount()) * g_ctas_per_sm[code][shape];
   grid = grid < kMaxCtas ? grid : kMaxCtas;
   grid = grid < most ? grid : most;
@@ -773,7 +886,7 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, v.main, args);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, v.main, args, key_map, value_map);
   stats->launches = 1;
   if (e == cudaSuccess && cut) {
     cfg.blockDim = dim3(kJoinThreads);

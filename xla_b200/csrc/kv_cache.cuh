@@ -28,7 +28,7 @@ Status ValidateCache(const Args& a, int32_t value_dtype, bool check_pointers) {
   if (a.head_dim < 16 || a.head_dim > 256 || a.head_dim % 16) return bad("head_dim must be a multiple of 16 between 16 and 256");
   if (!(a.page_tokens == 16 || a.page_tokens == 32 || a.page_tokens == 64 || a.page_tokens == 128)) return bad("a page must hold 16, 32, 64 or 128 tokens");
   if (a.batch > 4096) return Status::Error(kUnimplemented, "more than 4096 sequences");
-  if (a.num_pages > INT32_MAX) return bad("too many pages for 32-bit page numbers");
+  if (a.num_pages > INT32_MAX / a.kv_heads) return bad("too many pages for 32-bit numbers of (page, head)");
   if (a.table_width > (int64_t{1} << 30) / a.page_tokens) return bad("page_table is too wide: a sequence has at most 2^30 tokens");
   if (!check_pointers || a.batch == 0 || a.new_tokens == 0) return Status::Ok();
   if (a.seq_lens == nullptr) return bad("seq_lens must not be null");
