@@ -86,87 +86,67 @@ __device__ __forceinline__ Span SpanOf(const AttentionArgs& a, int b) {
   return s;
 }
 
-// The share of one CTA: `left` units from unit `offset` of item `item` of sequence `b` on.
+// The share of one CTA: `left` units from `begin` on, and where a unit lies: unit `offset` of item `item` of sequence `b`.
 struct Share {
   int32_t b, item, offset;
-  int64_t left;
-  int64_t begin;
+  int32_t left, begin;
 };
 
-__device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {           // of numbers that mostly fit 32 bits, above 0
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
-}
-
-// The line of units of `total`, dealt out to `ctas`: `per` to each, and one more to the first `more` of them.
+// The line of `total` units, dealt out to `ctas`: `per` to each, and one more to the first `more` of them.
 struct Deal {
-  int64_t total, ctas, per, more;
-  __device__ int64_t Begin(int64_t cta) const { return cta * per + min(cta, more); }
-  __device__ int64_t CtaOf(int64_t u) const {
-    const int64_t large = more * (per + 1);
-    return u < large ? Divide(u, per + 1) : more + Divide(u - large, per);
+  int32_t total, ctas, per, more;
+  __device__ int32_t Begin(int32_t cta) const { return cta * per + min(cta, more); }
+  __device__ int32_t CtaOf(int32_t u) const {
+    const int32_t large = more * (per + 1);
+    return u < large ? u / (per + 1) : more + (u - large) / per;
   }
 };
 
-// The share of CTA `cta`, with b, item and offset of its first or of its last unit.  Every thread of the block calls it.
-template <int kBlock>
+// The share of CTA `cta`, with b, item and offset of its first or of its last unit.  Every warp finds out for itself, its
+// lanes taking consecutive sequences.  The launch chooses units large enough that the line has less than 2^31.
 __device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit, Deal* deal) {
-  __shared__ int64_t warp_sum[kBlock / 32];
-  __shared__ Share found;
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int per = (a.batch + kBlock - 1) / kBlock, first = min(tid * per, a.batch), end = min(first + per, a.batch);
-  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.blocks;
-  int64_t mine = 0;
+  const int lane = threadIdx.x % 32;
+  const int each = (a.batch + 31) / 32, first = min(lane * each, a.batch), end = min(first + each, a.batch);
+  const int32_t items = a.kv_heads * a.blocks;
+  int32_t mine = 0;
 #pragma unroll 1
   for (int b = first; b < end; ++b) mine += SpanOf(a, b).units * items;
-  int64_t before = mine;
+  int32_t before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+    const int32_t v = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += v;
   }
-  if (lane == 31) warp_sum[warp] = before;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kBlock / 32; ++w) {
-    if (w == warp) before += total;
-    total += warp_sum[w];
-  }
+  const int32_t total = __shfl_sync(0xffffffffu, before, 31);
   before -= mine;
   deal->total = total;
-  deal->ctas = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), Divide(total, a.min_units)));
-  deal->per = Divide(total, deal->ctas);
+  deal->ctas = max(1, min(static_cast<int32_t>(gridDim.x), total / a.min_units));
+  deal->per = total / deal->ctas;
   deal->more = total - deal->per * deal->ctas;
-  const int64_t u0 = cta < deal->ctas ? deal->Begin(cta) : total, u1 = cta < deal->ctas ? deal->Begin(cta + 1) : total;
-  const int64_t u = last_unit ? u1 - 1 : u0;
-  if (u0 < u1 && u >= before && u < before + mine) {
-#pragma unroll 1
-    for (int b = first; b < end; ++b) {
-      const int64_t units = SpanOf(a, b).units;
-      if (u < before + units * items) {
-        const int64_t at = u - before, item = Divide(at, units);
-        found = {b, static_cast<int32_t>(item), static_cast<int32_t>(at - item * units), u1 - u0, u0};
-        break;
-      }
-      before += units * items;
+  if (cta >= deal->ctas) return {0, 0, 0, 0, 0};
+  const int32_t u0 = deal->Begin(cta), u1 = deal->Begin(cta + 1), u = last_unit ? u1 - 1 : u0;
+  const bool here = u >= before && u < before + mine;
+  int32_t b = first, at = u - before, units = 1;
+  if (here) {
+    units = SpanOf(a, b).units;
+    while (at >= units * items) {
+      at -= units * items;
+      units = SpanOf(a, ++b).units;
     }
   }
-  __syncthreads();
-  if (u0 >= u1) return {0, 0, 0, 0, 0};
-  return found;
+  const int32_t item = at / units, from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  return {__shfl_sync(0xffffffffu, b, from), __shfl_sync(0xffffffffu, item, from), __shfl_sync(0xffffffffu, at - item * units, from), u1 - u0, u0};
 }
 
 // Steps through the pieces of items that make up a share.
 struct Walk {
-  int32_t b, item, offset;
-  int64_t left;
+  int32_t b, item, offset, left;
   Span span;
 
   __device__ Walk(const AttentionArgs& a, const Share& s) : b(s.b), item(s.item), offset(s.offset), left(s.left) {
     if (left > 0) span = SpanOf(a, b);
   }
-  __device__ int32_t Units() const { return static_cast<int32_t>(min(left, static_cast<int64_t>(span.units - offset))); }
+  __device__ int32_t Units() const { return min(left, span.units - offset); }
   __device__ int32_t Begin(const AttentionArgs& a) const { return span.lo + offset * a.unit; }
   __device__ int32_t End(const AttentionArgs& a) const {
     return static_cast<int32_t>(min(static_cast<int64_t>(span.hi), static_cast<int64_t>(Begin(a)) + static_cast<int64_t>(Units()) * a.unit));
@@ -309,12 +289,42 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
     fence_mbar_init();
   }
+  __syncthreads();
   griddep_wait();
   // From here on the second kernel may start: it reads the lengths, which are final now, before it waits for this one.
   if (threadIdx.x == 0) griddep_launch_dependents();
   Deal deal;
-  const Share share = Locate<kThreads>(a, blockIdx.x, false, &deal);            // its barriers make the set-up above visible
+  const Share share = Locate(a, blockIdx.x, false, &deal);
   if (share.left == 0) return;
+
+  // This lane's part of an item's queries, as they are.  The first item's are sent for before the tiles, which they would
+  // otherwise queue behind.
+  const int group = a.heads / a.kv_heads;
+  uint32_t q[kRowTiles][kDim / 64][4][2];
+  auto load_queries = [&](int b, int item) {
+    const int head = item / a.blocks, row0 = (item - head * a.blocks) * L::kRows;
+#pragma unroll
+    for (int n = 0; n < kRowTiles; ++n) {
+      const int row = row0 + n * 8 + g;
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) +
+          ((static_cast<int64_t>(b) * a.new_tokens + row / group) * a.heads + head * group + row % group) * a.head_dim;
+#pragma unroll
+      for (int hf = 0; hf < kDim / 64; ++hf) {
+        uint4 v[2] = {};
+        if (row < a.rows && 64 * hf + 16 * t < a.head_dim) {
+          v[0] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t);
+          v[1] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t + 8);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          q[n][hf][j][0] = j < 2 ? (j == 0 ? v[0].x : v[0].z) : (j == 2 ? v[1].x : v[1].z);
+          q[n][hf][j][1] = j < 2 ? (j == 0 ? v[0].y : v[0].w) : (j == 2 ? v[1].y : v[1].w);
+        }
+      }
+    }
+  };
+  load_queries(share.b, share.item);
+  bool loaded = false;
 
   // ---- loading: this warp's tiles of the whole share, one after the other -----------------------
   // Pages and scales come for 32 tiles at a time, one per lane.  A tile is sent for as soon as its page is known; what the
@@ -322,12 +332,15 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
   Walk ahead(a, share);
   int32_t load_pos = ahead.Begin(a) + warp * (kTile * kPair), load_end = ahead.End(a), batch_at = 32;      // batch_at: tile of the batch that comes next
   int32_t page_of = -1, load_stage = 0, pending = 0;       // lane j: page of tile j of the batch; stages whose numbers are not written
-  float key_scale = 0.0f, value_scale = 0.0f;
+  bool raw = false;
+  float4 of_tile = {};                                     // key scale, log2 of the value scale, its inverse, its sign; -infinity marks a tile that is not there
   auto flush = [&] {
     if (pending == 0) return;
-    // Key scale, log2 of the value scale, its inverse and its sign; -infinity marks a tile that is not there.
-    const float size = fminf(fmaxf(fabsf(value_scale), 0x1p-100f), 0x1p100f);
-    const float4 of_tile = page_of >= 0 ? make_float4(key_scale, log2f(size), 1.0f / size, value_scale / size) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    if (raw) {
+      const float size = fminf(fmaxf(fabsf(of_tile.w), 0x1p-100f), 0x1p100f);
+      of_tile = page_of >= 0 ? make_float4(of_tile.x, log2f(size), 1.0f / size, of_tile.w / size) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+      raw = false;
+    }
     const int at = lane - (batch_at - pending * kPair);    // this lane's tile among the pending ones
     if (at >= 0 && at < pending * kPair) {
       int stage = load_stage - pending + at / kPair;
@@ -359,7 +372,8 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
         }
       }
       const int64_t at = static_cast<int64_t>(max(page_of, 0)) * a.kv_heads + head;
-      if (page_of >= 0) key_scale = a.k_scale[at], value_scale = a.v_scale[at];
+      if (page_of >= 0) of_tile.x = a.k_scale[at], of_tile.w = a.v_scale[at];
+      raw = true;
       batch_at = 0;
     }
     int32_t pages[kPair];
@@ -393,7 +407,6 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
   // ---- computing, piece by piece ---------------------------------------------------------------
   int stage = 0;
   uint32_t parity = 0;
-  const int group = a.heads / a.kv_heads;
   for (Walk walk(a, share); walk.left > 0; walk.Next(a)) {
     const int head = walk.item / a.blocks, row0 = (walk.item % a.blocks) * L::kRows;
     const Span& span = walk.span;
@@ -404,27 +417,12 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     }
 
     // Queries as the products want them, and what turns a product into a score, for the rows 2t and 2t + 1 of each 8.
-    uint32_t q[kRowTiles][kDim / 64][4][2];
+    if (loaded) load_queries(walk.b, walk.item);
+    loaded = true;
     float factor[kRowTiles][2];
     int32_t row_end[kRowTiles][2], row_begin[kRowTiles][2];
 #pragma unroll
     for (int n = 0; n < kRowTiles; ++n) {
-      const int row = row0 + n * 8 + g;
-      const uint16_t* from = static_cast<const uint16_t*>(a.q) +
-          ((static_cast<int64_t>(walk.b) * a.new_tokens + row / group) * a.heads + head * group + row % group) * a.head_dim;
-#pragma unroll
-      for (int hf = 0; hf < kDim / 64; ++hf) {
-        uint4 v[2] = {};
-        if (row < a.rows && 64 * hf + 16 * t < a.head_dim) {
-          v[0] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t);
-          v[1] = *reinterpret_cast<const uint4*>(from + 64 * hf + 16 * t + 8);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          q[n][hf][j][0] = j < 2 ? (j == 0 ? v[0].x : v[0].z) : (j == 2 ? v[1].x : v[1].z);
-          q[n][hf][j][1] = j < 2 ? (j == 0 ? v[0].y : v[0].w) : (j == 2 ? v[1].y : v[1].w);
-        }
-      }
       float mine = 1.0f;
       if (a.is_bf16) {
         uint32_t top = 0;                                  // exponent of the row's largest value
@@ -730,35 +728,57 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   __shared__ float part_sum[kParts][L::kRows];
   const int c = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = warp % L::kRows, part = warp / L::kRows;
   Deal deal;
-  const Share at = Locate<kJoinThreads>(a, c, true, &deal);
+  const Share at = Locate(a, c, true, &deal);
   griddep_wait();
   if (threadIdx.x == 0) griddep_launch_dependents();
   if (at.left == 0) return;
   const Span span = SpanOf(a, at.b);
-  const int64_t first = at.begin + at.left - 1 - at.offset;              // the item's first unit
+  const int32_t first = at.begin + at.left - 1 - at.offset;              // the item's first unit
   if (at.offset + 1 == span.units || first < at.begin) return;
-  const int last_cta = static_cast<int>(deal.CtaOf(first + span.units - 1));
-  const int pieces = last_cta - c + 1;
+  const int pieces = deal.CtaOf(first + span.units - 1) - c + 1;
   auto slot_of = [&](int p) { return a.work + (static_cast<int64_t>(c + p) * 2 + (p == 0 ? 1 : 0)) * L::kSlot; };
+  // A few pieces are sent for at once; their maximum is known when they come.
+  constexpr int kAtOnce = 4;
+  const bool mine = lane * 4 < kDim;
+  float first_max[kAtOnce], first_sum[kAtOnce];
+  float4 first_values[kAtOnce][kVectors];
+#pragma unroll
+  for (int j = 0; j < kAtOnce; ++j) {
+    const int p = part + j * kParts;
+    first_max[j] = -INFINITY, first_sum[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) first_values[j][i] = make_float4(0, 0, 0, 0);
+    if (p < pieces) {
+      const float* slot = slot_of(p);
+      first_max[j] = slot[L::kRows * kDim + row], first_sum[j] = slot[L::kRows * kDim + L::kRows + row];
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i)
+        if (mine) first_values[j][i] = *reinterpret_cast<const float4*>(slot + row * kDim + i * 128 + lane * 4);
+    }
+  }
   float m = -INFINITY;
   for (int p = lane; p < pieces; p += 32) m = fmaxf(m, slot_of(p)[L::kRows * kDim + row]);
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float total = 0.0f;
   float4 y[kVectors] = {};
-  const bool mine = lane * 4 < kDim;
+  auto add = [&](float piece_max, float piece_sum, const float4 (&v)[kVectors]) {
+    const float fade = piece_max == -INFINITY ? 0.0f : Exp2(piece_max - m);
+    total = fmaf(piece_sum, fade, total);
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) y[i].x = fmaf(v[i].x, fade, y[i].x), y[i].y = fmaf(v[i].y, fade, y[i].y), y[i].z = fmaf(v[i].z, fade, y[i].z), y[i].w = fmaf(v[i].w, fade, y[i].w);
+  };
+#pragma unroll
+  for (int j = 0; j < kAtOnce; ++j) add(first_max[j], first_sum[j], first_values[j]);
 #pragma unroll 4
-  for (int p = part; p < pieces; p += kParts) {
+  for (int p = part + kAtOnce * kParts; p < pieces; p += kParts) {
     const float* slot = slot_of(p);
-    const float mp = slot[L::kRows * kDim + row], sp = slot[L::kRows * kDim + L::kRows + row];
+    const float piece_max = slot[L::kRows * kDim + row], piece_sum = slot[L::kRows * kDim + L::kRows + row];
     float4 v[kVectors] = {};
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
       if (mine) v[i] = *reinterpret_cast<const float4*>(slot + row * kDim + i * 128 + lane * 4);
-    const float fade = mp == -INFINITY ? 0.0f : Exp2(mp - m);
-    total = fmaf(sp, fade, total);
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) y[i].x = fmaf(v[i].x, fade, y[i].x), y[i].y = fmaf(v[i].y, fade, y[i].y), y[i].z = fmaf(v[i].z, fade, y[i].z), y[i].w = fmaf(v[i].w, fade, y[i].w);
+    add(piece_max, piece_sum, v);
   }
   if (part > 0) {
     if (lane == 0) part_sum[part][row] = total;
@@ -816,6 +836,9 @@ Status InitAttentionKernels() {
       const Variant& v = kVariants[c][s];
       cudaError_t e = cudaFuncSetAttribute(v.main, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes);
       int n = 0;
+      // The two kernels alternate on an SM; with the same split of its memory it needs not be empty in between.
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(v.main, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(v.join, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
       if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, v.main, kThreads, v.bytes);
       if (e != cudaSuccess) return Status::Error(kInternal, std::string("kv_attention_kernel set-up: ") + cudaGetErrorString(e));
       g_ctas_per_sm[c][s] = n > 0 ? n : 1;
@@ -860,19 +883,21 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   const int64_t capacity = a.table_width * a.page_tokens;
   // A sequence that the table cannot make longer than this is not cut: the second kernel would cost more than it saves.
   const bool cut = capacity > 512;
+  int64_t unit = cut ? v.step : 1 << 30;
+  while (a.batch * a.kv_heads * blocks * ((capacity + unit - 1) / unit) >= INT32_MAX) unit *= 2;       // the line's positions are 32-bit numbers
   AttentionArgs args{a.q, static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages), a.k_scale, a.v_scale,
                      a.page_table, a.seq_lens, a.new_lens, a.out, a.lse, static_cast<float*>(a.workspace),
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
                      static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
-                     cut ? v.step : 1 << 30, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
+                     static_cast<int32_t>(unit), cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
   CUtensorMap key_map, value_map;
   const bool none = a.num_pages == 0;                                 // then no page is valid, and no tile is loaded
   const int64_t matrices = none ? 1 : a.num_pages * a.kv_heads;
   Status st = MakeTileMap(&key_map, none ? a.q : a.k_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
   if (st.ok()) st = MakeTileMap(&value_map, none ? a.q : a.v_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
   if (!st.ok()) return st;
-  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + v.step - 1) / v.step : 1);
+  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + unit - 1) / unit : 1);
   int64_t grid = static_cast<int64_t>(DeviceSmCount()) * g_ctas_per_sm[code][shape];
   grid = grid < kMaxCtas ? grid : kMaxCtas;
   grid = grid < most ? grid : most;
