@@ -4,10 +4,10 @@
 // one product, so the cache is read once for all of them: 8 or 16 rows per pass.  A step is bound by reading the codes:
 // one byte of keys or values is used for 2 * rows operations.
 //
-// Work.  An item is (sequence, key head, block of rows); a unit is kUnit tokens of an item.  The units of all items, in
-// one line, are dealt out to the CTAs in equal consecutive shares, whatever the lengths are; an item that a share's end
-// cuts leaves its pieces (maximum, sum, weighted values) in the workspace, and a second kernel joins them in order, so
-// that the result does not depend on timing.
+// Work.  An item is (sequence, key head, block of rows); its units are one for every 128 tokens (64 of wide heads) behind a
+// few that stand for what an item costs besides its tokens.  The units of all items, in one line, are dealt out to the CTAs in equal consecutive shares, whatever the lengths are; an item that
+// a share's end cuts leaves its pieces (maximum, sum, weighted values) in the workspace, and a second kernel joins them in
+// order, so that the result does not depend on timing.
 //
 // A CTA is four warps, and each warp works on its own tokens, two tiles of 16 of every 128: they come through a ring in
 // shared memory that only this warp fills (TMA, one box per tile of keys or values) and reads, so no barrier stands
@@ -31,6 +31,8 @@
 // more than 6, so most tiles rescale nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "kv_cache.cuh"
 
@@ -59,7 +61,7 @@ struct AttentionArgs {
   int32_t batch, new_tokens, heads, kv_heads, head_dim, page_shift;
   int32_t rows, blocks;                         // rows of a (sequence, key head), and blocks of them
   int32_t num_pages, table_width, window;       // window: 0 none
-  int32_t unit;                                 // tokens of a unit, a multiple of the CTA's step
+  int32_t unit, extra;                          // tokens of a unit, a multiple of the CTA's step; units without tokens in front of an item
   int32_t min_units;                            // a CTA's share is not smaller
   float scale;                                  // softmax_scale * log2(e)
   int32_t is_bf16;
@@ -82,7 +84,7 @@ __device__ __forceinline__ Span SpanOf(const AttentionArgs& a, int b) {
   const int32_t capacity = a.table_width << a.page_shift;
   s.hi = s.count > 0 ? min(max(len, 0), capacity) : 0;
   s.lo = a.window > 0 ? max(0, s.base + 1 - a.window) & ~(kTile - 1) : 0;
-  s.units = s.hi > s.lo ? (s.hi - s.lo + a.unit - 1) / a.unit : 1;        // an item without tokens still has rows to write
+  s.units = max(1, a.extra + (s.hi > s.lo ? (s.hi - s.lo + a.unit - 1) / a.unit : 0));      // an item without tokens still has rows to write
   return s;
 }
 
@@ -124,18 +126,32 @@ __device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit, Deal* d
   deal->per = total / deal->ctas;
   deal->more = total - deal->per * deal->ctas;
   if (cta >= deal->ctas) return {0, 0, 0, 0, 0};
-  const int32_t u0 = deal->Begin(cta), u1 = deal->Begin(cta + 1), u = last_unit ? u1 - 1 : u0;
-  const bool here = u >= before && u < before + mine;
-  int32_t b = first, at = u - before, units = 1;
-  if (here) {
-    units = SpanOf(a, b).units;
-    while (at >= units * items) {
-      at -= units * items;
-      units = SpanOf(a, ++b).units;
+  auto place = [&](int32_t u) -> Share {
+    const bool here = u >= before && u < before + mine;
+    int32_t b = first, at = u - before, units = 1;
+    if (here) {
+      units = SpanOf(a, b).units;
+      while (at >= units * items) {
+        at -= units * items;
+        units = SpanOf(a, ++b).units;
+      }
     }
+    const int32_t item = at / units, from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    return {__shfl_sync(0xffffffffu, b, from), __shfl_sync(0xffffffffu, item, from), __shfl_sync(0xffffffffu, at - item * units, from), 0, u};
+  };
+  // A share does not end with units without tokens; the next one takes them.
+  int32_t u0 = deal->Begin(cta), u1 = deal->Begin(cta + 1);
+  Share at_begin = place(u0);
+  if (at_begin.offset <= a.extra) u0 -= at_begin.offset, at_begin.offset = 0;
+  if (u1 < total) {
+    const int32_t into = place(u1).offset;
+    if (into <= a.extra) u1 -= into;
   }
-  const int32_t item = at / units, from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-  return {__shfl_sync(0xffffffffu, b, from), __shfl_sync(0xffffffffu, item, from), __shfl_sync(0xffffffffu, at - item * units, from), u1 - u0, u0};
+  if (u0 >= u1) return {0, 0, 0, 0, 0};
+  Share share = last_unit ? place(u1 - 1) : at_begin;
+  share.begin = u0;
+  share.left = u1 - u0;
+  return share;
 }
 
 // Steps through the pieces of items that make up a share.
@@ -147,9 +163,9 @@ struct Walk {
     if (left > 0) span = SpanOf(a, b);
   }
   __device__ int32_t Units() const { return min(left, span.units - offset); }
-  __device__ int32_t Begin(const AttentionArgs& a) const { return span.lo + offset * a.unit; }
+  __device__ int32_t Begin(const AttentionArgs& a) const { return span.lo + max(0, offset - a.extra) * a.unit; }
   __device__ int32_t End(const AttentionArgs& a) const {
-    return static_cast<int32_t>(min(static_cast<int64_t>(span.hi), static_cast<int64_t>(Begin(a)) + static_cast<int64_t>(Units()) * a.unit));
+    return static_cast<int32_t>(min(static_cast<int64_t>(span.hi), span.lo + static_cast<int64_t>(max(0, offset + Units() - a.extra)) * a.unit));
   }
   __device__ void Next(const AttentionArgs& a) {
     const int32_t n = Units();
@@ -324,7 +340,6 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     }
   };
   load_queries(share.b, share.item);
-  bool loaded = false;
 
   // ---- loading: this warp's tiles of the whole share, one after the other -----------------------
   // Pages and scales come for 32 tiles at a time, one per lane.  A tile is sent for as soon as its page is known; what the
@@ -417,8 +432,6 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     }
 
     // Queries as the products want them, and what turns a product into a score, for the rows 2t and 2t + 1 of each 8.
-    if (loaded) load_queries(walk.b, walk.item);
-    loaded = true;
     float factor[kRowTiles][2];
     int32_t row_end[kRowTiles][2], row_begin[kRowTiles][2];
 #pragma unroll
@@ -636,6 +649,11 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
       }
       __syncwarp();                                        // all lanes have read the stage
       issue();
+    }
+
+    if (walk.left > walk.Units()) {                        // the next item's queries, on their way while this one is put together
+      const bool same = walk.item + 1 < a.kv_heads * a.blocks;
+      load_queries(same ? walk.b : walk.b + 1, same ? walk.item + 1 : 0);
     }
 
     // ---- the piece's end: warps 2 and 3 hand their parts to 0 and 1, then 1 to 0; a lane's part is one of the same places ----
@@ -884,20 +902,23 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   // A sequence that the table cannot make longer than this is not cut: the second kernel would cost more than it saves.
   const bool cut = capacity > 512;
   int64_t unit = cut ? v.step : 1 << 30;
-  while (a.batch * a.kv_heads * blocks * ((capacity + unit - 1) / unit) >= INT32_MAX) unit *= 2;       // the line's positions are 32-bit numbers
+  while (a.batch * a.kv_heads * blocks * ((capacity + unit - 1) / unit + 16) >= INT32_MAX) unit *= 2;       // the line's positions are 32-bit numbers
+  // An item costs a CTA about 4 us besides its tokens, as much as it needs for 192 KiB of them shared by the CTAs of an SM.
+  // (Sequences of 0 to 4096 tokens, in us without and with: 41 and 37; 40 rows per key head: 107 and 60.)
+  const int extra = cut ? std::max(1, static_cast<int>((192 << 10) / (g_ctas_per_sm[code][shape] * v.step * v.dim * 2))) : 0;
   AttentionArgs args{a.q, static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages), a.k_scale, a.v_scale,
                      a.page_table, a.seq_lens, a.new_lens, a.out, a.lse, static_cast<float*>(a.workspace),
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
                      static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
-                     static_cast<int32_t>(unit), cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
+                     static_cast<int32_t>(unit), extra, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
   CUtensorMap key_map, value_map;
   const bool none = a.num_pages == 0;                                 // then no page is valid, and no tile is loaded
   const int64_t matrices = none ? 1 : a.num_pages * a.kv_heads;
   Status st = MakeTileMap(&key_map, none ? a.q : a.k_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
   if (st.ok()) st = MakeTileMap(&value_map, none ? a.q : a.v_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
   if (!st.ok()) return st;
-  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + unit - 1) / unit : 1);
+  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + unit - 1) / unit + extra : 1);
   int64_t grid = static_cast<int64_t>(DeviceSmCount()) * g_ctas_per_sm[code][shape];
   grid = grid < kMaxCtas ? grid : kMaxCtas;
   grid = grid < most ? grid : most;
