@@ -180,19 +180,6 @@ struct Attr {
   size_t count = 0;               // array length
 };
 
-struct Call {
-  std::string target;
-  struct Buf {
-    XLA_FFI_DataType dtype;
-    void* data;
-    std::vector<int64_t> dims;
-  };
-  std::vector<Buf> args, rets;
-  std::vector<Attr> attrs;
-  std::map<int, std::pair<int64_t, void*>> state;
-  bool instantiated = false;
-};
-
 struct BuiltFrame {
   std::vector<XLA_FFI_Buffer> arg_bufs, ret_bufs;
   std::vector<XLA_FFI_ArgType> arg_types;
@@ -206,6 +193,25 @@ struct BuiltFrame {
   std::vector<XLA_FFI_AttrType> attr_types;
   std::vector<void*> attr_ptrs;
   XLA_FFI_CallFrame frame{};
+};
+
+struct Call {
+  std::string target;
+  struct Buf {
+    XLA_FFI_DataType dtype;
+    void* data;
+    std::vector<int64_t> dims;
+  };
+  std::vector<Buf> args, rets;
+  std::vector<Attr> attrs;
+  std::map<int, std::pair<int64_t, void*>> state;
+  bool instantiated = false;
+  // The execute frame, kept between calls of the same site (XLA, too, only updates the addresses in it).
+  std::mutex mu;
+  bool have_handlers = false, have_frame = false;
+  Registration handlers;
+  XLA_FFI_InvokeContext ctx;
+  BuiltFrame frame;
 };
 
 void Build(Call& c, bool null_data, XLA_FFI_InvokeContext* ctx, XLA_FFI_ExecutionStage stage, BuiltFrame* b) {
@@ -348,8 +354,18 @@ MOCK_EXPORT void mockffi_call_add_ret(void* call, int dtype, void* data, int ran
   static_cast<Call*>(call)->rets.push_back({static_cast<XLA_FFI_DataType>(dtype), data, std::vector<int64_t>(dims, dims + rank)});
 }
 // Re-points an operand / result at a new device address (XLA's UpdateWithBuffers).
-MOCK_EXPORT void mockffi_call_set_arg_data(void* call, int index, void* data) { static_cast<Call*>(call)->args.at(index).data = data; }
-MOCK_EXPORT void mockffi_call_set_ret_data(void* call, int index, void* data) { static_cast<Call*>(call)->rets.at(index).data = data; }
+MOCK_EXPORT void mockffi_call_set_arg_data(void* call, int index, void* data) {
+  Call* c = static_cast<Call*>(call);
+  std::lock_guard<std::mutex> lock(c->mu);
+  c->args.at(index).data = data;
+  if (c->have_frame) c->frame.arg_bufs.at(index).data = data;
+}
+MOCK_EXPORT void mockffi_call_set_ret_data(void* call, int index, void* data) {
+  Call* c = static_cast<Call*>(call);
+  std::lock_guard<std::mutex> lock(c->mu);
+  c->rets.at(index).data = data;
+  if (c->have_frame) c->frame.ret_bufs.at(index).data = data;
+}
 MOCK_EXPORT void mockffi_call_attr_i64(void* call, const char* name, int64_t v) { AddScalar(static_cast<Call*>(call), name, XLA_FFI_DataType_S64, &v, sizeof(v)); }
 MOCK_EXPORT void mockffi_call_attr_i32(void* call, const char* name, int32_t v) { AddScalar(static_cast<Call*>(call), name, XLA_FFI_DataType_S32, &v, sizeof(v)); }
 MOCK_EXPORT void mockffi_call_attr_f64(void* call, const char* name, double v) { AddScalar(static_cast<Call*>(call), name, XLA_FFI_DataType_F64, &v, sizeof(v)); }
@@ -379,27 +395,32 @@ MOCK_EXPORT void mockffi_call_attr_i64_array(void* call, const char* name, const
 // Runs one stage of the call.  INSTANTIATE hides the buffer addresses, as XLA does.
 MOCK_EXPORT int mockffi_call_invoke(void* call, int stage, void* stream, int device_ordinal, char* err, size_t err_len) {
   Call* c = static_cast<Call*>(call);
-  Registration reg;
-  {
+  std::lock_guard<std::mutex> call_lock(c->mu);
+  if (!c->have_handlers) {
     std::lock_guard<std::mutex> lock(g_mu);
     auto it = Registry().find("CUDA:" + c->target);
     if (it == Registry().end()) {
       if (err && err_len) snprintf(err, err_len, "No FFI handler registered for %s on platform CUDA", c->target.c_str());
       return XLA_FFI_Error_Code_NOT_FOUND;
     }
-    reg = it->second;
+    c->handlers = it->second;
+    c->have_handlers = true;
   }
-  XLA_FFI_Handler* h = StageHandler(reg, stage);
+  XLA_FFI_Handler* h = StageHandler(c->handlers, stage);
   if (h == nullptr) {   // optional stage not provided: nothing to do
     if (err && err_len) err[0] = '\0';
     return 0;
   }
-  XLA_FFI_InvokeContext ctx;
-  ctx.stream = stage >= XLA_FFI_ExecutionStage_INITIALIZE ? stream : nullptr;
-  ctx.device_ordinal = device_ordinal;
-  ctx.state = &c->state;
+  c->ctx.stream = stage >= XLA_FFI_ExecutionStage_INITIALIZE ? stream : nullptr;
+  c->ctx.device_ordinal = device_ordinal;
+  c->ctx.state = &c->state;
+  if (stage == XLA_FFI_ExecutionStage_EXECUTE) {
+    if (!c->have_frame) Build(*c, /*null_data=*/false, &c->ctx, XLA_FFI_ExecutionStage_EXECUTE, &c->frame);
+    c->have_frame = true;
+    return Finish(h(&c->frame.frame), err, err_len);
+  }
   BuiltFrame built;
-  Build(*c, stage == XLA_FFI_ExecutionStage_INSTANTIATE, &ctx, static_cast<XLA_FFI_ExecutionStage>(stage), &built);
+  Build(*c, stage == XLA_FFI_ExecutionStage_INSTANTIATE, &c->ctx, static_cast<XLA_FFI_ExecutionStage>(stage), &built);
   return Finish(h(&built.frame), err, err_len);
 }
 

@@ -126,6 +126,7 @@ class FfiCall:
     def __init__(self, target: str, operands: Sequence, results: Sequence, attrs: dict):
         _native.ensure_registered()
         self._h = _native.mock.mockffi_call_new(target.encode())
+        self._err = _err_buf()              # of `execute`, kept: a site is executed many times
         self.target = target
         self._keep = []
         for op in operands:
@@ -177,8 +178,9 @@ class FfiCall:
         self._check(_native.mock.mockffi_call_run(self._h, stream, device, err, len(err)), err)
 
     def execute(self, stream: int = 0, device: int = 0) -> None:
-        err = _err_buf()
-        self._check(_native.mock.mockffi_call_execute(self._h, stream, device, err, len(err)), err)
+        rc = _native.mock.mockffi_call_execute(self._h, stream, device, self._err, 1024)
+        if rc != 0:
+            self._check(rc, self._err)
 
     def set_operand(self, index: int, tensor) -> None:
         _native.mock.mockffi_call_set_arg_data(self._h, index, tensor.data_ptr())
