@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   };
 #pragma unroll
   for (int j = 0; j < kAtOnce; ++j) add(first_max[j], first_sum[j], first_values[j]);
-#pragma unroll 4
+#pragma unroll 8
   for (int p = part + kAtOnce * kParts; p < pieces; p += kParts) {
     const float* slot = slot_of(p);
     const float piece_max = slot[L::kRows * kDim + row], piece_sum = slot[L::kRows * kDim + L::kRows + row];
@@ -921,6 +921,9 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + unit - 1) / unit + extra : 1);
   int64_t grid = static_cast<int64_t>(DeviceSmCount()) * g_ctas_per_sm[code][shape];
   grid = grid < kMaxCtas ? grid : kMaxCtas;
+  // The second kernel walks through an item's pieces, so one is cut into 128 at most.
+  const int64_t items = a.batch * a.kv_heads * blocks;
+  grid = grid < items * 128 ? grid : items * 128;
   grid = grid < most ? grid : most;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // see griddep_wait() in the kernels

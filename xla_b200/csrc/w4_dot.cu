@@ -632,7 +632,10 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
   const int group_at = a.group == 32 ? 0 : a.group == 64 ? 1 : 2, scale_at = a.scale_dtype == kF16 ? 0 : a.scale_dtype == kBF16 ? 1 : 2;
   const auto& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
   const auto& ring = TheVariants().ring[a.x_dtype == kBF16][group_at];
-  int pick = 0;
+  // Every CTA converts all of x for a resident one.  Against four rows and more of it a CTA needs about six rows of weights
+  // for each, or the conversion costs more than the cheaper decoding saves (k 4096, resident against ring, in us: m 5, n
+  // 2400 12.6 against 10.4, n 10000 22.9 against 23.6; m 8, n 2400 16.7 against 12.3; m 3, n 2400 10.7 against 14.1).
+  int pick = a.m >= 4 && a.n < int64_t{6} * a.m * DeviceSmCount() ? kResidentShapes : 0;
   auto shape = [&](int i) -> const Variant& { return i < kResidentShapes ? resident[i] : ring[i - kResidentShapes]; };
   while (a.m > shape(pick).most || shape(pick).bytes(a.m, steps, step_group) > kSmemPerCta) ++pick;       // the last one always fits
   const Variant& v = shape(pick);
