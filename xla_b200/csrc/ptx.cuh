@@ -19,7 +19,7 @@ enum DeviceStatusBits : uint32_t {
   kStatusProbeTimeout = 1u << 4,      // a wait made to expire on purpose (host-visible status test)
   kStatusPeerTimeout = 1u << 5,       // gave up waiting for another rank's partial tile or end-of-call signal
   kStatusBadPage = 1u << 6,           // a page table entry or a length led outside of the cache
-  kStatusTileTimeout = 1u << 7,       // a warp gave up waiting for a tile of the cache
+  kStatusTileTimeout = 1u << 7,       // a warp gave up waiting for a tile of the cache, or for its part of x
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

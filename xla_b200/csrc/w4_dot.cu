@@ -45,7 +45,8 @@ struct W4Args {
   int32_t group_shift;                          // log2 of the 128-blocks of k in a group (groups of 128 and more) ...
   int32_t blocks_per_group;                     // ... or their number where it is no power of two
   int32_t rows, rows_left;                      // of a CTA: `rows`, and one more for the first `rows_left`
-  int32_t steps, per_round;                     // 128-blocks of k; blocks of rows whose sums fit shared memory
+  int32_t steps, per_round;                     // 128-blocks of k; blocks of rows whose sums fit shared memory, or steps of a phase
+  uint32_t* status;
   uint32_t piece_inverse;                       // 2^32 / (16 * steps), rounded up
   int32_t x_is_bf16, scale_dtype, bias_dtype, d_dtype, is_signed;
 };
@@ -534,15 +535,233 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
   }
 }
 
+// 9 to 32 rows of x that do not fit as a whole.  All warps of a CTA share a phase of x, a few steps of k for all rows, as it
+// is stored; the next one is on its way meanwhile.  A warp keeps its block of 32 weight rows from the first phase to the
+// last, alone or with others that take every so manieth step of it, and its sums in registers, so x is read once per CTA
+// (per 512 of its rows) where the rings above read it once per block of rows.
+template <typename T_, int kCols_>
+struct WideShape {
+  using T = T_;
+  static constexpr int kCols = kCols_, kWarps = 16, kStages = 3, kRows = 32, kStride = kRows + 4;
+  static constexpr int kRing = kWarps * kStages * 2048;
+  // Steps of a phase: as many as fit, twice, for every phase costs a barrier.
+  static int64_t Phase(int64_t m, int64_t steps) { return std::min<int64_t>(steps, (227 * 1024 - kRing - 64) / (2 * 256 * m)); }
+  static int64_t Bytes(int64_t m, int64_t steps, int64_t) { return kRing + 64 + m * std::max<int64_t>(2 * Phase(m, steps) * 256, kWarps * kStride * 4); }
+};
+
+template <int kGroup, typename S>
+__global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __grid_constant__ W4Args a) {
+  using T = typename S::T;
+  constexpr int kPerStep = 128 / kGroup, kWords = kGroup / 32, kCols = S::kCols, kWarps = S::kWarps;
+  extern __shared__ __align__(128) uint8_t smem[];
+  if (threadIdx.x == 0) griddep_launch_dependents();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const bool is_signed = a.is_signed != 0;
+  const uint32_t flip = is_signed ? 0x00080008u : 0u;
+  const int cta = blockIdx.x, first = cta * a.rows + min(cta, a.rows_left), last = first + a.rows + (cta < a.rows_left ? 1 : 0);
+  const int steps = a.steps, row_bytes = a.k / 2, phase_steps = a.per_round, phases = (steps + phase_steps - 1) / phase_steps;
+  uint8_t* ring = smem + warp * S::kStages * 2048;
+  uint64_t* arrived = reinterpret_cast<uint64_t*>(smem + S::kRing);          // of the two halves of the buffer of x
+  int* abort_flag = reinterpret_cast<int*>(arrived + 2);
+  uint8_t* x_buffer = smem + S::kRing + 64;
+  float* sums = reinterpret_cast<float*>(x_buffer);                          // at the end
+  const int x_step = a.m * 256;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    mbar_init(&arrived[0], kWarps * 32);
+    mbar_init(&arrived[1], kWarps * 32);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();
+
+  auto load_x = [&](int phase) {                            // by all threads; counted on the half's barrier when it has come
+    uint64_t* bar = &arrived[phase & 1];
+    if (phase < phases) {
+      const uint32_t dst = smem_u32(x_buffer) + (phase & 1) * (phase_steps * x_step);
+      const int begin = phase * phase_steps, pieces = min(phase_steps, steps - begin) * 16;
+      // A warp takes 32 neighbouring pieces of a row, so that it reads 512 bytes in a row.
+      for (int i = warp; i < (pieces + 31) / 32 * a.m; i += kWarps) {
+        const int part = i / a.m, r = i - part * a.m, c = part * 32 + lane, at = begin * 128 + c * 8;
+        if (c < pieces)
+          CopyAsync16OrZero(dst + c / 16 * x_step + InputPiece<kGroup>(r, c % 16), at < a.k ? static_cast<const uint16_t*>(a.x) + (r * a.k + at) : a.x, at < a.k);
+      }
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  };
+  uint32_t x_parity = 0;                                    // bit h: parity of the next wait for half h
+
+  for (int chunk = first; chunk < last; chunk += kWarps * S::kRows) {
+    const int rows = min(last - chunk, kWarps * S::kRows), blocks = (rows + S::kRows - 1) / S::kRows, shares = kWarps / blocks;
+    const int block = warp % blocks, share = warp / blocks;  // warps with share >= shares only help with x
+    const int row = chunk + block * S::kRows;
+    const bool works = share < shares;
+
+    const uint8_t* w_base = a.w + static_cast<int64_t>(row + g) * row_bytes + t * 16;
+    const int left = chunk + rows - row - g;
+    const uint32_t to = Kept(smem_u32(ring) + WeightPiece(g, t));
+    int load_step = works ? share : steps, load_stage = 0;
+    auto load = [&] {
+      if (load_step < steps) {
+        const bool there = load_step * 64 + t * 16 < row_bytes;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          CopyAsync16If(there && 8 * i < left, to + load_stage * 2048 + i * 512, w_base + (static_cast<int64_t>(8 * i) * row_bytes + load_step * 64));
+        load_step += shares;
+        load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    uint32_t scale[2][2], zero[2][2], row_at[2][2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(block * S::kRows + r * 16 + h * 8 + g, rows - 1)) * a.groups;
+    const uint8_t* scale_base = static_cast<const uint8_t*>(a.scale) + static_cast<int64_t>(chunk) * a.groups * (a.scale_dtype == kF32 ? 4 : 2);
+    const uint8_t* zero_base = a.zero + static_cast<int64_t>(chunk) * a.groups;
+    auto load_numbers = [&](int step) {
+      const uint32_t group = kGroup == 128 ? (a.group_shift >= 0 ? step >> a.group_shift : step / a.blocks_per_group) : step * kPerStep + t % kPerStep;
+      const bool there = kGroup == 128 || group < a.groups;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t at = row_at[r][h] + (there ? group : 0);
+          scale[r][h] = LoadBits<0>(scale_base, at, a.scale_dtype);
+          if (!there) scale[r][h] = 0;
+          zero[r][h] = 8;
+          if (!is_signed) zero[r][h] = zero_base[at] & 15u;
+        }
+    };
+    __syncthreads();                                        // the sums of the chunk before, where x goes, have been read
+    load_x(0);
+    for (int s = 0; s < S::kStages - 1; ++s) load();
+    int step = share, stage = 0;
+    if (works && step < steps) load_numbers(step);
+    float acc[2][kCols][4] = {};
+
+#pragma unroll 1
+    for (int phase = 0; phase < phases; ++phase) {
+      __syncthreads();                                      // the phase before has been read by all warps
+      load_x(phase + 1);
+      (void)mbar_wait(&arrived[phase & 1], (x_parity >> (phase & 1)) & 1, abort_flag, a.status, kStatusTileTimeout);
+      x_parity ^= 1u << (phase & 1);
+      const uint32_t x_at = smem_u32(x_buffer) + (phase & 1) * (phase_steps * x_step);
+      const int end = min(steps, (phase + 1) * phase_steps);
+#pragma unroll 1
+      for (; works && step < end; step += shares) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+        __syncwarp();
+        load();
+        const uint32_t weights = smem_u32(ring) + stage * 2048, inputs = x_at + (step - phase * phase_steps) * x_step;
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+#pragma unroll
+        for (int group = 0; group < kPerStep; ++group) {
+          const int holder = (lane & ~3) | group;
+          Offset<T> decoder[2][2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) decoder[r][h].Set(kGroup == 128 || is_signed ? zero[r][h] : __shfl_sync(0xffffffffu, zero[r][h], holder));
+          float part[2][kCols][4] = {};
+          uint32_t w[2][2][kWords];
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int at = r * 16 + h * 8 + g;
+              if constexpr (kGroup == 128) {
+                const uint4 v = LoadShared16(weights + WeightPiece(at, t));
+                w[r][h][0] = v.x, w[r][h][1] = v.y, w[r][h][2] = v.z, w[r][h][3] = v.w;
+              } else if constexpr (kGroup == 64) {
+                const uint2 v = LoadShared8(weights + WeightPiece(at, group * 2 + t / 2) + t % 2 * 8);
+                w[r][h][0] = v.x, w[r][h][1] = v.y;
+              } else {
+                w[r][h][0] = LoadShared4(weights + WeightPiece(at, group) + t * 4);
+              }
+            }
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            uint32_t low[2][4], high[2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              decoder[r][0].Decode8(w[r][0][i], flip, low[r]);
+              decoder[r][1].Decode8(w[r][1][i], flip, high[r]);
+            }
+            const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? group * 8 + t * 2 + i : group * 4 + t;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              const uint4 b = Paired(LoadShared16(inputs + InputPiece<kGroup>(min(c * 8 + g, a.m - 1), piece)));
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                Mma<T>(part[r][c], low[r][0], high[r][0], low[r][1], high[r][1], b.x, b.y);
+                Mma<T>(part[r][c], low[r][2], high[r][2], low[r][3], high[r][3], b.z, b.w);
+              }
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float s0 = ValueOf<0>(scale[r][0], a.scale_dtype), s1 = ValueOf<0>(scale[r][1], a.scale_dtype);
+            if (kGroup < 128) s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              acc[r][c][0] = fmaf(part[r][c][0], s0, acc[r][c][0]), acc[r][c][1] = fmaf(part[r][c][1], s0, acc[r][c][1]);
+              acc[r][c][2] = fmaf(part[r][c][2], s1, acc[r][c][2]), acc[r][c][3] = fmaf(part[r][c][3], s1, acc[r][c][3]);
+            }
+          }
+        }
+        if (step + shares < steps) load_numbers(step + shares);
+      }
+    }
+    // The half that the last load_x counted on without loading is waited for, too, so that every chunk begins alike.
+    (void)mbar_wait(&arrived[phases & 1], (x_parity >> (phases & 1)) & 1, abort_flag, a.status, kStatusTileTimeout);
+    x_parity ^= 1u << (phases & 1);
+    __syncthreads();                                        // x has been read: its place takes the sums
+    if (works) {
+      float* mine = sums + warp * a.m * S::kStride;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (c * 8 + 2 * t + e < a.m) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + g] = acc[r][c][e];
+              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + 8 + g] = acc[r][c][e + 2];
+            }
+          }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < rows * a.m; i += kWarps * 32) {
+      const int x_row = i / rows, in_chunk = i - x_row * rows, at = chunk + in_chunk;
+      const float* part = sums + (in_chunk / S::kRows * a.m + x_row) * S::kStride + in_chunk % S::kRows;
+      float y = 0.0f;
+#pragma unroll 1
+      for (int w = 0; w < shares; ++w) y += part[w * blocks * a.m * S::kStride];
+      if (a.bias != nullptr) y += ValueOf<0>(LoadBits<0>(a.bias, at, a.bias_dtype), a.bias_dtype);
+      const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
+      if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
+      else if (a.d_dtype == kF16) static_cast<__half*>(a.d)[place] = __float2half_rn(y);
+      else static_cast<float*>(a.d)[place] = y;
+    }
+  }
+}
+
 struct Variant {
   void (*kernel)(W4Args);
   int64_t (*bytes)(int64_t m, int64_t steps, int64_t group);
-  int most, rows, warps, sums, registers;        // most: rows of x; sums: floats for those of a round
+  int64_t (*per_round)(int64_t m, int64_t steps);
+  int most, rows, warps, registers;              // most: rows of x
 };
 constexpr int64_t kSmemPerSm = 228 * 1024, kSmemPerCta = 227 * 1024, kSmemReserved = 1024;
 template <int kGroup, int kScale, int kSign, typename S>
 Variant Make() {
-  return {w4_dot_kernel<kGroup, kScale, kSign, S>, S::Bytes, 8 * S::kCols, S::kRows, S::kWarps, S::kSums / (S::kWarps * S::kStride), 0};
+  return {w4_dot_kernel<kGroup, kScale, kSign, S>, S::Bytes, [](int64_t m, int64_t) -> int64_t { return S::kSums / (S::kWarps * S::kStride) / m; }, 8 * S::kCols, S::kRows, S::kWarps, 0};
+}
+template <int kGroup, typename S>
+Variant MakeWide() {
+  return {w4_dot_wide_kernel<kGroup, S>, S::Bytes, S::Phase, 8 * S::kCols, S::kRows, S::kWarps, 0};
 }
 // In order of preference: the first that takes m rows of x and fits shared memory.  Without a resident x a CTA reads it once
 // per block of rows, m / (4 * tiles) bytes of it for a byte of weights.
@@ -571,8 +790,8 @@ struct Variants {
   template <int kGroup, typename T>
   void FillRing(Variant* to) {
     to[0] = Make<kGroup, 0, 2, Shape<2, 1, 8, 4, T>>();
-    to[1] = Make<kGroup, 0, 2, Shape<4, 2, 4, 4, T>>();
-    to[2] = Make<kGroup, 0, 2, Shape<4, 4, 4, 4, T>>();
+    to[1] = MakeWide<kGroup, WideShape<T, 2>>();
+    to[2] = MakeWide<kGroup, WideShape<T, 4>>();
     to[3] = Make<kGroup, 0, 2, Shape<2, 8, 4, 2, T>>();
   }
   Variants() {
@@ -651,7 +870,7 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
   const W4Args args{a.x, static_cast<const uint8_t*>(a.w), a.scale, static_cast<const uint8_t*>(a.zero), a.epilogue == B200SD_EPILOGUE_BIAS ? a.bias : nullptr, a.d,
                     static_cast<int32_t>(a.m), static_cast<int32_t>(a.n), static_cast<int32_t>(a.k), static_cast<int32_t>(a.k / a.group),
                     group_shift, static_cast<int32_t>(blocks_per_group),
-                    static_cast<int32_t>(a.n / ctas), static_cast<int32_t>(a.n % ctas), static_cast<int32_t>(steps), v.sums / static_cast<int32_t>(a.m),
+                    static_cast<int32_t>(a.n / ctas), static_cast<int32_t>(a.n % ctas), static_cast<int32_t>(steps), static_cast<int32_t>(v.per_round(a.m, steps)), StatusWordPtr(),
                     0xffffffffu / static_cast<uint32_t>(steps * 16) + 1, a.x_dtype == kBF16, a.scale_dtype, a.bias_dtype, a.d_dtype, a.weight_type == kS4};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // see griddep_wait() in the kernel
