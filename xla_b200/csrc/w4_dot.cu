@@ -535,8 +535,8 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
   }
 }
 
-// 9 to 32 rows of x that do not fit as a whole.  All warps of a CTA share a phase of x, a few steps of k for all rows, as it
-// is stored; the next one is on its way meanwhile.  A warp keeps its block of 32 weight rows from the first phase to the
+// 9 to 32 rows of x that do not fit as a whole.  All warps of a CTA share a phase of x, some steps of k for all rows, as it
+// is stored (one bulk copy per row); the next one is on its way meanwhile.  A warp keeps its block of 32 weight rows from the first phase to the
 // last, alone or with others that take every so manieth step of it, and its sums in registers, so x is read once per CTA
 // (per 512 of its rows) where the rings above read it once per block of rows.
 template <typename T_, int kCols_>
@@ -545,8 +545,8 @@ struct WideShape {
   static constexpr int kCols = kCols_, kWarps = 16, kStages = 3, kRows = 32, kStride = kRows + 4;
   static constexpr int kRing = kWarps * kStages * 2048;
   // Steps of a phase: as many as fit, twice, for every phase costs a barrier.
-  static int64_t Phase(int64_t m, int64_t steps) { return std::min<int64_t>(steps, (227 * 1024 - kRing - 64) / (2 * 256 * m)); }
-  static int64_t Bytes(int64_t m, int64_t steps, int64_t) { return kRing + 64 + m * std::max<int64_t>(2 * Phase(m, steps) * 256, kWarps * kStride * 4); }
+  static int64_t Phase(int64_t m, int64_t steps) { return std::min<int64_t>(steps, ((227 * 1024 - kRing - 64) / (2 * m) - 16) / 256); }
+  static int64_t Bytes(int64_t m, int64_t steps, int64_t) { return kRing + 64 + m * std::max<int64_t>(2 * (Phase(m, steps) * 256 + 16), kWarps * kStride * 4); }
 };
 
 template <int kGroup, typename S>
@@ -565,31 +565,35 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
   int* abort_flag = reinterpret_cast<int*>(arrived + 2);
   uint8_t* x_buffer = smem + S::kRing + 64;
   float* sums = reinterpret_cast<float*>(x_buffer);                          // at the end
-  const int x_step = a.m * 256;
+  const int x_pitch = phase_steps * 256 + 16;               // bytes between two rows of x in a phase: neighbours not in the same banks
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    mbar_init(&arrived[0], kWarps * 32);
-    mbar_init(&arrived[1], kWarps * 32);
+    mbar_init(&arrived[0], 1);
+    mbar_init(&arrived[1], 1);
     fence_mbar_init();
   }
   __syncthreads();
   griddep_wait();
 
-  auto load_x = [&](int phase) {                            // by all threads; counted on the half's barrier when it has come
-    uint64_t* bar = &arrived[phase & 1];
-    if (phase < phases) {
-      const uint32_t dst = smem_u32(x_buffer) + (phase & 1) * (phase_steps * x_step);
-      const int begin = phase * phase_steps, pieces = min(phase_steps, steps - begin) * 16;
-      // A warp takes 32 neighbouring pieces of a row, so that it reads 512 bytes in a row.
-      for (int i = warp; i < (pieces + 31) / 32 * a.m; i += kWarps) {
-        const int part = i / a.m, r = i - part * a.m, c = part * 32 + lane, at = begin * 128 + c * 8;
-        if (c < pieces)
-          CopyAsync16OrZero(dst + c / 16 * x_step + InputPiece<kGroup>(r, c % 16), at < a.k ? static_cast<const uint16_t*>(a.x) + (r * a.k + at) : a.x, at < a.k);
-      }
+  auto load_x = [&](int phase) {                            // one copy per row, by the first warp; and zeros behind the end of k
+    if (phase >= phases) return;
+    uint8_t* to = x_buffer + (phase & 1) * (a.m * x_pitch);
+    const int begin = phase * phase_steps * 128, end = min(a.k, begin + phase_steps * 128), bytes = (end - begin) * 2;
+    if (warp == 0) {
+      if (lane == 0) mbar_arrive_expect_tx(&arrived[phase & 1], a.m * bytes);
+      __syncwarp();
+      if (lane < a.m)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to + lane * x_pitch)),
+                     "l"(static_cast<const uint16_t*>(a.x) + (lane * static_cast<int64_t>(a.k) + begin)), "r"(bytes), "r"(smem_u32(&arrived[phase & 1])) : "memory");
     }
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    const int missing = ((end + 127) / 128 * 128 - end) * 2 / 16;        // pieces of 16 bytes; the next barrier comes before their use
+    for (int i = threadIdx.x; i < a.m * missing; i += kWarps * 32)
+      *reinterpret_cast<uint4*>(to + i / missing * x_pitch + bytes + i % missing * 16) = make_uint4(0, 0, 0, 0);
   };
   uint32_t x_parity = 0;                                    // bit h: parity of the next wait for half h
+  uint32_t row_offset[kCols];                               // of this lane's rows of x; behind the last one any will do
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) row_offset[c] = min(c * 8 + g, a.m - 1) * x_pitch;
 
   for (int chunk = first; chunk < last; chunk += kWarps * S::kRows) {
     const int rows = min(last - chunk, kWarps * S::kRows), blocks = (rows + S::kRows - 1) / S::kRows, shares = kWarps / blocks;
@@ -646,14 +650,14 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
       load_x(phase + 1);
       (void)mbar_wait(&arrived[phase & 1], (x_parity >> (phase & 1)) & 1, abort_flag, a.status, kStatusTileTimeout);
       x_parity ^= 1u << (phase & 1);
-      const uint32_t x_at = smem_u32(x_buffer) + (phase & 1) * (phase_steps * x_step);
+      const uint32_t x_at = smem_u32(x_buffer) + (phase & 1) * (a.m * x_pitch) + t * (kGroup == 128 ? 64 : kGroup == 64 ? 32 : 16);
       const int end = min(steps, (phase + 1) * phase_steps);
 #pragma unroll 1
       for (; works && step < end; step += shares) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
         __syncwarp();
         load();
-        const uint32_t weights = smem_u32(ring) + stage * 2048, inputs = x_at + (step - phase * phase_steps) * x_step;
+        const uint32_t weights = smem_u32(ring) + stage * 2048, inputs = x_at + (step - phase * phase_steps) * 256;
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
 #pragma unroll
         for (int group = 0; group < kPerStep; ++group) {
@@ -688,10 +692,9 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
               decoder[r][0].Decode8(w[r][0][i], flip, low[r]);
               decoder[r][1].Decode8(w[r][1][i], flip, high[r]);
             }
-            const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? group * 8 + t * 2 + i : group * 4 + t;
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
-              const uint4 b = Paired(LoadShared16(inputs + InputPiece<kGroup>(min(c * 8 + g, a.m - 1), piece)));
+              const uint4 b = Paired(LoadShared16(inputs + row_offset[c] + (group * (kGroup / 8) + i) * 16));
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 Mma<T>(part[r][c], low[r][0], high[r][0], low[r][1], high[r][1], b.x, b.y);
@@ -713,9 +716,6 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
         if (step + shares < steps) load_numbers(step + shares);
       }
     }
-    // The half that the last load_x counted on without loading is waited for, too, so that every chunk begins alike.
-    (void)mbar_wait(&arrived[phases & 1], (x_parity >> (phases & 1)) & 1, abort_flag, a.status, kStatusTileTimeout);
-    x_parity ^= 1u << (phases & 1);
     __syncthreads();                                        // x has been read: its place takes the sums
     if (works) {
       float* mine = sums + warp * a.m * S::kStride;
