@@ -82,6 +82,8 @@ def test_attention_frames():
                dict(workspace=False), dict(code=BF16), dict(page=48), dict(width=1 << 27), dict(pages=1 << 31)):
         _refused(INVALID, _attend, **kw)
     _refused(UNIMPLEMENTED, _attend, q=(3, 65, 4, 64))
+    _refused(UNIMPLEMENTED, _attend, q=(4096, 64, 4096, 256), dim=256, batch=4096, kv_heads=512)     # 2^27 items; 2^26 are the most
+    _attend(q=(4096, 64, 4096, 64), batch=4096, kv_heads=512).instantiate()
     _refused(INVALID, lambda: FfiCall("b200$paged_attention$kv8", [Buffer(BF16, (3, 1, 4, 64))] + _cache(), [Buffer(BF16, (3, 1, 4, 64)), Buffer(S8, (64,))], {}))
 
 

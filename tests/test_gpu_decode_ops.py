@@ -68,6 +68,65 @@ def test_dot_w4(cuda_device, m, n, k, group, dtype, zeros, bias):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("m,n,k,group,dtype,zeros,bias", [
+    (1, 19000, 4096, 128, F16, False, False),      # one or two rows of x against many rows of weights: x is converted first
+    (1, 40000, 4096, 256, BF16, True, True),       # more blocks of rows than the sums have room for
+    (1, 4800, 4224, 32, BF16, False, True),
+    (1, 19000, 4160, 64, F16, True, False),        # k ends inside a step
+    (2, 28500, 4096, 128, BF16, False, True),
+    (2, 9600, 4128, 32, F16, True, True),
+    (2, 28500, 12288, 384, BF16, True, False),
+    (1, 4800, 32768, 32, F16, False, False),       # ... which does not fit any more
+    (20, 80000, 160, 32, BF16, True, True),        # more rows than a CTA's warps take at once
+    (32, 76300, 2080, 32, F16, False, True),       # ... and x in several phases, k ending inside a step
+    (3, 75777, 96, 32, BF16, False, False),
+    (12, 1000, 5152, 32, BF16, True, False),
+    (9, 150, 28672, 128, F16, True, True),
+    (32, 2500, 11008, 64, BF16, False, True),
+    (47, 2400, 4160, 64, BF16, False, True),
+])
+def test_dot_w4_large(cuda_device, m, n, k, group, dtype, zeros, bias):
+    inputs = _dot_inputs(cuda_device, m, n, k, group, dtype, zeros, bias, seed=m + n + k)
+    x, w, scale, zero, b = inputs
+    _check_dot(xla_b200.dot_w4(x, w, scale, zero=zero, bias=b), inputs, k)
+    _check_dot(xla_b200.dot_w4(x, w, scale, zero=zero, bias=b, out_dtype=F32), inputs, k)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("scale_dtype", [F32, F16, BF16])
+def test_dot_w4_scale_types_of_many_rows(cuda_device, scale_dtype, group):
+    for dtype, zeros in ((BF16, False), (F16, True)):
+        inputs = _dot_inputs(cuda_device, 1, 19000, 4096, group, dtype, zeros, False, scale_dtype)
+        _check_dot(xla_b200.dot_w4(*inputs[:3], zero=inputs[3]), inputs, 4096)
+
+
+def test_dot_w4_many_rows_large_magnitudes_and_infinities(cuda_device):
+    x, w, scale, _, _ = _dot_inputs(cuda_device, 2, 9600, 4096, 32, BF16, False, False)
+    x[0] *= 2.0 ** 100
+    x[1] *= 2.0 ** -100
+    _check_dot(xla_b200.dot_w4(x, w, scale, out_dtype=F32), [x, w, scale, None, None], 4096)
+    for value in (math.inf, -math.inf, math.nan):
+        x[1, 17] = value
+        out = xla_b200.dot_w4(x, w, scale, out_dtype=F32)
+        _check_dot(out[:1], [x[:1], w, scale, None, None], 4096)
+        want = value * ref.weights(w, None, 32)[:, 17]
+        assert torch.equal(out[1].isposinf(), want.isposinf()) and torch.equal(out[1].isneginf(), want.isneginf()) and torch.equal(out[1].isnan(), want.isnan())
+
+
+def test_dot_w4_many_rows_one_value_at_a_time(cuda_device):
+    """Powers of two at one place of k: exact, for every nibble and zero point."""
+    n, k = 4800, 4096
+    w = (torch.arange(n * k // 2, device=cuda_device) * 2654435761 // 65536 % 256).to(torch.uint8).reshape(n, k // 2)
+    scale = torch.ones((n, k // 32), dtype=F32, device=cuda_device)
+    for zero in (None, (torch.arange(n * k // 32, device=cuda_device) % 16).to(torch.uint8).reshape(n, k // 32)):
+        full = ref.weights(w, zero, 32)
+        for at in (0, 1, 2, 3, 4, 5, 6, 7, 45, 127, 128, 2047, 4095):
+            x = torch.zeros((1, k), dtype=F16, device=cuda_device)
+            x[0, at] = 2.0 ** (at % 5)
+            assert torch.equal(xla_b200.dot_w4(x, w, scale, zero=zero, out_dtype=F32)[0].double(), full[:, at] * 2.0 ** (at % 5))
+
+
 @pytest.mark.parametrize("scale_dtype", [F32, F16, BF16])
 def test_dot_w4_scale_types(cuda_device, scale_dtype):
     for dtype in (BF16, F16):
@@ -149,6 +208,20 @@ def test_append(cuda_device, batch, new, kv_heads, dim, page, lens, code, dtype,
     args, fresh = _append_inputs(cuda_device, batch, new, kv_heads, dim, page, lens, code, dtype, new_lens, seed=sum(lens))
     _check_append(args, fresh)
     _check_append(args, fresh)          # again at the same place: the same cache
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("batch,new,kv_heads,dim,page,lens,code,dtype,new_lens", [
+    (1, 300, 1, 256, 128, [310], E4M3, BF16, None),           # a lane has more pieces than it keeps
+    (2, 130, 2, 16, 16, [133, 140], E5M2, F16, [130, 9]),     # nine pages of one call, several to a block
+    (3, 70, 2, 64, 32, [70, 100, 69], S8, BF16, [70, 70, 69]),
+    (100, 1, 1, 32, 16, list(range(100)), E4M3, F16, [min(i, 1) for i in range(100)]),
+])
+def test_append_many_pages(cuda_device, batch, new, kv_heads, dim, page, lens, code, dtype, new_lens):
+    args, fresh = _append_inputs(cuda_device, batch, new, kv_heads, dim, page, lens, code, dtype, new_lens, seed=sum(lens))
+    _check_append(args, fresh)
+    args[0][0, 0, 0, 3], args[1][0, -1, 0, 5], args[0][-1, -1, -1, -1] = math.inf, -math.inf, math.nan
+    _check_append(args, fresh)
     assert _status() == 0
 
 
@@ -258,6 +331,31 @@ def test_attention_of_long_and_short_sequences_together(cuda_device):
         _check_attention(args, [min(n, new) for n in (3, 20000, 64, 0, 7001)])
     _check_attention(_attention_inputs(cuda_device, 6, 3, 64, 16, [9000], 1, S8, BF16), window=5000)
     _check_attention(_attention_inputs(cuda_device, 2, 1, 256, 128, [6000, 1], 1, E4M3, BF16))
+
+
+def test_attention_of_many_sequences(cuda_device):
+    """More sequences than a warp has lanes, their work in shares that begin and end anywhere."""
+    for heads, kv_heads, dim, new, code in ((8, 2, 64, 1, E4M3), (16, 1, 128, 2, S8), (2, 2, 256, 1, E5M2)):
+        g = torch.Generator().manual_seed(dim)
+        lens = (torch.randint(0, 900, (70,), generator=g) * (torch.rand(70, generator=g) < 0.8)).tolist()
+        lens[33] = 3000
+        args = _attention_inputs(cuda_device, heads, kv_heads, dim, 32, lens, new, code, BF16)
+        _check_attention(args, [min(n, new) for n in lens])
+        _check_attention(args, [min(n, new) for n in lens], window=200)
+    assert _status() == 0
+
+
+def test_attention_keeps_a_bad_page_scale_to_the_rows_that_see_it(cuda_device):
+    """The second drafted token opens a page whose scales are no numbers: the first token's rows do not see it."""
+    for bad in (math.nan, math.inf):
+        args = _attention_inputs(cuda_device, 4, 2, 128, 16, [33], 2, E4M3, BF16)
+        want, want_lse, size, slack = ref.attention(*args)
+        for scales in args[3:5]:
+            scales[int(args[5][0, 2])] = bad                 # position 32
+            got, lse = xla_b200.paged_attention_kv8(*args, return_lse=True)
+            assert bool(((got.double() - want).abs() <= _attention_tolerance(want, size, slack, got.dtype))[0, 0].all())
+            assert bool(((lse.double() - want_lse).abs() <= slack + 2.0 ** -18 + want_lse.abs() * 2.0 ** -22)[0, 0].all())
+            assert torch.equal(torch.isfinite(got[0, 1]), torch.isfinite(ref.attention(*args)[0][0, 1]))
 
 
 def test_attention_scales_and_sharp_rows(cuda_device):

@@ -92,7 +92,7 @@ struct PageWork {
   uint32_t inverse_chunks;
 
   __device__ __forceinline__ uint4 Load(int c) const {
-    const int t = chunks == 1 ? c : static_cast<int>(__umulhi(c, inverse_chunks)), d = (c - t * chunks) * 8;      // c below 2^13
+    const int t = static_cast<int>(__umulhi(c, inverse_chunks)), d = (c - t * chunks) * 8;      // c below 2^13, two chunks at least
     return *reinterpret_cast<const uint4*>(rows + t * row_stride + d);
   }
   // The rounding of everything, by lanes `lane` of `lanes`; `kept` are the first chunks of this lane.

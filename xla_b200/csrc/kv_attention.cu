@@ -43,6 +43,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                       // tokens of a warp's step
 constexpr int kMaxCtas = 148 * 5;               // of one launch; bounds the workspace
+constexpr int64_t kMostItems = 1 << 26;         // of a launch: an item is at least one unit and less than 17
 constexpr float kLift = 9.0f;                   // binary digits that a row's largest weight is lifted by ...
 constexpr float kSlack = 6.0f;                  // ... and that a later one may pass it by: together below f16's 2^15.99
 
@@ -353,7 +354,8 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     if (pending == 0) return;
     if (raw) {
       const float size = fminf(fmaxf(fabsf(of_tile.w), 0x1p-100f), 0x1p100f);
-      of_tile = page_of >= 0 ? make_float4(of_tile.x, log2f(size), 1.0f / size, of_tile.w / size) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+      // x + (x - x): an infinite scale makes infinities of both signs of a key, whose product is no number.
+      of_tile = page_of >= 0 ? make_float4(of_tile.x + (of_tile.x - of_tile.x), log2f(size), 1.0f / size, of_tile.w / size) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
       raw = false;
     }
     const int at = lane - (batch_at - pending * kPair);    // this lane's tile among the pending ones
@@ -567,7 +569,13 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
           for (int e = 0; e < 4; ++e) {
             s[i][n][e] = Exp2(s[i][n][e] - from[e % 2]);
             sum[n][e % 2] = fmaf(s[i][n][e], num[i].z, sum[n][e % 2]);
-            s[i][n][e] *= num[i].w;
+          }
+          if (num[i].w != 1.0f) {                          // a negative scale, or one that is no number: not for rows that do not see the token
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int32_t at = pos + i * kTile + kr + (e / 2) * 8;
+              s[i][n][e] = at < row_end[n][e % 2] && at >= row_begin[n][e % 2] ? s[i][n][e] * num[i].w : 0.0f;
+            }
           }
           const __half2 l = __floats2half2_rn(s[i][n][0], s[i][n][1]), h = __floats2half2_rn(s[i][n][2], s[i][n][3]);
           p[i][n][0] = Transpose8x8(*reinterpret_cast<const uint32_t*>(&l));
@@ -873,6 +881,8 @@ Status ValidatePagedAttention(const B200SD_PagedAttention& a, bool check_pointer
   if (a.new_tokens > 64) return Status::Error(kUnimplemented, "more than 64 new tokens for a sequence");
   if (a.window < 0) return bad("window must not be negative");
   if (!(a.softmax_scale - a.softmax_scale == 0.0f)) return bad("softmax_scale must be finite");
+  const int64_t rows = a.new_tokens * (a.heads / a.kv_heads), block = 8 * kVariants[0][ShapeIndex(a.head_dim, rows)].row_tiles;
+  if (a.batch * a.kv_heads * ((rows + block - 1) / block) > kMostItems) return Status::Error(kUnimplemented, "too many queries for one call");
   if (!check_pointers || a.batch == 0 || a.new_tokens == 0) return Status::Ok();
   if (a.q == nullptr || a.out == nullptr) return bad("q and out must not be null");
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) % 16) return bad("q and out must be 16-byte aligned");

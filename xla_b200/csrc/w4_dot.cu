@@ -99,21 +99,16 @@ __device__ __forceinline__ uint32_t MaskXor(uint32_t w, uint32_t mask, uint32_t 
   return v;
 }
 
-// How a word's nibbles become operands.  Subnormal: as they are, see above; `flip` (8 for two's complement) turns -8 .. 7
-// into 0 .. 15 with zero point 8.
-struct Subnormal {
-  using Operand = __half;
-  __device__ void Set(uint32_t) {}
-  __device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, uint32_t (&v)[4]) const {
-    v[0] = MaskXor(w, 0x000f000fu, flip), v[1] = MaskXor(w, 0x00f000f0u, flip << 4);
-    v[2] = MaskXor(w >> 8, 0x000f000fu, flip), v[3] = MaskXor(w >> 8, 0x00f000f0u, flip << 4);
-  }
-};
-// w - z exactly.  The offsets -(1024 + z), -(64 + z) and -(128 + z) of one weight row and group have z in their low bits,
+// How a word's nibbles become operands; `flip` (8 for two's complement) turns -8 .. 7 into 0 .. 15 with zero point 8.
+// As subnormals, see above:
+__device__ __forceinline__ void DecodeSubnormal(uint32_t w, uint32_t flip, uint32_t (&v)[4]) {
+  v[0] = MaskXor(w, 0x000f000fu, flip), v[1] = MaskXor(w, 0x00f000f0u, flip << 4);
+  v[2] = MaskXor(w >> 8, 0x000f000fu, flip), v[3] = MaskXor(w >> 8, 0x00f000f0u, flip << 4);
+}
+// As w - z, exactly.  The offsets -(1024 + z), -(64 + z) and -(128 + z) of one weight row and group have z in their low bits,
 // so they are put together, not converted.
 template <typename T> struct Offset;
 template <> struct Offset<__half> {
-  using Operand = __half;
   uint32_t low, high;
   __device__ void Set(uint32_t z) { low = 0xe400e400u | z * 0x00010001u, high = 0xd400d400u | z * 0x00100010u; }
   __device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, uint32_t (&v)[4]) const {
@@ -127,7 +122,6 @@ template <> struct Offset<__half> {
   }
 };
 template <> struct Offset<__nv_bfloat16> {
-  using Operand = __nv_bfloat16;
   uint32_t low;
   __device__ void Set(uint32_t z) { low = 0xc300c300u | z * 0x00010001u; }
   __device__ __forceinline__ void Decode8(uint32_t w, uint32_t flip, uint32_t (&v)[4]) const {
@@ -149,23 +143,10 @@ __device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Weight row tiles of 16 of a unit, tiles of 8 rows of x, warps of a CTA, stages of a ring; T is the type of x in the
-// rings, void where x is resident.
-template <int kTiles_, int kCols_, int kWarps_, int kStages_, typename T_>
-struct Shape {
-  using T = T_;
-  static constexpr int kTiles = kTiles_, kCols = kCols_, kWarps = kWarps_, kStages = kStages_;
-  static constexpr bool kResident = std::is_void_v<T>;
-  static constexpr int kRows = 16 * kTiles;                 // weight rows of a unit
-  static constexpr int kStride = kRows + 4;                 // floats between two rows of x in the sums
-  static constexpr int kSums = kWarps * 8 * kCols * kStride;            // floats: one block for the most rows of x, more for fewer
-  static constexpr int kFactors = 16 * kCols;               // floats: the inverse of each resident row's power of two, its largest value
-  static int64_t Bytes(int64_t m, int64_t steps, int64_t group) {
-    const int64_t ring = kWarps * kStages * (kTiles * 1024 + (kResident ? 0 : m * 256));
-    const int64_t resident = kResident ? steps * m * 256 + steps * (128 / group) * ((m + 1) / 2 * 2) * 4 : 0;
-    return (kSums + kFactors) * 4 + ring + resident;
-  }
-};
+// Either kernel's unit is 32 weight rows, in two tiles of the products, by 128 of k.
+constexpr int kTiles = 2, kRows = 16 * kTiles, kStageBytes = kTiles * 1024;
+constexpr int kSumStride = kRows + 4;           // floats between two rows of x in the sums
+constexpr int kStages = 3;                      // of a warp's ring
 
 // Where 16-byte piece `c` of weight row `r` (64 bytes of a unit) and piece `c` of row `r` of x (256 bytes) lie: so that the
 // reads below have no bank conflicts.
@@ -188,7 +169,7 @@ __device__ __forceinline__ float2 Unpack(uint32_t w, bool is_bf16) {
 }
 
 // All of x to shared memory: `inputs` as paired, scaled f16, `factors` the inverse powers of two (0 for a row that is not
-// finite), `sums` [group][row] the sums of the scaled values over each group (each 128 of k for groups longer than that).
+// finite), `sums` [group][2] the sums of the scaled values over each group (each 128 of k for groups longer than that).
 // The copies are under way before the weights', so that they do not queue behind them; a thread works on the pieces that
 // it has copied itself, in place.  The loops are not unrolled: this code runs once, and its instructions are fetched cold.
 template <int kGroup, int kThreads>
@@ -216,7 +197,6 @@ struct Staging {
   // `top` [row] holds zeros on entry.
   __device__ __forceinline__ void Convert(float* factors, uint32_t* top, float* sums) const {
     const uint32_t lanes = threadIdx.x % 32 < 16 ? 0x0000ffffu : 0xffff0000u;       // 16 lanes in a row share r and the step
-    const int columns = (a.m + 1) / 2 * 2;
     int r, c;
     uint32_t at;
 #pragma unroll 1
@@ -243,7 +223,7 @@ struct Staging {
       float sum = ((f0.x + f0.y) + (f2.x + f2.y)) + 16.0f * ((f1.x + f1.y) + (f3.x + f3.y));
 #pragma unroll
       for (int o = kGroup / 16; o > 0; o /= 2) sum += __shfl_xor_sync(lanes, sum, o);
-      if (c % (kGroup / 8) == 0) sums[c / (kGroup / 8) * columns + r] = sum;
+      if (c % (kGroup / 8) == 0) sums[c / (kGroup / 8) * 2 + r] = sum;
       if (c == 0) factors[r] = bits >= 0x7f800000u ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
     }
     __syncthreads();
@@ -264,32 +244,39 @@ __device__ __noinline__ float PlainDot(const W4Args& a, int x_row, int row) {
   return y;
 }
 
-// kGroup: 32, 64 or 128 (which stands for its multiples too).  kScale: the scales' type, kSign: 1 for two's complement, 0
-// for zero points; ring variants have 0 and 2 there and go by the arguments.
-template <int kGroup, int kScale, int kSign, typename S>
-__global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
-  using Decoder = std::conditional_t<S::kResident, Subnormal, Offset<std::conditional_t<S::kResident, __half, typename S::T>>>;
-  using Operand = typename Decoder::Operand;
+struct Resident {
+  static constexpr int kWarps = 24, kMost = 2;              // kMost: rows of x
+  static constexpr int kBlocks = 8;                         // whose sums have room, for one row of x
+  static constexpr int kSums = kBlocks * kWarps * kSumStride;
+  // The inverse of each row's power of two, its largest value, and what is behind them up to whole lines of banks.
+  static constexpr int kHead = (kSums * 4 + 2 * kMost * 4 + 127) / 128 * 128, kRing = kWarps * kStages * kStageBytes;
+  static int64_t PerRound(int64_t m, int64_t) { return kBlocks / m; }
+  static int64_t Bytes(int64_t m, int64_t steps, int64_t group) { return kHead + kRing + steps * m * 256 + steps * (128 / group) * 2 * 4; }
+};
+
+// One or two rows of x, all of it in shared memory.  kGroup: 32, 64 or 128 (which stands for its multiples too).  kScale: the
+// scales' type, kSigned: two's complement, no zero points.
+template <int kGroup, int kScale, bool kSigned>
+__global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
+  using S = Resident;
   constexpr int kPerStep = 128 / kGroup;                    // groups of a step
   constexpr int kWords = kGroup / 32;                       // words of a lane in a group
-  constexpr int kTiles = S::kTiles, kCols = S::kCols, kWarps = S::kWarps;
-  const bool is_signed = kSign == 2 ? a.is_signed != 0 : kSign == 1;
+  constexpr int kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
   if (threadIdx.x == 0) griddep_launch_dependents();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int cta = blockIdx.x, first = cta * a.rows + min(cta, a.rows_left), last = first + a.rows + (cta < a.rows_left ? 1 : 0);
-  const int steps = a.steps, row_bytes = a.k / 2, blocks = (last - first + S::kRows - 1) / S::kRows, per_round = a.per_round;
-  const int stage_bytes = kTiles * 1024 + (S::kResident ? 0 : a.m * 256);
+  const int steps = a.steps, row_bytes = a.k / 2, blocks = (last - first + kRows - 1) / kRows, per_round = a.per_round;
   float* sums = reinterpret_cast<float*>(smem);
   float* factors = sums + S::kSums;
-  uint8_t* ring = smem + (S::kSums + S::kFactors) * 4 + warp * S::kStages * stage_bytes;
-  uint8_t* resident = smem + (S::kSums + S::kFactors) * 4 + kWarps * S::kStages * stage_bytes;
+  uint8_t* ring = smem + S::kHead + warp * kStages * kStageBytes;
+  uint8_t* resident = smem + S::kHead + S::kRing;
   float* group_sums = reinterpret_cast<float*>(resident + steps * a.m * 256);
-  const int columns = (a.m + 1) / 2 * 2;
-  const uint32_t flip = is_signed ? 0x00080008u : 0u;
+  constexpr int columns = 2;                                // of the group sums
+  constexpr uint32_t flip = kSigned ? 0x00080008u : 0u;
   // A CTA's rows of the weights and of the scales span less than 4 GiB, so 32-bit offsets from its first row do.
   const uint8_t* w_base = a.w + static_cast<int64_t>(first) * row_bytes;
-  const uint8_t* scale_base = static_cast<const uint8_t*>(a.scale) + static_cast<int64_t>(first) * a.groups * ((kScale == 0 ? a.scale_dtype : kScale) == kF32 ? 4 : 2);
+  const uint8_t* scale_base = static_cast<const uint8_t*>(a.scale) + static_cast<int64_t>(first) * a.groups * (kScale == kF32 ? 4 : 2);
   const uint8_t* zero_base = a.zero + static_cast<int64_t>(first) * a.groups;
 
   // A warp's units of a round of blocks are the warp-th, the (warp + warps)-th ... of the line (block, step): within a block
@@ -297,13 +284,13 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
   //
   // Loading: each lane brings piece `t` of rows g, g + 8, ... of a unit.  What lies behind the last row or the end of k is
   // not loaded: old bytes there are finite weights too, of rows that are not stored or against a 0 of x.
-  const uint32_t eight_rows = 8 * row_bytes, next_block = S::kRows * row_bytes - steps * 64;
+  const uint32_t eight_rows = 8 * row_bytes, next_block = kRows * row_bytes - steps * 64;
   int load_step = warp, load_block = 0, load_round = per_round, load_rows = last - first - g;
   uint32_t load_from = static_cast<uint32_t>(g) * row_bytes + warp * 64 + t * 16, load_to = Kept(smem_u32(ring) + WeightPiece(g, t));
   auto to_next_block = [&] {
     while (load_step >= steps && load_block < blocks) {
       ++load_block;
-      load_rows -= S::kRows;
+      load_rows -= kRows;
       load_step -= steps;
       load_from += next_block;
       if (load_block == load_round) {                       // every round starts with the warp-th unit
@@ -321,14 +308,6 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
 #pragma unroll
       for (int i = 0; i < 2 * kTiles; ++i)
         CopyAsync16If(8 * i < rows, dst + i * 512, w_base + (load_from + i * eight_rows));
-      if constexpr (!S::kResident) {
-#pragma unroll
-        for (int i = 0; i < 4 * kCols; ++i) {
-          const int r = i * 2 + lane / 16, c = lane % 16, at = load_step * 128 + c * 8;
-          if (r < a.m)
-            CopyAsync16OrZero(smem_u32(ring) + stage + kTiles * 1024 + InputPiece<kGroup>(r, c), at < a.k ? static_cast<const uint16_t*>(a.x) + (r * a.k + at) : a.x, at < a.k);
-        }
-      }
       load_step += kWarps;
       load_from += kWarps * 64;
       if (load_step >= steps) to_next_block();
@@ -349,78 +328,59 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
         const uint32_t at = row_at[r][h] + (there ? group : 0);
         scale[r][h] = LoadBits<kScale>(scale_base, at, a.scale_dtype);
         if (!there) scale[r][h] = 0;
-        if (!is_signed) zero[r][h] = zero_base[at] & 15u;
-        else if (!S::kResident) zero[r][h] = 8;
+        if (!kSigned) zero[r][h] = zero_base[at] & 15u;
       }
   };
   auto set_rows = [&](int block) {
-    const int row = min(block, blocks - 1) * S::kRows + g, most = last - first - 1;
+    const int row = min(block, blocks - 1) * kRows + g, most = last - first - 1;
 #pragma unroll
     for (int r = 0; r < kTiles; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(row + r * 16 + h * 8, most)) * a.groups;
   };
 
-  uint32_t* top = reinterpret_cast<uint32_t*>(factors + 8 * kCols);
-  if (S::kResident && threadIdx.x < 8 * kCols) top[threadIdx.x] = 0;
+  uint32_t* top = reinterpret_cast<uint32_t*>(factors + S::kMost);
+  if (threadIdx.x < S::kMost) top[threadIdx.x] = 0;
   __syncthreads();
   griddep_wait();
   const Staging<kGroup, kWarps * 32> staging(a, smem_u32(resident));
-  if constexpr (S::kResident) staging.Copy();
+  staging.Copy();
 #pragma unroll 1
-  for (int s = 0; s < S::kStages - 1; ++s) load(s * stage_bytes);
+  for (int s = 0; s < kStages - 1; ++s) load(s * kStageBytes);
   set_rows(0);
   load_numbers(min(warp, steps - 1));
-  if constexpr (S::kResident) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");       // this thread's part of x has come
-    staging.Convert(factors, top, group_sums);
-  }
+  asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");         // this thread's part of x has come
+  staging.Convert(factors, top, group_sums);
 
   // Places of this lane's words and of its pieces of x, of the sums that belong to them; behind the last row of x any will
   // do, its column is not stored.
-  uint32_t weight_at[kPerStep], input_at[kCols][4], sums_at[kCols];
+  uint32_t weight_at[kPerStep], input_at[4];
 #pragma unroll
   for (int i = 0; i < kPerStep; ++i)
     weight_at[i] = Kept(smem_u32(ring) + (kGroup == 128 ? WeightPiece(g, t) : kGroup == 64 ? WeightPiece(g, i * 2 + t / 2) + t % 2 * 8 : WeightPiece(g, i) + t * 4));
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? i / 2 * 8 + t * 2 + i % 2 : i * 4 + t;
-      input_at[c][i] = Kept((S::kResident ? smem_u32(resident) : smem_u32(ring) + kTiles * 1024) + InputPiece<kGroup>(min(c * 8 + g, a.m - 1), piece));
-    }
-    sums_at[c] = Kept(smem_u32(group_sums) + min(c * 8 + 2 * t, columns - 2) * 4);
+  for (int i = 0; i < 4; ++i) {
+    const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? i / 2 * 8 + t * 2 + i % 2 : i * 4 + t;
+    input_at[i] = Kept(smem_u32(resident) + InputPiece<kGroup>(min(g, a.m - 1), piece));
   }
+  const uint32_t sums_at = Kept(smem_u32(group_sums));
 
-  uint32_t stage = 0, load_stage = (S::kStages - 1) * stage_bytes;
+  uint32_t stage = 0, load_stage = (kStages - 1) * kStageBytes;
   for (int round = 0; round < blocks; round += per_round) {
     const int round_end = min(round + per_round, blocks);
     int step = warp;
     for (int block = round; block < round_end; ++block) {
-      float acc[kTiles][kCols][4] = {};
+      float acc[kTiles][4] = {};
       for (; step < steps; step += kWarps) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
         load(load_stage);
         load_stage = stage;
-        const uint32_t inputs = S::kResident ? step * (a.m * 256) : stage, sums_step = step * (kPerStep * columns * 4);
-        Decoder decoder[kTiles][2];
-        if (kGroup == 128) {
-#pragma unroll
-          for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) decoder[r][h].Set(zero[r][h]);
-        }
+        const uint32_t inputs = step * (a.m * 256), sums_step = step * (kPerStep * columns * 4);
 #pragma unroll
         for (int group = 0; group < kPerStep; ++group) {
           const int holder = (lane & ~3) | group;           // the lane with this group's numbers
-          if (kGroup < 128 && !S::kResident) {
-#pragma unroll
-            for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) decoder[r][h].Set(__shfl_sync(0xffffffffu, zero[r][h], holder));
-          }
-          float part[kTiles][kCols][4] = {};
+          float part[kTiles][4] = {};
           // The words of this group, of rows g and g + 8 of each tile.
           uint32_t w[kTiles][2][kWords];
 #pragma unroll
@@ -440,57 +400,33 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
             }
 #pragma unroll
           for (int i = 0; i < kWords; ++i) {
-            uint4 b[kCols];
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              b[c] = LoadShared16(input_at[c][group * kWords + i] + inputs);
-              if constexpr (!S::kResident) b[c] = Paired(b[c]);
-            }
+            const uint4 b = LoadShared16(input_at[group * kWords + i] + inputs);
 #pragma unroll
             for (int r = 0; r < kTiles; ++r) {
               uint32_t low[4], high[4];
-              decoder[r][0].Decode8(w[r][0][i], flip, low);
-              decoder[r][1].Decode8(w[r][1][i], flip, high);
-#pragma unroll
-              for (int c = 0; c < kCols; ++c) {
-                Mma<Operand>(part[r][c], low[0], high[0], low[1], high[1], b[c].x, b[c].y);
-                Mma<Operand>(part[r][c], low[2], high[2], low[3], high[3], b[c].z, b[c].w);
-              }
+              DecodeSubnormal(w[r][0][i], flip, low);
+              DecodeSubnormal(w[r][1][i], flip, high);
+              Mma<__half>(part[r], low[0], high[0], low[1], high[1], b.x, b.y);
+              Mma<__half>(part[r], low[2], high[2], low[3], high[3], b.z, b.w);
             }
           }
-          if constexpr (S::kResident) {                     // the zero points' share
-            float2 sum[kCols];
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              const uint2 v = LoadShared8(sums_at[c] + sums_step + group * (columns * 4));
-              sum[c] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
-            }
-#pragma unroll
-            for (int r = 0; r < kTiles; ++r) {
-              float z0 = -0x1p-21f, z1 = -0x1p-21f;          // -8 * 2^-24
-              if (!is_signed) {
-                z0 = -0x1p-24f * static_cast<float>(kGroup == 128 ? zero[r][0] : __shfl_sync(0xffffffffu, zero[r][0], holder));
-                z1 = -0x1p-24f * static_cast<float>(kGroup == 128 ? zero[r][1] : __shfl_sync(0xffffffffu, zero[r][1], holder));
-              }
-#pragma unroll
-              for (int c = 0; c < kCols; ++c) {
-                part[r][c][0] = fmaf(z0, sum[c].x, part[r][c][0]), part[r][c][1] = fmaf(z0, sum[c].y, part[r][c][1]);
-                part[r][c][2] = fmaf(z1, sum[c].x, part[r][c][2]), part[r][c][3] = fmaf(z1, sum[c].y, part[r][c][3]);
-              }
-            }
-          }
+          // The zero points' share, then the scales.
+          const uint2 sum_bits = LoadShared8(sums_at + sums_step + group * (columns * 4));
+          const float sum0 = __uint_as_float(sum_bits.x), sum1 = __uint_as_float(sum_bits.y);
 #pragma unroll
           for (int r = 0; r < kTiles; ++r) {
-            float s0 = ValueOf<kScale>(scale[r][0], a.scale_dtype), s1 = ValueOf<kScale>(scale[r][1], a.scale_dtype);
-            if (kGroup < 128) s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              acc[r][c][0] = fmaf(part[r][c][0], s0, acc[r][c][0]), acc[r][c][1] = fmaf(part[r][c][1], s0, acc[r][c][1]);
-              acc[r][c][2] = fmaf(part[r][c][2], s1, acc[r][c][2]), acc[r][c][3] = fmaf(part[r][c][3], s1, acc[r][c][3]);
+            float s0 = ValueOf<kScale>(scale[r][0], kScale), s1 = ValueOf<kScale>(scale[r][1], kScale);
+            float z0 = -0x1p-21f, z1 = -0x1p-21f;            // -8 * 2^-24
+            if (!kSigned) z0 = -0x1p-24f * static_cast<float>(zero[r][0]), z1 = -0x1p-24f * static_cast<float>(zero[r][1]);
+            if (kGroup < 128) {
+              s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
+              if (!kSigned) z0 = __shfl_sync(0xffffffffu, z0, holder), z1 = __shfl_sync(0xffffffffu, z1, holder);
             }
+            acc[r][0] = fmaf(fmaf(z0, sum0, part[r][0]), s0, acc[r][0]), acc[r][1] = fmaf(fmaf(z0, sum1, part[r][1]), s0, acc[r][1]);
+            acc[r][2] = fmaf(fmaf(z1, sum0, part[r][2]), s1, acc[r][2]), acc[r][3] = fmaf(fmaf(z1, sum1, part[r][3]), s1, acc[r][3]);
           }
         }
-        stage = stage == (S::kStages - 1) * stage_bytes ? 0 : stage + stage_bytes;
+        stage = stage == (kStages - 1) * kStageBytes ? 0 : stage + kStageBytes;
         if (step + kWarps < steps) load_numbers(step + kWarps);
       }
       step -= steps;
@@ -498,32 +434,30 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
       set_rows(block + 1);
       if (step < steps) load_numbers(step);
       // This warp's sums of the block, zeros where it had no unit of it.
-      float* mine = sums + ((block - round) * kWarps + warp) * a.m * S::kStride;
+      float* mine = sums + ((block - round) * kWarps + warp) * a.m * kSumStride;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
+      for (int e = 0; e < 2; ++e)
+        if (2 * t + e < a.m) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (c * 8 + 2 * t + e < a.m) {
-#pragma unroll
-            for (int r = 0; r < kTiles; ++r) {
-              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + g] = acc[r][c][e];
-              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + 8 + g] = acc[r][c][e + 2];
-            }
+          for (int r = 0; r < kTiles; ++r) {
+            mine[(2 * t + e) * kSumStride + r * 16 + g] = acc[r][e];
+            mine[(2 * t + e) * kSumStride + r * 16 + 8 + g] = acc[r][e + 2];
           }
+        }
     }
     __syncthreads();
-    const int rows = min(round_end * S::kRows, last - first) - round * S::kRows;
+    const int rows = min(round_end * kRows, last - first) - round * kRows;
 #pragma unroll 1
     for (int i = threadIdx.x; i < rows; i += kWarps * 32) {
-      const int at = first + round * S::kRows + i;
+      const int at = first + round * kRows + i;
       const float bias = a.bias != nullptr ? ValueOf<0>(LoadBits<0>(a.bias, at, a.bias_dtype), a.bias_dtype) : 0.0f;
 #pragma unroll 1
       for (int x_row = 0; x_row < a.m; ++x_row) {
-        const float* part = sums + (i / S::kRows * kWarps * a.m + x_row) * S::kStride + i % S::kRows;
+        const float* part = sums + (i / kRows * kWarps * a.m + x_row) * kSumStride + i % kRows;
         float y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) y += part[w * a.m * S::kStride];
-        if constexpr (S::kResident) y = factors[x_row] != 0.0f ? y * 0x1p24f * factors[x_row] : PlainDot(a, x_row, at);
+        for (int w = 0; w < kWarps; ++w) y += part[w * a.m * kSumStride];
+        y = factors[x_row] != 0.0f ? y * 0x1p24f * factors[x_row] : PlainDot(a, x_row, at);
         y += bias;
         const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
         if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
@@ -535,18 +469,18 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_kernel(const __grid_con
   }
 }
 
-// 9 to 32 rows of x that do not fit as a whole.  All warps of a CTA share a phase of x, some steps of k for all rows, as it
+// Up to 32 rows of x, as they are.  All warps of a CTA share a phase of x, some steps of k for all rows, as it
 // is stored (one bulk copy per row); the next one is on its way meanwhile.  A warp keeps its block of 32 weight rows from the first phase to the
 // last, alone or with others that take every so manieth step of it, and its sums in registers, so x is read once per CTA
 // (per 512 of its rows) where the rings above read it once per block of rows.
 template <typename T_, int kCols_>
 struct WideShape {
   using T = T_;
-  static constexpr int kCols = kCols_, kWarps = 16, kStages = 3, kRows = 32, kStride = kRows + 4;
-  static constexpr int kRing = kWarps * kStages * 2048;
+  static constexpr int kCols = kCols_, kWarps = 16;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
   // Steps of a phase: as many as fit, twice, for every phase costs a barrier.
   static int64_t Phase(int64_t m, int64_t steps) { return std::min<int64_t>(steps, ((227 * 1024 - kRing - 64) / (2 * m) - 16) / 256); }
-  static int64_t Bytes(int64_t m, int64_t steps, int64_t) { return kRing + 64 + m * std::max<int64_t>(2 * (Phase(m, steps) * 256 + 16), kWarps * kStride * 4); }
+  static int64_t Bytes(int64_t m, int64_t steps, int64_t) { return kRing + 64 + m * std::max<int64_t>(2 * (Phase(m, steps) * 256 + 16), kWarps * kSumStride * 4); }
 };
 
 template <int kGroup, typename S>
@@ -560,7 +494,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
   const uint32_t flip = is_signed ? 0x00080008u : 0u;
   const int cta = blockIdx.x, first = cta * a.rows + min(cta, a.rows_left), last = first + a.rows + (cta < a.rows_left ? 1 : 0);
   const int steps = a.steps, row_bytes = a.k / 2, phase_steps = a.per_round, phases = (steps + phase_steps - 1) / phase_steps;
-  uint8_t* ring = smem + warp * S::kStages * 2048;
+  uint8_t* ring = smem + warp * kStages * 2048;
   uint64_t* arrived = reinterpret_cast<uint64_t*>(smem + S::kRing);          // of the two halves of the buffer of x
   int* abort_flag = reinterpret_cast<int*>(arrived + 2);
   uint8_t* x_buffer = smem + S::kRing + 64;
@@ -595,10 +529,10 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
 #pragma unroll
   for (int c = 0; c < kCols; ++c) row_offset[c] = min(c * 8 + g, a.m - 1) * x_pitch;
 
-  for (int chunk = first; chunk < last; chunk += kWarps * S::kRows) {
-    const int rows = min(last - chunk, kWarps * S::kRows), blocks = (rows + S::kRows - 1) / S::kRows, shares = kWarps / blocks;
+  for (int chunk = first; chunk < last; chunk += kWarps * kRows) {
+    const int rows = min(last - chunk, kWarps * kRows), blocks = (rows + kRows - 1) / kRows, shares = kWarps / blocks;
     const int block = warp % blocks, share = warp / blocks;  // warps with share >= shares only help with x
-    const int row = chunk + block * S::kRows;
+    const int row = chunk + block * kRows;
     const bool works = share < shares;
 
     const uint8_t* w_base = a.w + static_cast<int64_t>(row + g) * row_bytes + t * 16;
@@ -612,7 +546,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
         for (int i = 0; i < 4; ++i)
           CopyAsync16If(there && 8 * i < left, to + load_stage * 2048 + i * 512, w_base + (static_cast<int64_t>(8 * i) * row_bytes + load_step * 64));
         load_step += shares;
-        load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
+        load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -620,7 +554,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(block * S::kRows + r * 16 + h * 8 + g, rows - 1)) * a.groups;
+      for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(block * kRows + r * 16 + h * 8 + g, rows - 1)) * a.groups;
     const uint8_t* scale_base = static_cast<const uint8_t*>(a.scale) + static_cast<int64_t>(chunk) * a.groups * (a.scale_dtype == kF32 ? 4 : 2);
     const uint8_t* zero_base = a.zero + static_cast<int64_t>(chunk) * a.groups;
     auto load_numbers = [&](int step) {
@@ -637,9 +571,10 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
           if (!is_signed) zero[r][h] = zero_base[at] & 15u;
         }
     };
-    __syncthreads();                                        // the sums of the chunk before, where x goes, have been read
+    fence_proxy_async_smem();                               // what this thread wrote where x goes: zeros, sums
+    __syncthreads();                                        // the sums of the chunk before have been read
     load_x(0);
-    for (int s = 0; s < S::kStages - 1; ++s) load();
+    for (int s = 0; s < kStages - 1; ++s) load();
     int step = share, stage = 0;
     if (works && step < steps) load_numbers(step);
     float acc[2][kCols][4] = {};
@@ -654,11 +589,11 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
       const int end = min(steps, (phase + 1) * phase_steps);
 #pragma unroll 1
       for (; works && step < end; step += shares) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
         load();
         const uint32_t weights = smem_u32(ring) + stage * 2048, inputs = x_at + (step - phase * phase_steps) * 256;
-        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
 #pragma unroll
         for (int group = 0; group < kPerStep; ++group) {
           const int holder = (lane & ~3) | group;
@@ -718,7 +653,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
     }
     __syncthreads();                                        // x has been read: its place takes the sums
     if (works) {
-      float* mine = sums + warp * a.m * S::kStride;
+      float* mine = sums + warp * a.m * kSumStride;
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
@@ -726,8 +661,8 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
           if (c * 8 + 2 * t + e < a.m) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + g] = acc[r][c][e];
-              mine[(c * 8 + 2 * t + e) * S::kStride + r * 16 + 8 + g] = acc[r][c][e + 2];
+              mine[(c * 8 + 2 * t + e) * kSumStride + r * 16 + g] = acc[r][c][e];
+              mine[(c * 8 + 2 * t + e) * kSumStride + r * 16 + 8 + g] = acc[r][c][e + 2];
             }
           }
     }
@@ -735,10 +670,10 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
 #pragma unroll 1
     for (int i = threadIdx.x; i < rows * a.m; i += kWarps * 32) {
       const int x_row = i / rows, in_chunk = i - x_row * rows, at = chunk + in_chunk;
-      const float* part = sums + (in_chunk / S::kRows * a.m + x_row) * S::kStride + in_chunk % S::kRows;
+      const float* part = sums + (in_chunk / kRows * a.m + x_row) * kSumStride + in_chunk % kRows;
       float y = 0.0f;
 #pragma unroll 1
-      for (int w = 0; w < shares; ++w) y += part[w * blocks * a.m * S::kStride];
+      for (int w = 0; w < shares; ++w) y += part[w * blocks * a.m * kSumStride];
       if (a.bias != nullptr) y += ValueOf<0>(LoadBits<0>(a.bias, at, a.bias_dtype), a.bias_dtype);
       const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
       if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
@@ -752,47 +687,36 @@ struct Variant {
   void (*kernel)(W4Args);
   int64_t (*bytes)(int64_t m, int64_t steps, int64_t group);
   int64_t (*per_round)(int64_t m, int64_t steps);
-  int most, rows, warps, registers;              // most: rows of x
+  int warps, registers;
 };
 constexpr int64_t kSmemPerSm = 228 * 1024, kSmemPerCta = 227 * 1024, kSmemReserved = 1024;
-template <int kGroup, int kScale, int kSign, typename S>
-Variant Make() {
-  return {w4_dot_kernel<kGroup, kScale, kSign, S>, S::Bytes, [](int64_t m, int64_t) -> int64_t { return S::kSums / (S::kWarps * S::kStride) / m; }, 8 * S::kCols, S::kRows, S::kWarps, 0};
-}
 template <int kGroup, typename S>
 Variant MakeWide() {
-  return {w4_dot_wide_kernel<kGroup, S>, S::Bytes, S::Phase, 8 * S::kCols, S::kRows, S::kWarps, 0};
+  return {w4_dot_wide_kernel<kGroup, S>, S::Bytes, S::Phase, S::kWarps, 0};
 }
-// In order of preference: the first that takes m rows of x and fits shared memory.  Without a resident x a CTA reads it once
-// per block of rows, m / (4 * tiles) bytes of it for a byte of weights.
-constexpr int kResidentShapes = 4, kRingShapes = 4;
 struct Variants {
-  Variant resident[3][3][2][kResidentShapes];    // group, type of the scales, sign
-  Variant ring[2][3][kRingShapes];               // type of x, group
-  template <int kGroup, int kScale, int kSign>
-  void Fill(Variant* to) {
-    to[0] = Make<kGroup, kScale, kSign, Shape<2, 1, 24, 3, void>>();
-    to[1] = Make<kGroup, kScale, kSign, Shape<2, 1, 16, 3, void>>();
-    to[2] = Make<kGroup, kScale, kSign, Shape<2, 1, 16, 2, void>>();
-    to[3] = Make<kGroup, kScale, kSign, Shape<2, 2, 16, 3, void>>();
+  Variant resident[3][3][2];                     // group, type of the scales, two's complement
+  Variant wide[2][3][3];                         // type of x, group, for 8, 16 and 32 rows of x
+  template <int kGroup, int kScale, bool kSigned>
+  void Fill(Variant& to) {
+    to = {w4_dot_kernel<kGroup, kScale, kSigned>, Resident::Bytes, Resident::PerRound, Resident::kWarps, 0};
+  }
+  template <int kGroup, typename T>
+  void FillWide(Variant* to) {
+    to[0] = MakeWide<kGroup, WideShape<T, 1>>();
+    to[1] = MakeWide<kGroup, WideShape<T, 2>>();
+    to[2] = MakeWide<kGroup, WideShape<T, 4>>();
   }
   template <int kGroup>
   void FillGroup(int at) {
-    Fill<kGroup, kF16, 0>(resident[at][0][0]);
-    Fill<kGroup, kF16, 1>(resident[at][0][1]);
-    Fill<kGroup, kBF16, 0>(resident[at][1][0]);
-    Fill<kGroup, kBF16, 1>(resident[at][1][1]);
-    Fill<kGroup, kF32, 0>(resident[at][2][0]);
-    Fill<kGroup, kF32, 1>(resident[at][2][1]);
-    FillRing<kGroup, __half>(ring[0][at]);
-    FillRing<kGroup, __nv_bfloat16>(ring[1][at]);
-  }
-  template <int kGroup, typename T>
-  void FillRing(Variant* to) {
-    to[0] = Make<kGroup, 0, 2, Shape<2, 1, 8, 4, T>>();
-    to[1] = MakeWide<kGroup, WideShape<T, 2>>();
-    to[2] = MakeWide<kGroup, WideShape<T, 4>>();
-    to[3] = Make<kGroup, 0, 2, Shape<2, 8, 4, 2, T>>();
+    Fill<kGroup, kF16, false>(resident[at][0][0]);
+    Fill<kGroup, kF16, true>(resident[at][0][1]);
+    Fill<kGroup, kBF16, false>(resident[at][1][0]);
+    Fill<kGroup, kBF16, true>(resident[at][1][1]);
+    Fill<kGroup, kF32, false>(resident[at][2][0]);
+    Fill<kGroup, kF32, true>(resident[at][2][1]);
+    FillWide<kGroup, __half>(wide[0][at]);
+    FillWide<kGroup, __nv_bfloat16>(wide[1][at]);
   }
   Variants() {
     FillGroup<32>(0);
@@ -847,17 +771,31 @@ Status ValidateDotW4(const B200SD_DotW4& a, bool check_pointers) {
 
 Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stats) {
   if (a.m == 0) return Status::Ok();
+  if (a.m > 32) {                                           // half of the rows at a time: the sums of 64 do not fit the registers
+    B200SD_DotW4 half = a;
+    LaunchStats first, second;
+    half.m = a.m / 2;
+    Status st = LaunchDotW4(half, stream, &first);
+    if (!st.ok()) return st;
+    half.x = static_cast<const uint16_t*>(a.x) + half.m * a.k;
+    half.d = static_cast<uint8_t*>(a.d) + half.m * a.n * (a.d_dtype == kF32 ? 4 : 2);
+    half.m = a.m - half.m;
+    st = LaunchDotW4(half, stream, &second);
+    stats->launches = first.launches + second.launches;
+    return st;
+  }
   const int64_t steps = (a.k + 127) / 128, step_group = std::min<int64_t>(a.group, 128);
   const int group_at = a.group == 32 ? 0 : a.group == 64 ? 1 : 2, scale_at = a.scale_dtype == kF16 ? 0 : a.scale_dtype == kBF16 ? 1 : 2;
-  const auto& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
-  const auto& ring = TheVariants().ring[a.x_dtype == kBF16][group_at];
-  // Every CTA converts all of x for a resident one.  Against four rows and more of it a CTA needs about six rows of weights
-  // for each, or the conversion costs more than the cheaper decoding saves (k 4096, resident against ring, in us: m 5, n
-  // 2400 12.6 against 10.4, n 10000 22.9 against 23.6; m 8, n 2400 16.7 against 12.3; m 3, n 2400 10.7 against 14.1).
-  int pick = a.m >= 4 && a.n < int64_t{6} * a.m * DeviceSmCount() ? kResidentShapes : 0;
-  auto shape = [&](int i) -> const Variant& { return i < kResidentShapes ? resident[i] : ring[i - kResidentShapes]; };
-  while (a.m > shape(pick).most || shape(pick).bytes(a.m, steps, step_group) > kSmemPerCta) ++pick;       // the last one always fits
-  const Variant& v = shape(pick);
+  const Variant& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
+  // With x resident every CTA converts all of it first, and decodes for less afterwards.  That pays for one and two rows of x
+  // where a CTA has many rows of weights, fewer of them where groups are short, and a line of k long enough for its warps.
+  // Resident against wide in us, two's complement: m 1, group 128, k 8192: n 8192 15.1 and 13.6, n 16384 22.3 and 23.0, n
+  // 28672 33.0 and 40.9; m 2, the same: n 16384 24.8 and 22.9, n 28672 37.5 and 41.0; m 2, n 28672, k 4096 23.8 and 22.1, n
+  // 131072, k 2048 46.7 and 40.6; m 3, n 28672, k 8192 43.0 and 41.4; group 32, k 8192: m 1, n 8192 16.8 and 20.0, m 2 18.0
+  // and 20.1, but n 2048 8.1 and 8.0; m 3, n 131072, k 4096 125 and 119.
+  const int64_t enough = DeviceSmCount() * (a.group == 32 ? 32 * a.m : 64 * (a.m + 1));
+  const bool is_resident = a.m <= Resident::kMost && a.n >= enough && a.k >= 4096 && resident.bytes(a.m, steps, step_group) <= kSmemPerCta;
+  const Variant& v = is_resident ? resident : TheVariants().wide[a.x_dtype == kBF16][group_at][a.m <= 8 ? 0 : a.m <= 16 ? 1 : 2];
   const int bytes = static_cast<int>(v.bytes(a.m, steps, step_group)), threads = v.warps * 32;
   const int by_registers = 65536 / (threads * ((v.registers + 7) / 8 * 8)), by_smem = static_cast<int>(kSmemPerSm / (bytes + kSmemReserved));
   const int per_sm = std::max(1, std::min({by_registers, by_smem, 2048 / threads}));
