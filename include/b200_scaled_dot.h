@@ -179,10 +179,11 @@ typedef struct B200SD_BlockScaledDotMx {
  *
  * The weights are K-minor like the MX call's: byte [n, j] holds w[n, 2j] in its low and w[n, 2j+1] in
  * its high four bits.  weight_type S4 is two's complement (-8 .. 7) and has no zero points; U4 (0 .. 15)
- * takes one zero point per group from the low four bits of a byte.  The weights enter the products as
- * the integers w - z, exactly; sums are f32, a group's sum is multiplied by its scale in f32, and D is
- * rounded once.  group is 32, 64 or a multiple of 128 that divides k; n is free; m is at most 64.
- * m == 0 does nothing. */
+ * takes one zero point per group from the low four bits of a byte.  The weights enter as the integers
+ * w - z, exactly; sums are f32, a group's sum is multiplied by its scale in f32, and D is rounded once.
+ * (One or two rows of x against many rows of weights are converted first: of a row, what lies more than
+ * 2^23 below its largest value is rounded to within 2^-34 of that.)  group is 32, 64 or a multiple of
+ * 128 that divides k; n is free; m is at most 64.  m == 0 does nothing. */
 typedef struct B200SD_DotW4 {
   size_t struct_size;            /* sizeof(B200SD_DotW4) */
   const void* x;                 /* [m, k] */
@@ -239,7 +240,7 @@ typedef struct B200SD_KvCacheAppend {
  * that see nothing (i >= new_lens[b] among them) get zeros, and -inf as their logarithm of the sum.
  * Scores, softmax sums and products are held in f32; a row's weights are rounded to 11 bits for the
  * product with the values.  new_tokens is at most 64, head_dim a multiple of 16 up to 256, page_tokens
- * 16, 32, 64 or 128, batch at most 4096. */
+ * 16, 32, 64 or 128, batch at most 4096.  Calls that may run at the same time need a workspace each. */
 typedef struct B200SD_PagedAttention {
   size_t struct_size;            /* sizeof(B200SD_PagedAttention) */
   const void* q;                 /* [batch, new_tokens, heads, head_dim] */
@@ -322,8 +323,8 @@ int b200sd_load_config_table(const char* path, int32_t* entries, char* err, size
 uint64_t b200sd_launch_count(void);
 
 /* Synchronises the device, then returns and clears the bit mask kernels set when one of their
- * bounded waits expired, or a page table led outside of its cache (0 = healthy).  The host-visible half of failure detection; stands where
- * the reference relies on its execution watchdog (xla/service/gpu/execution_watchdog.h:43-61). */
+ * bounded waits expired, or a page table led outside of its cache (0 = healthy).  The host-visible
+ * half of failure detection; stands where the reference relies on its execution watchdog (xla/service/gpu/execution_watchdog.h:43-61). */
 int b200sd_device_status(uint32_t* bits, char* err, size_t err_len);
 
 /* Launches a one-thread kernel that waits `limit_ns` on a barrier nobody signals and then reports

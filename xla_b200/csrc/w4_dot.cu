@@ -9,18 +9,21 @@
 // lane's word, half or whole 16-byte piece is chosen so that one product never mixes two groups; a group's f32 sum is
 // multiplied by its scale in f32 and added up.
 //
-// Where x fits shared memory beside the rings it is put there once, paired, as f16 whatever its type, each row multiplied
-// by the power of two that brings its largest value to 2^13 (what lies 2^23 below that is rounded, to 2^-34 of it).  A
-// nibble under a mask then is an f16 operand as it stands: the subnormal n * 2^-24, or 16 n * 2^-24 for the nibbles one
-// place higher, whose x is stored divided by 16.  That is 5 instructions for 8 weights; the zero point (8 for two's
-// complement) is taken off a group's sum as z times the sum of x over the group, which is formed once in f32.  The sum
-// before that is not much larger than after, so this costs at most a few bits of f32's 24.
-// Otherwise x comes through the rings with the weights and the products have x's type: a masked nibble plus an offset is
-// an f16 or bf16 number (1024 + n, 128 + n), and one subtraction leaves w - z, exactly; 9 and 11 instructions for 8.
-//
 // A CTA owns n / CTAs consecutive rows, whole rows of bytes with none read twice or by two CTAs whatever n is.  A block of
-// its rows and 128 of k are a unit; the warps take the units in turn, each through its own cp.async ring, and leave their
-// sums of each block in shared memory, where they are added in the order of the warps, as many blocks at a time as fit.
+// 32 of its rows and 128 of k are a unit, which a warp brings in through its own cp.async ring.
+//
+// The wide kernel takes x as it is, in phases that the warps of a CTA share.  A masked nibble plus an offset is an f16 or
+// bf16 number (1024 + n, 128 + n), and one subtraction leaves w - z, exactly; 9 and 11 instructions for 8 weights.
+// The other one, for one or two rows against many weights, first puts all of x into shared memory, paired, as f16 whatever
+// its type, each row multiplied by the power of two that brings its largest value to 2^13 (what lies 2^23 below that is
+// rounded, to 2^-34 of it).  A nibble under a mask then is an f16 operand as it stands: the subnormal n * 2^-24, or 16 n *
+// 2^-24 for the nibbles one place higher, whose x is stored divided by 16.  That is 5 instructions for 8 weights; the zero
+// point (8 for two's complement) is taken off a group's sum as z times the sum of x over the group, which is formed once
+// in f32.  The sum before that is not much larger than after, so this costs at most a few bits of f32's 24.
+//
+// Measured with cold caches: 28672 x 8192 in groups of 128 for one row 33 us (3.7 TB/s; the bytes alone take 18.5), 8192 x
+// 28672 with zero points for 16 rows 57.5 us, 5003 x 4416 in groups of 32 for 5 rows 11.7 us, 1024 x 2048 for one row 7.6 us, the
+// host's part of a call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -254,7 +257,10 @@ struct Resident {
   static int64_t Bytes(int64_t m, int64_t steps, int64_t group) { return kHead + kRing + steps * m * 256 + steps * (128 / group) * 2 * 4; }
 };
 
-// One or two rows of x, all of it in shared memory.  kGroup: 32, 64 or 128 (which stands for its multiples too).  kScale: the
+// One or two rows of x, all of it in shared memory.  The warps take the units of the CTA in turn and leave their sums of
+// each block in shared memory, where they are added in the order of the warps, as many blocks at a time as have room.  Bound
+// by issue, about 250 instructions of a warp for a unit of 2 KiB, and by 8 us in front and behind: x, the first units, the
+// sums.  24 warps instead of 16: 28672 x 8192 for one row 33 and 36 us.  kGroup: 32, 64 or 128 (which stands for its multiples too).  kScale: the
 // scales' type, kSigned: two's complement, no zero points.
 template <int kGroup, int kScale, bool kSigned>
 __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
@@ -469,10 +475,13 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
   }
 }
 
-// Up to 32 rows of x, as they are.  All warps of a CTA share a phase of x, some steps of k for all rows, as it
-// is stored (one bulk copy per row); the next one is on its way meanwhile.  A warp keeps its block of 32 weight rows from the first phase to the
-// last, alone or with others that take every so manieth step of it, and its sums in registers, so x is read once per CTA
-// (per 512 of its rows) where the rings above read it once per block of rows.
+// Up to 32 rows of x, as they are.  All warps of a CTA share a phase of x, some steps of k for all rows, as it is stored (one
+// bulk copy per row); the next one is on its way meanwhile.  A warp keeps its block of 32 weight rows from the first phase
+// to the last, alone or with others that take every so manieth step of it, and its sums in registers, so x is read once per
+// CTA (per 512 of its rows).  Bound by issue and the matrix pipe: 463 instructions of a warp for a unit and 16 rows.
+// (x through each warp's ring beside the weights, once for every block of 32 rows, took 292 us instead of 149 for 33 rows
+// against 8192 x 28672, 15.0 instead of 11.7 for 5 rows against 5003 x 4416.)  16 warps leave 128 registers to a thread; 20 and
+// 24 were slower, by 3 % and 7 % at 8 rows and, short of registers, by half and more at 16.
 template <typename T_, int kCols_>
 struct WideShape {
   using T = T_;
