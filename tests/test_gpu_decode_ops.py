@@ -93,6 +93,15 @@ def test_dot_w4_large(cuda_device, m, n, k, group, dtype, zeros, bias):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("rows", [1, 15, 16, 17, 32, 33, 48, 49, 100, 177, 250, 481, 511, 512])
+def test_dot_w4_rows_of_a_cta(cuda_device, rows):
+    """Every split of a CTA's warps: this many rows of weights each, and one more for some of them."""
+    for m, group, dtype, zeros in ((5, 64, F16, True), (20, 128, BF16, False)):
+        inputs = _dot_inputs(cuda_device, m, 148 * rows + 3, 1280, group, dtype, zeros, True)
+        _check_dot(xla_b200.dot_w4(*inputs[:3], zero=inputs[3], bias=inputs[4]), inputs, 1280)
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("scale_dtype", [F32, F16, BF16])
 def test_dot_w4_scale_types_of_many_rows(cuda_device, scale_dtype, group):

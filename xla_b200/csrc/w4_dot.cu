@@ -148,6 +148,8 @@ __device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 
 // Either kernel's unit is 32 weight rows, in two tiles of the products, by 128 of k.
 constexpr int kTiles = 2, kRows = 16 * kTiles, kStageBytes = kTiles * 1024;
+using One = std::integral_constant<int, 1>;      // tiles of a unit that have rows of weights
+using Two = std::integral_constant<int, 2>;
 constexpr int kSumStride = kRows + 4;           // floats between two rows of x in the sums
 constexpr int kStages = 3;                      // of a warp's ring
 
@@ -324,11 +326,11 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
   // each.  Rows behind the last take its numbers, groups behind the end of k a scale of 0.  They are loaded a unit ahead,
   // into the registers that the unit before has just used; in front of a block, its first unit's.
   uint32_t scale[kTiles][2], zero[kTiles][2], row_at[kTiles][2];
-  auto load_numbers = [&](int step) {
+  auto load_numbers = [&](int step, auto tiles_of_unit) {
     const uint32_t group = kGroup == 128 ? (a.group_shift >= 0 ? step >> a.group_shift : step / a.blocks_per_group) : step * kPerStep + t % kPerStep;
     const bool there = kGroup == 128 || group < a.groups;
 #pragma unroll
-    for (int r = 0; r < kTiles; ++r)
+    for (int r = 0; r < decltype(tiles_of_unit)::value; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t at = row_at[r][h] + (there ? group : 0);
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
 #pragma unroll 1
   for (int s = 0; s < kStages - 1; ++s) load(s * kStageBytes);
   set_rows(0);
-  load_numbers(min(warp, steps - 1));
+  load_numbers(min(warp, steps - 1), Two());
   asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");         // this thread's part of x has come
   staging.Convert(factors, top, group_sums);
 
@@ -371,74 +373,80 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
   }
   const uint32_t sums_at = Kept(smem_u32(group_sums));
 
+  const bool half = (last - first - 1) % kRows < 16;        // of the last block only one tile has rows
   uint32_t stage = 0, load_stage = (kStages - 1) * kStageBytes;
   for (int round = 0; round < blocks; round += per_round) {
     const int round_end = min(round + per_round, blocks);
     int step = warp;
     for (int block = round; block < round_end; ++block) {
       float acc[kTiles][4] = {};
-      for (; step < steps; step += kWarps) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncwarp();
-        load(load_stage);
-        load_stage = stage;
-        const uint32_t inputs = step * (a.m * 256), sums_step = step * (kPerStep * columns * 4);
+      auto run = [&](auto tiles_of_unit) {
+        constexpr int kOfUnit = decltype(tiles_of_unit)::value;
+        for (; step < steps; step += kWarps) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+          __syncwarp();
+          load(load_stage);
+          load_stage = stage;
+          const uint32_t inputs = step * (a.m * 256), sums_step = step * (kPerStep * columns * 4);
 #pragma unroll
-        for (int group = 0; group < kPerStep; ++group) {
-          const int holder = (lane & ~3) | group;           // the lane with this group's numbers
-          float part[kTiles][4] = {};
-          // The words of this group, of rows g and g + 8 of each tile.
-          uint32_t w[kTiles][2][kWords];
+          for (int group = 0; group < kPerStep; ++group) {
+            const int holder = (lane & ~3) | group;           // the lane with this group's numbers
+            float part[kTiles][4] = {};
+            // The words of this group, of rows g and g + 8 of each tile.
+            uint32_t w[kTiles][2][kWords];
 #pragma unroll
-          for (int r = 0; r < kTiles; ++r)
+            for (int r = 0; r < kOfUnit; ++r)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t at = weight_at[group] + stage + (r * 16 + h * 8) * 64;
-              if constexpr (kGroup == 128) {
-                const uint4 v = LoadShared16(at);
-                w[r][h][0] = v.x, w[r][h][1] = v.y, w[r][h][2] = v.z, w[r][h][3] = v.w;
-              } else if constexpr (kGroup == 64) {
-                const uint2 v = LoadShared8(at);
-                w[r][h][0] = v.x, w[r][h][1] = v.y;
-              } else {
-                w[r][h][0] = LoadShared4(at);
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t at = weight_at[group] + stage + (r * 16 + h * 8) * 64;
+                if constexpr (kGroup == 128) {
+                  const uint4 v = LoadShared16(at);
+                  w[r][h][0] = v.x, w[r][h][1] = v.y, w[r][h][2] = v.z, w[r][h][3] = v.w;
+                } else if constexpr (kGroup == 64) {
+                  const uint2 v = LoadShared8(at);
+                  w[r][h][0] = v.x, w[r][h][1] = v.y;
+                } else {
+                  w[r][h][0] = LoadShared4(at);
+                }
+              }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              const uint4 b = LoadShared16(input_at[group * kWords + i] + inputs);
+#pragma unroll
+              for (int r = 0; r < kOfUnit; ++r) {
+                uint32_t low[4], high[4];
+                DecodeSubnormal(w[r][0][i], flip, low);
+                DecodeSubnormal(w[r][1][i], flip, high);
+                Mma<__half>(part[r], low[0], high[0], low[1], high[1], b.x, b.y);
+                Mma<__half>(part[r], low[2], high[2], low[3], high[3], b.z, b.w);
               }
             }
+            // The zero points' share, then the scales.
+            const uint2 sum_bits = LoadShared8(sums_at + sums_step + group * (columns * 4));
+            const float sum0 = __uint_as_float(sum_bits.x), sum1 = __uint_as_float(sum_bits.y);
 #pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            const uint4 b = LoadShared16(input_at[group * kWords + i] + inputs);
-#pragma unroll
-            for (int r = 0; r < kTiles; ++r) {
-              uint32_t low[4], high[4];
-              DecodeSubnormal(w[r][0][i], flip, low);
-              DecodeSubnormal(w[r][1][i], flip, high);
-              Mma<__half>(part[r], low[0], high[0], low[1], high[1], b.x, b.y);
-              Mma<__half>(part[r], low[2], high[2], low[3], high[3], b.z, b.w);
+            for (int r = 0; r < kOfUnit; ++r) {
+              float s0 = ValueOf<kScale>(scale[r][0], kScale), s1 = ValueOf<kScale>(scale[r][1], kScale);
+              float z0 = -0x1p-21f, z1 = -0x1p-21f;            // -8 * 2^-24
+              if (!kSigned) z0 = -0x1p-24f * static_cast<float>(zero[r][0]), z1 = -0x1p-24f * static_cast<float>(zero[r][1]);
+              if (kGroup < 128) {
+                s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
+                if (!kSigned) z0 = __shfl_sync(0xffffffffu, z0, holder), z1 = __shfl_sync(0xffffffffu, z1, holder);
+              }
+              acc[r][0] = fmaf(fmaf(z0, sum0, part[r][0]), s0, acc[r][0]), acc[r][1] = fmaf(fmaf(z0, sum1, part[r][1]), s0, acc[r][1]);
+              acc[r][2] = fmaf(fmaf(z1, sum0, part[r][2]), s1, acc[r][2]), acc[r][3] = fmaf(fmaf(z1, sum1, part[r][3]), s1, acc[r][3]);
             }
           }
-          // The zero points' share, then the scales.
-          const uint2 sum_bits = LoadShared8(sums_at + sums_step + group * (columns * 4));
-          const float sum0 = __uint_as_float(sum_bits.x), sum1 = __uint_as_float(sum_bits.y);
-#pragma unroll
-          for (int r = 0; r < kTiles; ++r) {
-            float s0 = ValueOf<kScale>(scale[r][0], kScale), s1 = ValueOf<kScale>(scale[r][1], kScale);
-            float z0 = -0x1p-21f, z1 = -0x1p-21f;            // -8 * 2^-24
-            if (!kSigned) z0 = -0x1p-24f * static_cast<float>(zero[r][0]), z1 = -0x1p-24f * static_cast<float>(zero[r][1]);
-            if (kGroup < 128) {
-              s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
-              if (!kSigned) z0 = __shfl_sync(0xffffffffu, z0, holder), z1 = __shfl_sync(0xffffffffu, z1, holder);
-            }
-            acc[r][0] = fmaf(fmaf(z0, sum0, part[r][0]), s0, acc[r][0]), acc[r][1] = fmaf(fmaf(z0, sum1, part[r][1]), s0, acc[r][1]);
-            acc[r][2] = fmaf(fmaf(z1, sum0, part[r][2]), s1, acc[r][2]), acc[r][3] = fmaf(fmaf(z1, sum1, part[r][3]), s1, acc[r][3]);
-          }
+          stage = stage == (kStages - 1) * kStageBytes ? 0 : stage + kStageBytes;
+          if (step + kWarps < steps) load_numbers(step + kWarps, tiles_of_unit);
         }
-        stage = stage == (kStages - 1) * kStageBytes ? 0 : stage + kStageBytes;
-        if (step + kWarps < steps) load_numbers(step + kWarps);
-      }
+      };
+      if (half && block == blocks - 1) run(One());
+      else run(Two());
       step -= steps;
       if (block + 1 == round_end) step = warp;
       set_rows(block + 1);
-      if (step < steps) load_numbers(step);
+      if (step < steps) load_numbers(step, Two());
       // This warp's sums of the block, zeros where it had no unit of it.
       float* mine = sums + ((block - round) * kWarps + warp) * a.m * kSumStride;
 #pragma unroll
@@ -539,9 +547,13 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
   for (int c = 0; c < kCols; ++c) row_offset[c] = min(c * 8 + g, a.m - 1) * x_pitch;
 
   for (int chunk = first; chunk < last; chunk += kWarps * kRows) {
-    const int rows = min(last - chunk, kWarps * kRows), blocks = (rows + kRows - 1) / kRows, shares = kWarps / blocks;
-    const int block = warp % blocks, share = warp / blocks;  // warps with share >= shares only help with x
-    const int row = chunk + block * kRows;
+    // Blocks of two tiles, and one of one where the last 16 rows or fewer are left: it costs half, and gets the warps that
+    // the others leave.  A warp without a share only helps with x.
+    const int rows = min(last - chunk, kWarps * kRows), tiles = (rows + 15) / 16, whole = tiles / 2;
+    const int whole_shares = 2 * kWarps / tiles, half_shares = tiles % 2 ? max(1, min(whole_shares, kWarps - whole * whole_shares)) : 0;
+    const bool half = warp >= whole * whole_shares;
+    const int shares = half ? half_shares : whole_shares, block = half ? whole : warp % whole;
+    const int share = half ? warp - whole * whole_shares : warp / whole, row = chunk + block * kRows;
     const bool works = share < shares;
 
     const uint8_t* w_base = a.w + static_cast<int64_t>(row + g) * row_bytes + t * 16;
@@ -566,11 +578,11 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
       for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(block * kRows + r * 16 + h * 8 + g, rows - 1)) * a.groups;
     const uint8_t* scale_base = static_cast<const uint8_t*>(a.scale) + static_cast<int64_t>(chunk) * a.groups * (a.scale_dtype == kF32 ? 4 : 2);
     const uint8_t* zero_base = a.zero + static_cast<int64_t>(chunk) * a.groups;
-    auto load_numbers = [&](int step) {
+    auto load_numbers = [&](int step, auto tiles_of_unit) {
       const uint32_t group = kGroup == 128 ? (a.group_shift >= 0 ? step >> a.group_shift : step / a.blocks_per_group) : step * kPerStep + t % kPerStep;
       const bool there = kGroup == 128 || group < a.groups;
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < decltype(tiles_of_unit)::value; ++r)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t at = row_at[r][h] + (there ? group : 0);
@@ -585,7 +597,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
     load_x(0);
     for (int s = 0; s < kStages - 1; ++s) load();
     int step = share, stage = 0;
-    if (works && step < steps) load_numbers(step);
+    if (works && step < steps) load_numbers(step, Two());
     float acc[2][kCols][4] = {};
 
 #pragma unroll 1
@@ -596,69 +608,74 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
       x_parity ^= 1u << (phase & 1);
       const uint32_t x_at = smem_u32(x_buffer) + (phase & 1) * (a.m * x_pitch) + t * (kGroup == 128 ? 64 : kGroup == 64 ? 32 : 16);
       const int end = min(steps, (phase + 1) * phase_steps);
+      auto run = [&](auto tiles_of_unit) {
+        constexpr int kOfUnit = decltype(tiles_of_unit)::value;
 #pragma unroll 1
-      for (; works && step < end; step += shares) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncwarp();
-        load();
-        const uint32_t weights = smem_u32(ring) + stage * 2048, inputs = x_at + (step - phase * phase_steps) * 256;
-        stage = stage + 1 == kStages ? 0 : stage + 1;
+        for (; step < end; step += shares) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+          __syncwarp();
+          load();
+          const uint32_t weights = smem_u32(ring) + stage * 2048, inputs = x_at + (step - phase * phase_steps) * 256;
+          stage = stage + 1 == kStages ? 0 : stage + 1;
 #pragma unroll
-        for (int group = 0; group < kPerStep; ++group) {
-          const int holder = (lane & ~3) | group;
-          Offset<T> decoder[2][2];
+          for (int group = 0; group < kPerStep; ++group) {
+            const int holder = (lane & ~3) | group;
+            Offset<T> decoder[2][2];
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < kOfUnit; ++r)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) decoder[r][h].Set(kGroup == 128 || is_signed ? zero[r][h] : __shfl_sync(0xffffffffu, zero[r][h], holder));
-          float part[2][kCols][4] = {};
-          uint32_t w[2][2][kWords];
+              for (int h = 0; h < 2; ++h) decoder[r][h].Set(kGroup == 128 || is_signed ? zero[r][h] : __shfl_sync(0xffffffffu, zero[r][h], holder));
+            float part[2][kCols][4] = {};
+            uint32_t w[2][2][kWords];
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < kOfUnit; ++r)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int at = r * 16 + h * 8 + g;
-              if constexpr (kGroup == 128) {
-                const uint4 v = LoadShared16(weights + WeightPiece(at, t));
-                w[r][h][0] = v.x, w[r][h][1] = v.y, w[r][h][2] = v.z, w[r][h][3] = v.w;
-              } else if constexpr (kGroup == 64) {
-                const uint2 v = LoadShared8(weights + WeightPiece(at, group * 2 + t / 2) + t % 2 * 8);
-                w[r][h][0] = v.x, w[r][h][1] = v.y;
-              } else {
-                w[r][h][0] = LoadShared4(weights + WeightPiece(at, group) + t * 4);
+              for (int h = 0; h < 2; ++h) {
+                const int at = r * 16 + h * 8 + g;
+                if constexpr (kGroup == 128) {
+                  const uint4 v = LoadShared16(weights + WeightPiece(at, t));
+                  w[r][h][0] = v.x, w[r][h][1] = v.y, w[r][h][2] = v.z, w[r][h][3] = v.w;
+                } else if constexpr (kGroup == 64) {
+                  const uint2 v = LoadShared8(weights + WeightPiece(at, group * 2 + t / 2) + t % 2 * 8);
+                  w[r][h][0] = v.x, w[r][h][1] = v.y;
+                } else {
+                  w[r][h][0] = LoadShared4(weights + WeightPiece(at, group) + t * 4);
+                }
+              }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              uint32_t low[2][4], high[2][4];
+#pragma unroll
+              for (int r = 0; r < kOfUnit; ++r) {
+                decoder[r][0].Decode8(w[r][0][i], flip, low[r]);
+                decoder[r][1].Decode8(w[r][1][i], flip, high[r]);
+              }
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) {
+                const uint4 b = Paired(LoadShared16(inputs + row_offset[c] + (group * (kGroup / 8) + i) * 16));
+#pragma unroll
+                for (int r = 0; r < kOfUnit; ++r) {
+                  Mma<T>(part[r][c], low[r][0], high[r][0], low[r][1], high[r][1], b.x, b.y);
+                  Mma<T>(part[r][c], low[r][2], high[r][2], low[r][3], high[r][3], b.z, b.w);
+                }
               }
             }
 #pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            uint32_t low[2][4], high[2][4];
+            for (int r = 0; r < kOfUnit; ++r) {
+              float s0 = ValueOf<0>(scale[r][0], a.scale_dtype), s1 = ValueOf<0>(scale[r][1], a.scale_dtype);
+              if (kGroup < 128) s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              decoder[r][0].Decode8(w[r][0][i], flip, low[r]);
-              decoder[r][1].Decode8(w[r][1][i], flip, high[r]);
-            }
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              const uint4 b = Paired(LoadShared16(inputs + row_offset[c] + (group * (kGroup / 8) + i) * 16));
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                Mma<T>(part[r][c], low[r][0], high[r][0], low[r][1], high[r][1], b.x, b.y);
-                Mma<T>(part[r][c], low[r][2], high[r][2], low[r][3], high[r][3], b.z, b.w);
+              for (int c = 0; c < kCols; ++c) {
+                acc[r][c][0] = fmaf(part[r][c][0], s0, acc[r][c][0]), acc[r][c][1] = fmaf(part[r][c][1], s0, acc[r][c][1]);
+                acc[r][c][2] = fmaf(part[r][c][2], s1, acc[r][c][2]), acc[r][c][3] = fmaf(part[r][c][3], s1, acc[r][c][3]);
               }
             }
           }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float s0 = ValueOf<0>(scale[r][0], a.scale_dtype), s1 = ValueOf<0>(scale[r][1], a.scale_dtype);
-            if (kGroup < 128) s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              acc[r][c][0] = fmaf(part[r][c][0], s0, acc[r][c][0]), acc[r][c][1] = fmaf(part[r][c][1], s0, acc[r][c][1]);
-              acc[r][c][2] = fmaf(part[r][c][2], s1, acc[r][c][2]), acc[r][c][3] = fmaf(part[r][c][3], s1, acc[r][c][3]);
-            }
-          }
+          if (step + shares < steps) load_numbers(step + shares, tiles_of_unit);
         }
-        if (step + shares < steps) load_numbers(step + shares);
-      }
+      };
+      if (works && half) run(One());
+      else if (works) run(Two());
     }
     __syncthreads();                                        // x has been read: its place takes the sums
     if (works) {
@@ -679,10 +696,13 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
 #pragma unroll 1
     for (int i = threadIdx.x; i < rows * a.m; i += kWarps * 32) {
       const int x_row = i / rows, in_chunk = i - x_row * rows, at = chunk + in_chunk;
-      const float* part = sums + (in_chunk / kRows * a.m + x_row) * kSumStride + in_chunk % kRows;
+      const int of_block = in_chunk / kRows;
+      const bool in_whole = of_block < whole;
+      const float* part = sums + ((in_whole ? of_block : whole * whole_shares) * a.m + x_row) * kSumStride + in_chunk % kRows;
+      const int parts = in_whole ? whole_shares : half_shares, apart = (in_whole ? whole : 1) * a.m * kSumStride;
       float y = 0.0f;
 #pragma unroll 1
-      for (int w = 0; w < shares; ++w) y += part[w * blocks * a.m * kSumStride];
+      for (int w = 0; w < parts; ++w) y += part[w * apart];
       if (a.bias != nullptr) y += ValueOf<0>(LoadBits<0>(a.bias, at, a.bias_dtype), a.bias_dtype);
       const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
       if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
