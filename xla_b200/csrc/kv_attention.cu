@@ -62,7 +62,8 @@ struct AttentionArgs {
   const int32_t* new_lens;
   void* out;
   float* lse;
-  float* work;
+  float* work;                                  // the pieces of cut items, two places for each CTA ...
+  int4* cut;                                    // ... and for each CTA the item that the end of its share cuts first: b, item, pieces (0: none), new tokens
   int32_t batch, new_tokens, heads, kv_heads, head_dim, page_shift;
   int32_t rows, blocks;                         // rows of a (sequence, key head), and blocks of them
   int32_t num_pages, table_width, window;       // window: 0 none
@@ -109,9 +110,9 @@ struct Deal {
   }
 };
 
-// The share of CTA `cta`, with b, item and offset of its first or of its last unit.  Every warp finds out for itself, its
+// The share of CTA `cta`, with b, item and offset of its first unit.  Every warp finds out for itself, its
 // lanes taking consecutive sequences.  The launch chooses units large enough that the line has less than 2^31.
-__device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit, Deal* deal) {
+__device__ Share Locate(const AttentionArgs& a, int cta, Deal* deal) {
   const int lane = threadIdx.x % 32;
   const int each = (a.batch + 31) / 32, first = min(lane * each, a.batch), end = min(first + each, a.batch);
   const int32_t items = a.kv_heads * a.blocks;
@@ -153,10 +154,9 @@ __device__ Share Locate(const AttentionArgs& a, int cta, bool last_unit, Deal* d
     if (into <= a.extra) u1 -= into;
   }
   if (u0 >= u1) return {0, 0, 0, 0, 0};
-  Share share = last_unit ? place(u1 - 1) : at_begin;
-  share.begin = u0;
-  share.left = u1 - u0;
-  return share;
+  at_begin.begin = u0;
+  at_begin.left = u1 - u0;
+  return at_begin;
 }
 
 // Steps through the pieces of items that make up a share.
@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;       // the swizzle goes by the address
   __shared__ int abort_flag;
+  __shared__ Deal shared_deal;                             // for the end of the share
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   uint8_t* ring = smem + warp * kStages * kStageBytes;
   float4* exchange = reinterpret_cast<float4*>(smem + L::kRing);
@@ -312,10 +313,13 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
   }
   __syncthreads();
   griddep_wait();
-  // From here on the second kernel may start: it reads the lengths, which are final now, before it waits for this one.
   if (threadIdx.x == 0) griddep_launch_dependents();
   Deal deal;
-  const Share share = Locate(a, blockIdx.x, false, &deal);
+  const Share share = Locate(a, blockIdx.x, &deal);
+  if (threadIdx.x == 0) {
+    shared_deal = deal;
+    a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
   if (share.left == 0) return;
 
   // This lane's part of an item's queries, as they are.  The first item's are sent for before the tiles, which they would
@@ -728,6 +732,10 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     }
     if (warp == 0) {
       const bool complete = walk.offset == 0 && walk.Units() == span.units;
+      if (lane == 0 && walk.offset == 0 && !complete) {
+        const int32_t first = share.begin + (share.left - walk.left);    // the item's first unit
+        a.cut[blockIdx.x] = make_int4(walk.b, walk.item, shared_deal.CtaOf(first + span.units - 1) - static_cast<int32_t>(blockIdx.x) + 1, span.count);
+      }
       float* slot = a.work + (static_cast<int64_t>(blockIdx.x) * 2 + (walk.offset == 0 ? 1 : 0)) * L::kSlot;
       constexpr int kRun = kDim == 64 ? 8 : 16;              // columns in a row that a lane holds
 #pragma unroll
@@ -769,15 +777,11 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   __shared__ float4 part_values[kParts][L::kRows][kDim / 4];
   __shared__ float part_sum[kParts][L::kRows];
   const int c = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = warp % L::kRows, part = warp / L::kRows;
-  Deal deal;
-  const Share at = Locate(a, c, true, &deal);
   griddep_wait();
   if (threadIdx.x == 0) griddep_launch_dependents();
-  if (at.left == 0) return;
-  const Span span = SpanOf(a, at.b);
-  const int32_t first = at.begin + at.left - 1 - at.offset;              // the item's first unit
-  if (at.offset + 1 == span.units || first < at.begin) return;
-  const int pieces = deal.CtaOf(first + span.units - 1) - c + 1;
+  const int4 cut = a.cut[c];
+  const int pieces = cut.z;
+  if (pieces == 0) return;
   auto slot_of = [&](int p) { return a.work + (static_cast<int64_t>(c + p) * 2 + (p == 0 ? 1 : 0)) * L::kSlot; };
   // A few pieces are sent for at once; their maximum is known when they come.
   constexpr int kAtOnce = 4;
@@ -829,7 +833,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
       if (mine) part_values[part][row][i * 32 + lane] = y[i];
   }
   __syncthreads();
-  const int item_row = (at.item % a.blocks) * L::kRows + row;
+  const int item_row = (cut.y % a.blocks) * L::kRows + row;
   if (part > 0 || item_row >= a.rows) return;
   for (int p = 1; p < kParts; ++p) {
     total += part_sum[p][row];
@@ -844,7 +848,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   for (int i = 0; i < kVectors; ++i)
     if (mine) {
       const float run[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
-      StoreRow(a, at.b, at.item / a.blocks, item_row, span.count, i * 128 + lane * 4, run, m, total);
+      StoreRow(a, cut.x, cut.y / a.blocks, item_row, cut.w, i * 128 + lane * 4, run, m, total);
     }
 }
 
@@ -912,7 +916,7 @@ Status ValidatePagedAttention(const B200SD_PagedAttention& a, bool check_pointer
 size_t PagedAttentionWorkspaceBytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
   if (batch < 1 || new_tokens < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || head_dim < 16 || head_dim > 256) return 0;
   const Variant& v = kVariants[0][ShapeIndex(head_dim, new_tokens * (heads / kv_heads))];
-  return static_cast<size_t>(kMaxCtas) * 2 * v.slot * sizeof(float);
+  return kMaxCtas * (2 * v.slot * sizeof(float) + sizeof(int4));
 }
 
 Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream, LaunchStats* stats) {
@@ -934,6 +938,7 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   const int extra = cut ? std::max(1, static_cast<int>((192 << 10) / (g_ctas_per_sm[code][shape] * v.step * v.dim * 2))) : 0;
   AttentionArgs args{a.q, static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages), a.k_scale, a.v_scale,
                      a.page_table, a.seq_lens, a.new_lens, a.out, a.lse, static_cast<float*>(a.workspace),
+                     reinterpret_cast<int4*>(static_cast<float*>(a.workspace) + int64_t{kMaxCtas} * 2 * v.slot),
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
                      static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
