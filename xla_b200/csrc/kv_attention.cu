@@ -767,12 +767,16 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
 
 // Joins the pieces of the item that the end of CTA blockIdx.x's share cuts first: maximum over the pieces, then the
 // pieces' sums and values times exp2(their maximum - it), in the order of the pieces.
-constexpr int kJoinThreads = 512;
+
+// Small blocks of 8 rows come in as soon as one block of the first kernel has left, and send for more pieces at once (32
+// sequences of 0 to 4096 tokens: 33.7 us; with 512 threads and 4 pieces 34.1, with 256 and 4 34.4).
+template <int kRowTiles>
+constexpr int kJoinThreads = kRowTiles == 1 ? 256 : 512;
 
 template <int kDim, int kRowTiles>
-__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(kJoinThreads<kRowTiles>) kv_attention_join_kernel(const AttentionArgs a) {
   using L = Layout<kDim, kRowTiles>;
-  constexpr int kParts = kJoinThreads / 32 / L::kRows;      // warps of a row
+  constexpr int kParts = kJoinThreads<kRowTiles> / 32 / L::kRows;      // warps of a row
   constexpr int kVectors = kDim == 256 ? 2 : 1;             // of four columns, per lane
   __shared__ float4 part_values[kParts][L::kRows][kDim / 4];
   __shared__ float part_sum[kParts][L::kRows];
@@ -784,7 +788,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const A
   if (pieces == 0) return;
   auto slot_of = [&](int p) { return a.work + (static_cast<int64_t>(c + p) * 2 + (p == 0 ? 1 : 0)) * L::kSlot; };
   // A few pieces are sent for at once; their maximum is known when they come.
-  constexpr int kAtOnce = 4;
+  constexpr int kAtOnce = kRowTiles == 1 ? 8 : 4;
   const bool mine = lane * 4 < kDim;
   float first_max[kAtOnce], first_sum[kAtOnce];
   float4 first_values[kAtOnce][kVectors];
@@ -969,7 +973,7 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   cudaError_t e = cudaLaunchKernelEx(&cfg, v.main, args, key_map, value_map);
   stats->launches = 1;
   if (e == cudaSuccess && cut) {
-    cfg.blockDim = dim3(kJoinThreads);
+    cfg.blockDim = dim3(v.row_tiles == 1 ? kJoinThreads<1> : kJoinThreads<2>);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, v.join, args);
     stats->launches = 2;
