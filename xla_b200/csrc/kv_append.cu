@@ -8,9 +8,9 @@
 // is exact down to the subnormals; a scale of amax / max would round every earlier code of the page again each time a
 // token raises it.
 //
-// 4096 tokens for each of 8 sequences, 8 heads of 128, bf16 to e4m3, take 29 us (123 MB, 4.2 TB/s; the bytes alone 18.8), bound
-// by issue.  With a warp for a whole page of 64 slots, which looks at its values in one pass and reads them again to round them, it was
-// 52 us.  One token for each sequence of a batch takes 7.6 us, the host's part of the call.
+// 4096 tokens for each of 8 sequences, 8 heads of 128, bf16 to e4m3, take 30 us (123 MB, 4.1 TB/s; the bytes alone 18.8), bound
+// by issue.  With a warp for a whole page of 64 slots, which looks at its values in one pass and reads them again to round
+// them, it was 52 us.  One token for each sequence of a batch takes 7.7 us, the host's part of the call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -23,9 +23,10 @@
 //     two tokens with prmt and decodes the pairs; the weights turn from score layout to operand layout with movmatrix.
 // Token m of the 16 is row m ^ ((m & 1) << 2) of the tile in both products.
 //
-// Measured with cold caches: two sequences of 100003 to 131072 tokens, 8 key heads of 128, 88 us (5.3 TB/s of codes); 32 of 0
-// to 4096 tokens 37 us (3.6 TB/s: about 10 us pass before the tiles flow and 3 to 4 in joining the pieces); one of 37 tokens
-// 7.8 us, the host's part of the call.
+// Measured with cold caches: two sequences of 100003 to 131072 tokens, 8 key heads of 128, 86 us (5.5 TB/s of codes); 32 of 0
+// to 4096 tokens 34 us (4.0 TB/s: 9 us pass before the tiles flow and 3 to 4 in joining the pieces); 16 of 5 to 8191 with 5
+// new tokens, 40 rows for each of 4 key heads, 59 us (bound by issue: the codes are decoded for each 16 rows); one of 37
+// tokens 7.8 us, the host's part of the call.
 //
 // Softmax.  A page has one scale for its values, so the weight of a token that enters the product is
 // exp2(score + log2(value scale) - M) with one running M per row: the largest weight stays the same even if the scales of
@@ -938,7 +939,7 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   int64_t unit = cut ? v.step : 1 << 30;
   while (a.batch * a.kv_heads * blocks * ((capacity + unit - 1) / unit + 16) >= INT32_MAX) unit *= 2;       // the line's positions are 32-bit numbers
   // An item costs a CTA about 4 us besides its tokens, as much as it needs for 192 KiB of them shared by the CTAs of an SM.
-  // (Sequences of 0 to 4096 tokens, in us without and with: 41 and 37; 40 rows per key head: 107 and 60.)
+  // (When it was added, sequences of 0 to 4096 tokens, in us without and with: 41 and 37; 40 rows per key head: 107 and 60.)
   const int extra = cut ? std::max(1, static_cast<int>((192 << 10) / (g_ctas_per_sm[code][shape] * v.step * v.dim * 2))) : 0;
   AttentionArgs args{a.q, static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages), a.k_scale, a.v_scale,
                      a.page_table, a.seq_lens, a.new_lens, a.out, a.lse, static_cast<float*>(a.workspace),

@@ -21,9 +21,9 @@
 // point (8 for two's complement) is taken off a group's sum as z times the sum of x over the group, which is formed once
 // in f32.  The sum before that is not much larger than after, so this costs at most a few bits of f32's 24.
 //
-// Measured with cold caches: 28672 x 8192 in groups of 128 for one row 33 us (3.7 TB/s; the bytes alone take 18.5), 8192 x
-// 28672 with zero points for 16 rows 57.5 us, 5003 x 4416 in groups of 32 for 5 rows 11.7 us, 1024 x 2048 for one row 7.6 us, the
-// host's part of a call.
+// Measured with cold caches: 28672 x 8192 in groups of 128 for one row 32 us (3.8 TB/s; the bytes alone take 18.5), 8192 x
+// 28672 with zero points for 16 rows 58.6 us, 5003 x 4416 in groups of 32 for 5 rows 10.7 us, 1024 x 2048 for one row 7.6
+// us, the host's part of a call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -262,8 +262,8 @@ struct Resident {
 // One or two rows of x, all of it in shared memory.  The warps take the units of the CTA in turn and leave their sums of
 // each block in shared memory, where they are added in the order of the warps, as many blocks at a time as have room.  Bound
 // by issue, about 250 instructions of a warp for a unit of 2 KiB, and by 8 us in front and behind: x, the first units, the
-// sums.  24 warps instead of 16: 28672 x 8192 for one row 33 and 36 us.  kGroup: 32, 64 or 128 (which stands for its multiples too).  kScale: the
-// scales' type, kSigned: two's complement, no zero points.
+// sums.  24 warps instead of 16: 28672 x 8192 for one row 33.4 and 36.4 us, before half blocks.  kGroup: 32, 64 or 128
+// (which stands for its multiples too).  kScale: the scales' type, kSigned: two's complement, no zero points.
 template <int kGroup, int kScale, bool kSigned>
 __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
   using S = Resident;
@@ -488,8 +488,8 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
 // to the last, alone or with others that take every so manieth step of it, and its sums in registers, so x is read once per
 // CTA (per 512 of its rows).  Bound by issue and the matrix pipe: 463 instructions of a warp for a unit and 16 rows.
 // (x through each warp's ring beside the weights, once for every block of 32 rows, took 292 us instead of 149 for 33 rows
-// against 8192 x 28672, 15.0 instead of 11.7 for 5 rows against 5003 x 4416.)  16 warps leave 128 registers to a thread; 20 and
-// 24 were slower, by 3 % and 7 % at 8 rows and, short of registers, by half and more at 16.
+// against 28672 x 8192, 15.0 instead of 11.7 for 5 rows against 5003 x 4416.)  16 warps leave 128 registers to a thread;
+// 20 and 24 were slower, by 3 % and 7 % at 8 rows and, short of registers, by half and more at 16.
 template <typename T_, int kCols_>
 struct WideShape {
   using T = T_;
