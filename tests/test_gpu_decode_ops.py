@@ -326,6 +326,10 @@ def _check_attention(args, new_lens=None, window=0, scale=None, out=None):
     (4, 2, 128, 32, [200], 64, E4M3, BF16, None, 100),
     (2, 1, 32, 16, [64], 64, S8, F16, None, 0),
     (8, 8, 256, 128, [700], 2, E5M2, BF16, None, 0),
+    (256, 1, 64, 16, [90, 1], 1, E4M3, BF16, None, 0),
+    (60, 4, 128, 64, [700, 130], 3, S8, F16, [3, 1], 0),
+    (1, 1, 16, 16, [i % 23 for i in range(1500)], 1, E5M2, F16, [min(i % 23, 1) for i in range(1500)], 0),
+    (2, 1, 48, 16, [2000 - i for i in range(40)], 2, S8, BF16, None, 0),
 ])
 def test_attention(cuda_device, heads, kv_heads, dim, page, lens, new, code, dtype, new_lens, window):
     args = _attention_inputs(cuda_device, heads, kv_heads, dim, page, lens, new, code, dtype, seed=sum(lens) + dim)
@@ -339,6 +343,8 @@ def test_attention_of_long_and_short_sequences_together(cuda_device):
         args = _attention_inputs(cuda_device, 4, 1, 128, 64, [3, 20000, 64, 0, 7001], new, E4M3, dtype)
         _check_attention(args, [min(n, new) for n in (3, 20000, 64, 0, 7001)])
     _check_attention(_attention_inputs(cuda_device, 6, 3, 64, 16, [9000], 1, S8, BF16), window=5000)
+    for window in (300, 351, 352, 600):
+        _check_attention(_attention_inputs(cuda_device, 8, 2, 128, 64, [5000, 40, 700], 17, E4M3, BF16), window=window)
     _check_attention(_attention_inputs(cuda_device, 2, 1, 256, 128, [6000, 1], 1, E4M3, BF16))
 
 

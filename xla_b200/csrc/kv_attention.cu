@@ -68,7 +68,7 @@ struct AttentionArgs {
   int32_t batch, new_tokens, heads, kv_heads, head_dim, page_shift;
   int32_t rows, blocks;                         // rows of a (sequence, key head), and blocks of them
   int32_t num_pages, table_width, window;       // window: 0 none
-  int32_t unit, extra;                          // tokens of a unit, a multiple of the CTA's step; units without tokens in front of an item
+  int32_t unit_shift, extra;                    // log2 of the tokens of a unit, a multiple of the CTA's step; units without tokens in front of an item
   int32_t min_units;                            // a CTA's share is not smaller
   float scale;                                  // softmax_scale * log2(e)
   int32_t is_bf16;
@@ -91,7 +91,7 @@ __device__ __forceinline__ Span SpanOf(const AttentionArgs& a, int b) {
   const int32_t capacity = a.table_width << a.page_shift;
   s.hi = s.count > 0 ? min(max(len, 0), capacity) : 0;
   s.lo = a.window > 0 ? max(0, s.base + 1 - a.window) & ~(kTile - 1) : 0;
-  s.units = max(1, a.extra + (s.hi > s.lo ? (s.hi - s.lo + a.unit - 1) / a.unit : 0));      // an item without tokens still has rows to write
+  s.units = max(1, a.extra + (s.hi > s.lo ? ((s.hi - s.lo - 1) >> a.unit_shift) + 1 : 0));      // an item without tokens still has rows to write
   return s;
 }
 
@@ -169,9 +169,9 @@ struct Walk {
     if (left > 0) span = SpanOf(a, b);
   }
   __device__ int32_t Units() const { return min(left, span.units - offset); }
-  __device__ int32_t Begin(const AttentionArgs& a) const { return span.lo + max(0, offset - a.extra) * a.unit; }
+  __device__ int32_t Begin(const AttentionArgs& a) const { return span.lo + (max(0, offset - a.extra) << a.unit_shift); }
   __device__ int32_t End(const AttentionArgs& a) const {
-    return static_cast<int32_t>(min(static_cast<int64_t>(span.hi), span.lo + static_cast<int64_t>(max(0, offset + Units() - a.extra)) * a.unit));
+    return static_cast<int32_t>(min(static_cast<int64_t>(span.hi), span.lo + (static_cast<int64_t>(max(0, offset + Units() - a.extra)) << a.unit_shift)));
   }
   __device__ void Next(const AttentionArgs& a) {
     const int32_t n = Units();
@@ -933,11 +933,17 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   const int64_t block = 8 * v.row_tiles, blocks = (rows + block - 1) / block;
   int shift = 4;
   while ((1 << shift) < a.page_tokens) ++shift;
-  const int64_t capacity = a.table_width * a.page_tokens;
-  // A sequence that the table cannot make longer than this is not cut: the second kernel would cost more than it saves.
-  const bool cut = capacity > 512;
-  int64_t unit = cut ? v.step : 1 << 30;
-  while (a.batch * a.kv_heads * blocks * ((capacity + unit - 1) / unit + 16) >= INT32_MAX) unit *= 2;       // the line's positions are 32-bit numbers
+  // The most positions that a sequence's rows see.  Where their keys are few bytes it is not cut: the second kernel would
+  // cost more than it saves.  (Cut and not, in us: 4 sequences, 8 heads of 128, up to 250 tokens 10.5 and 8.8, 500 10.9 and
+  // 11.4, 1000 11.3 and 16.5; heads of 64, 500 tokens 10.7 and 10.3, 1000 13.4 and 14.8; of 256, 250 tokens 11.8 and 12.2; 64
+  // sequences, heads of 128, 250 tokens 17.8 and 16.7, 500 24.4 and 25.2.)
+  const int64_t capacity = a.table_width * a.page_tokens, seen = a.window > 0 ? std::min(capacity, a.window + a.new_tokens + kTile) : capacity;
+  const bool cut = seen * v.dim > (48 << 10);
+  int unit_shift = 30;
+  if (cut)
+    for (unit_shift = 6; (1 << unit_shift) < v.step; ++unit_shift) {}
+  const auto units = [&] { return (seen + (int64_t{1} << unit_shift) - 1) >> unit_shift; };
+  while (a.batch * a.kv_heads * blocks * (units() + 16) >= INT32_MAX) ++unit_shift;       // the line's positions are 32-bit numbers
   // An item costs a CTA about 4 us besides its tokens, as much as it needs for 192 KiB of them shared by the CTAs of an SM.
   // (When it was added, sequences of 0 to 4096 tokens, in us without and with: 41 and 37; 40 rows per key head: 107 and 60.)
   const int extra = cut ? std::max(1, static_cast<int>((192 << 10) / (g_ctas_per_sm[code][shape] * v.step * v.dim * 2))) : 0;
@@ -947,14 +953,14 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
                      static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
-                     static_cast<int32_t>(unit), extra, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
+                     unit_shift, extra, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
   CUtensorMap key_map, value_map;
   const bool none = a.num_pages == 0;                                 // then no page is valid, and no tile is loaded
   const int64_t matrices = none ? 1 : a.num_pages * a.kv_heads;
   Status st = MakeTileMap(&key_map, none ? a.q : a.k_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
   if (st.ok()) st = MakeTileMap(&value_map, none ? a.q : a.v_pages, matrices, none ? 16 : a.page_tokens, none ? 16 : a.head_dim, v.dim == 64 ? 64 : 128);
   if (!st.ok()) return st;
-  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? (capacity + unit - 1) / unit + extra : 1);
+  const int64_t most = a.batch * a.kv_heads * blocks * (cut ? units() + extra : 1);
   int64_t grid = static_cast<int64_t>(DeviceSmCount()) * g_ctas_per_sm[code][shape];
   grid = grid < kMaxCtas ? grid : kMaxCtas;
   // The second kernel walks through an item's pieces, so one is cut into 128 at most.
