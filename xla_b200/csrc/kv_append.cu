@@ -8,9 +8,11 @@
 // is exact down to the subnormals; a scale of amax / max would round every earlier code of the page again each time a
 // token raises it.
 //
-// 4096 tokens for each of 8 sequences, 8 heads of 128, bf16 to e4m3, take 30 us (123 MB, 4.1 TB/s; the bytes alone 18.8), bound
-// by issue.  With a warp for a whole page of 64 slots, which looks at its values in one pass and reads them again to round
-// them, it was 52 us.  One token for each sequence of a batch takes 7.7 us, the host's part of the call.
+// 4096 tokens for each of 8 sequences, 8 heads of 128, bf16 to e4m3, take 26.5 us (123 MB, 4.6 TB/s; the bytes alone 18.8).
+// A block's loads are all under way at once, behind its length and its page, and their rounding follows; only other blocks
+// fill its pauses: four to an SM, at 64 registers and a few of them spilled, where three took 29.4 us, and warps of 8 slots
+// in blocks of 512 threads 40.  With a warp for a whole page of 64 slots, which looks at its values in one pass and reads
+// them again to round them, it was 52 us.  One token for each sequence of a batch takes 7.7 us, the host's part of the call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -122,16 +124,21 @@ struct PageWork {
       Unpack<T>(raw, x);
       *(reinterpret_cast<uint2*>(codes) + held * chunks + c) = EncodeScaled<kCode, kByPower>(x, scale, inverse);
     };
+    if (kKept * lanes <= total) {
 #pragma unroll
-    for (int j = 0; j < kKept; ++j)
-      if (j * lanes < total) store(kept[j], min(lane + j * lanes, total - 1));
+      for (int j = 0; j < kKept; ++j) store(kept[j], lane + j * lanes);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kKept; ++j)
+        if (lane + j * lanes < total) store(kept[j], lane + j * lanes);
+    }
 #pragma unroll 1
     for (int c = lane + kKept * lanes; c < total; c += lanes) store(Load(c), c);
   }
 };
 
 template <int kCode, typename T>
-__global__ void __launch_bounds__(32 * kMostWarps) kv_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(32 * kMostWarps, 4) kv_append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ uint32_t warp_max[kMostWarps];
   const int b = blockIdx.z >> 1, which = blockIdx.z & 1, head = blockIdx.y, warp = threadIdx.x / 32;
   const int page_warps = a.page_tokens / 16, lanes = 32 * page_warps, lane = threadIdx.x % lanes;
@@ -167,12 +174,28 @@ __global__ void __launch_bounds__(32 * kMostWarps) kv_append_kernel(const __grid
   const float before = page >= 0 && work.held > 0 ? *scale_at : 0.0f;
 
   // A lane's chunks are kept, all their loads under way at once (16 slots of 128 columns are 8 for each lane; of wider heads
-  // the rest is read twice).  Past the last chunk it is looked at, and later stored, once more.
+  // the rest is read twice).  From one to the next, `lanes` chunks on, it is some tokens and `rest` chunks, or a token more
+  // where that passes the token's end; a page full of new tokens needs no other test.
   uint4 kept[kKept];
+  const int tokens_on = static_cast<int>(__umulhi(lanes, work.inverse_chunks)), rest = lanes - tokens_on * work.chunks;
+  const int first_token = static_cast<int>(__umulhi(lane, work.inverse_chunks));
+  int place = lane - first_token * work.chunks;             // of the chunk in its token
+  int offset = first_token * work.row_stride + place * 8;
+  const int on = tokens_on * work.row_stride + rest * 8, over = work.row_stride - work.chunks * 8;
+  auto next = [&] {
+    place += rest;
+    offset += on;
+    if (place >= work.chunks) place -= work.chunks, offset += over;
+  };
+  if (kKept * lanes <= work.total) {
 #pragma unroll
-  for (int j = 0; j < kKept; ++j) {
-    kept[j] = make_uint4(0, 0, 0, 0);
-    if (j * lanes < work.total) kept[j] = work.Load(min(lane + j * lanes, work.total - 1));
+    for (int j = 0; j < kKept; ++j, next()) kept[j] = *reinterpret_cast<const uint4*>(work.rows + offset);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kKept; ++j, next()) {
+      kept[j] = make_uint4(0, 0, 0, 0);
+      if (lane + j * lanes < work.total) kept[j] = *reinterpret_cast<const uint4*>(work.rows + offset);
+    }
   }
   constexpr uint32_t kInfinity = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
   auto most_of = [](const uint4& v, uint32_t so_far) {     // the larger magnitudes, as the type's bits, in both halves
