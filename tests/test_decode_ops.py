@@ -139,6 +139,17 @@ def test_functions_refuse_tensors_off_the_device_and_with_strides():
         xla_b200.dot_w4(x, w.t().contiguous().t(), s)
 
 
+def test_a_call_site_that_is_given_more_operands_after_a_call():
+    """The frame that a site keeps between calls is built again."""
+    call = _dot()
+    for want in ("null", "got 4"):
+        with pytest.raises(XlaFfiError) as e:
+            call.execute()
+        assert e.value.code == INVALID and want in str(e.value)
+        _native.mock.mockffi_call_add_arg(call._h, U8, None, 2, (C.c_int64 * 2)(48, 4))
+    call.close()
+
+
 # ---- the plain forms themselves ------------------------------------------------------------------
 def test_plain_quantiser_is_torch_s():
     """Rounding in 64 bits equals torch's conversion from f32, at every code and halfway between them."""

@@ -209,6 +209,7 @@ struct Call {
   // The execute frame, kept between calls of the same site (XLA, too, only updates the addresses in it).
   std::mutex mu;
   bool have_handlers = false, have_frame = false;
+  size_t frame_parts = 0;                        // arguments, results and attributes in the frame
   Registration handlers;
   XLA_FFI_InvokeContext ctx;
   BuiltFrame frame;
@@ -358,13 +359,13 @@ MOCK_EXPORT void mockffi_call_set_arg_data(void* call, int index, void* data) {
   Call* c = static_cast<Call*>(call);
   std::lock_guard<std::mutex> lock(c->mu);
   c->args.at(index).data = data;
-  if (c->have_frame) c->frame.arg_bufs.at(index).data = data;
+  if (c->have_frame && static_cast<size_t>(index) < c->frame.arg_bufs.size()) c->frame.arg_bufs[index].data = data;
 }
 MOCK_EXPORT void mockffi_call_set_ret_data(void* call, int index, void* data) {
   Call* c = static_cast<Call*>(call);
   std::lock_guard<std::mutex> lock(c->mu);
   c->rets.at(index).data = data;
-  if (c->have_frame) c->frame.ret_bufs.at(index).data = data;
+  if (c->have_frame && static_cast<size_t>(index) < c->frame.ret_bufs.size()) c->frame.ret_bufs[index].data = data;
 }
 MOCK_EXPORT void mockffi_call_attr_i64(void* call, const char* name, int64_t v) { AddScalar(static_cast<Call*>(call), name, XLA_FFI_DataType_S64, &v, sizeof(v)); }
 MOCK_EXPORT void mockffi_call_attr_i32(void* call, const char* name, int32_t v) { AddScalar(static_cast<Call*>(call), name, XLA_FFI_DataType_S32, &v, sizeof(v)); }
@@ -415,8 +416,13 @@ MOCK_EXPORT int mockffi_call_invoke(void* call, int stage, void* stream, int dev
   c->ctx.device_ordinal = device_ordinal;
   c->ctx.state = &c->state;
   if (stage == XLA_FFI_ExecutionStage_EXECUTE) {
-    if (!c->have_frame) Build(*c, /*null_data=*/false, &c->ctx, XLA_FFI_ExecutionStage_EXECUTE, &c->frame);
+    const size_t parts = c->args.size() + c->rets.size() + c->attrs.size();
+    if (!c->have_frame || c->frame_parts != parts) {       // built once, and again where the call has been given more since
+      c->frame = BuiltFrame();
+      Build(*c, /*null_data=*/false, &c->ctx, XLA_FFI_ExecutionStage_EXECUTE, &c->frame);
+    }
     c->have_frame = true;
+    c->frame_parts = parts;
     return Finish(h(&c->frame.frame), err, err_len);
   }
   BuiltFrame built;
