@@ -181,8 +181,8 @@ typedef struct B200SD_BlockScaledDotMx {
  * its high four bits.  weight_type S4 is two's complement (-8 .. 7) and has no zero points; U4 (0 .. 15)
  * takes one zero point per group from the low four bits of a byte.  The weights enter as the integers
  * w - z, exactly; sums are f32, a group's sum is multiplied by its scale in f32, and D is rounded once.
- * (One or two rows of x against many rows of weights are converted first: of a row, what lies more than
- * 2^23 below its largest value is rounded to within 2^-34 of that.)  group is 32, 64 or a multiple of
+ * (One or two BF16 rows of x may be converted to scaled f16 first: of a row, what lies more than 2^32 below
+ * its largest finite value is rounded to within 2^-40 of that.)  group is 32, 64 or a multiple of
  * 128 that divides k; n is free; m is at most 64.  m == 0 does nothing. */
 typedef struct B200SD_DotW4 {
   size_t struct_size;            /* sizeof(B200SD_DotW4) */

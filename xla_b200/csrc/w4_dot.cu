@@ -15,13 +15,14 @@
 // The wide kernel takes x as it is, in phases that the warps of a CTA share.  A masked nibble plus an offset is an f16 or
 // bf16 number (1024 + n, 128 + n), and one subtraction leaves w - z, exactly; 9 and 11 instructions for 8 weights.
 // The other one, for one or two rows against many weights, first puts all of x into shared memory, paired, as f16 whatever
-// its type, each row multiplied by the power of two that brings its largest value to 2^13 (what lies 2^23 below that is
-// rounded, to 2^-34 of it).  A nibble under a mask then is an f16 operand as it stands: the subnormal n * 2^-24, or 16 n *
-// 2^-24 for the nibbles one place higher, whose x is stored divided by 16.  That is 5 instructions for 8 weights; the zero
-// point (8 for two's complement) is taken off a group's sum as z times the sum of x over the group, which is formed once
-// in f32.  The sum before that is not much larger than after, so this costs at most a few bits of f32's 24.
+// its type: f16 as it is, a bf16 row multiplied by the power of two that brings its largest finite value to 2^15 (what lies
+// 2^32 below that is rounded, to 2^-40 of it).  A nibble under a mask then is an f16 number as it stands, the subnormal n *
+// 2^-24, or 16 n * 2^-24 for the nibbles one place higher, and one subtraction leaves (w - z) 2^-24, exactly: 9 instructions
+// for 8 weights of either type of x.  (The nibbles themselves as operands are 5, but then the zero points come off a
+// group's sum, as z times the sum of x: where w = z at an outlier of x, the sum before is many times the one after, and what
+// it loses below the outlier's last bit is larger than f32 sums of the definition's terms lose.)
 //
-// Measured with cold caches: 28672 x 8192 in groups of 128 for one row 32 us (3.8 TB/s; the bytes alone take 18.5), 8192 x
+// Measured with cold caches: 28672 x 8192 in groups of 128 for one row 34 us (3.6 TB/s; the bytes alone take 18.5), 8192 x
 // 28672 with zero points for 16 rows 58.6 us, 5003 x 4416 in groups of 32 for 5 rows 10.7 us, 1024 x 2048 for one row 7.6
 // us, the host's part of a call.
 #include <cuda_bf16.h>
@@ -103,10 +104,15 @@ __device__ __forceinline__ uint32_t MaskXor(uint32_t w, uint32_t mask, uint32_t 
 }
 
 // How a word's nibbles become operands; `flip` (8 for two's complement) turns -8 .. 7 into 0 .. 15 with zero point 8.
-// As subnormals, see above:
-__device__ __forceinline__ void DecodeSubnormal(uint32_t w, uint32_t flip, uint32_t (&v)[4]) {
-  v[0] = MaskXor(w, 0x000f000fu, flip), v[1] = MaskXor(w, 0x00f000f0u, flip << 4);
-  v[2] = MaskXor(w >> 8, 0x000f000fu, flip), v[3] = MaskXor(w >> 8, 0x00f000f0u, flip << 4);
+// As (w - z) 2^-24, see above; the offset -z 2^-24 has z in its low bits.
+__device__ __forceinline__ uint32_t SubnormalOffset(uint32_t z) { return 0x80008000u | z * 0x00010001u; }
+__device__ __forceinline__ void DecodeSubnormal(uint32_t w, uint32_t flip, uint32_t offset, uint32_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t a = MaskXor(w >> (8 * i), 0x000f000fu, flip), b = MaskXor(w >> (8 * i), 0x00f000f0u, flip << 4);
+    asm("add.f16x2 %0, %1, %2;" : "=r"(v[2 * i]) : "r"(a), "r"(offset));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[2 * i + 1]) : "r"(b), "r"(0x2c002c00u), "r"(offset));              // times 1 / 16
+  }
 }
 // As w - z, exactly.  The offsets -(1024 + z), -(64 + z) and -(128 + z) of one weight row and group have z in their low bits,
 // so they are put together, not converted.
@@ -173,10 +179,10 @@ __device__ __forceinline__ float2 Unpack(uint32_t w, bool is_bf16) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// All of x to shared memory: `inputs` as paired, scaled f16, `factors` the inverse powers of two (0 for a row that is not
-// finite), `sums` [group][2] the sums of the scaled values over each group (each 128 of k for groups longer than that).
-// The copies are under way before the weights', so that they do not queue behind them; a thread works on the pieces that
-// it has copied itself, in place.  The loops are not unrolled: this code runs once, and its instructions are fetched cold.
+// All of x to shared memory, `inputs`: paired, as f16, scaled if it was bf16; `factors` [row][2] what brings a row's sums back,
+// as two powers of two between which nothing overflows.  The copies are under way before the weights', so that they do not
+// queue behind them; a thread works on the pieces that it has copied itself, in place.  The loops are not unrolled: this
+// code runs once, and its instructions are fetched cold.
 template <int kGroup, int kThreads>
 struct Staging {
   const W4Args& a;
@@ -200,69 +206,67 @@ struct Staging {
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   // `top` [row] holds zeros on entry.
-  __device__ __forceinline__ void Convert(float* factors, uint32_t* top, float* sums) const {
-    const uint32_t lanes = threadIdx.x % 32 < 16 ? 0x0000ffffu : 0xffff0000u;       // 16 lanes in a row share r and the step
+  __device__ __forceinline__ void Convert(float* factors, uint32_t* top) const {
     int r, c;
     uint32_t at;
+    if (a.x_is_bf16) {
+      const uint32_t lanes = threadIdx.x % 32 < 16 ? 0x0000ffffu : 0xffff0000u;     // 16 lanes in a row share r
+      auto finite = [](uint32_t w) {
+        w &= 0x7fff7fffu;
+        if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+        if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+        return w;
+      };
 #pragma unroll 1
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-      Place(i, r, c, at);
-      const uint4 v = LoadShared16(at);
-      const uint32_t both = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-      const uint32_t most = __reduce_max_sync(lanes, max(both & 0xffffu, both >> 16));
-      if (threadIdx.x % 16 == 0 && most > 0) atomicMax(top + r, __float_as_uint(Unpack(most, a.x_is_bf16).x));
+      for (int i = threadIdx.x; i < total; i += kThreads) {
+        Place(i, r, c, at);
+        const uint4 v = LoadShared16(at);
+        const uint32_t both = __vmaxu2(__vmaxu2(finite(v.x), finite(v.y)), __vmaxu2(finite(v.z), finite(v.w)));
+        const uint32_t most = __reduce_max_sync(lanes, max(both & 0xffffu, both >> 16));
+        if (threadIdx.x % 16 == 0 && most > 0) atomicMax(top + r, most << 16);
+      }
+      __syncthreads();
     }
-    __syncthreads();
 #pragma unroll 1
     for (int i = threadIdx.x; i < total; i += kThreads) {
       Place(i, r, c, at);
-      const uint4 v = LoadShared16(at);
-      const uint32_t bits = top[r];
-      const int power = bits >= 0x7f800000u || bits == 0 ? 0 : min(126, 13 - (static_cast<int>(bits >> 23) - 127));
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23), up16 = up * 0.0625f;
-      const float2 x01 = Unpack(v.x, a.x_is_bf16), x23 = Unpack(v.y, a.x_is_bf16), x45 = Unpack(v.z, a.x_is_bf16), x67 = Unpack(v.w, a.x_is_bf16);
-      const __half2 p0 = __floats2half2_rn(x01.x * up, x45.x * up), p1 = __floats2half2_rn(x01.y * up16, x45.y * up16);
-      const __half2 p2 = __floats2half2_rn(x23.x * up, x67.x * up), p3 = __floats2half2_rn(x23.y * up16, x67.y * up16);
-      StoreShared16(at, make_uint4(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1), *reinterpret_cast<const uint32_t*>(&p2), *reinterpret_cast<const uint32_t*>(&p3)));
-      const float2 f0 = __half22float2(p0), f1 = __half22float2(p1), f2 = __half22float2(p2), f3 = __half22float2(p3);
-      float sum = ((f0.x + f0.y) + (f2.x + f2.y)) + 16.0f * ((f1.x + f1.y) + (f3.x + f3.y));
-#pragma unroll
-      for (int o = kGroup / 16; o > 0; o /= 2) sum += __shfl_xor_sync(lanes, sum, o);
-      if (c % (kGroup / 8) == 0) sums[c / (kGroup / 8) * 2 + r] = sum;
-      if (c == 0) factors[r] = bits >= 0x7f800000u ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
+      uint4 v = LoadShared16(at);
+      const int power = top[r] == 0 ? 0 : min(126, 15 - (static_cast<int>(top[r] >> 23) - 127));
+      if (a.x_is_bf16) {
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+        auto scaled = [&](uint32_t w) {
+          const float2 x = Unpack(w, true);
+          const __half2 h = __floats2half2_rn(x.x * up, x.y * up);
+          return *reinterpret_cast<const uint32_t*>(&h);
+        };
+        v = make_uint4(scaled(v.x), scaled(v.y), scaled(v.z), scaled(v.w));
+      }
+      StoreShared16(at, Paired(v));
+      if (c == 0) {
+        const int back = 24 - power, half = back / 2;
+        factors[2 * r] = __uint_as_float(static_cast<uint32_t>(127 + half) << 23);
+        factors[2 * r + 1] = __uint_as_float(static_cast<uint32_t>(127 + back - half) << 23);
+      }
     }
     __syncthreads();
   }
 };
-
-// One result from its definition, for a row of x with an infinity or a NaN: there the sums above would take one from another.
-__device__ __noinline__ float PlainDot(const W4Args& a, int x_row, int row) {
-  float y = 0.0f;
-  const int group = a.k / a.groups;
-  for (int k = 0; k < a.k; ++k) {
-    const int64_t at = static_cast<int64_t>(row) * a.groups + k / group;
-    const int n = a.w[static_cast<int64_t>(row) * (a.k / 2) + k / 2] >> (k % 2 * 4) & 15;
-    const int w = a.is_signed ? (n ^ 8) - 8 : n - (a.zero[at] & 15);
-    const uint32_t raw = static_cast<const uint16_t*>(a.x)[static_cast<int64_t>(x_row) * a.k + k];
-    y += static_cast<float>(w) * Unpack(raw, a.x_is_bf16).x * ValueOf<0>(LoadBits<0>(a.scale, at, a.scale_dtype), a.scale_dtype);
-  }
-  return y;
-}
 
 struct Resident {
   static constexpr int kWarps = 24, kMost = 2;              // kMost: rows of x
   static constexpr int kBlocks = 8;                         // whose sums have room, for one row of x
   static constexpr int kSums = kBlocks * kWarps * kSumStride;
-  // The inverse of each row's power of two, its largest value, and what is behind them up to whole lines of banks.
-  static constexpr int kHead = (kSums * 4 + 2 * kMost * 4 + 127) / 128 * 128, kRing = kWarps * kStages * kStageBytes;
+  // Each row's factors, its largest value, and what is behind them up to whole lines of banks.
+  static constexpr int kHead = (kSums * 4 + 3 * kMost * 4 + 127) / 128 * 128, kRing = kWarps * kStages * kStageBytes;
   static int64_t PerRound(int64_t m, int64_t) { return kBlocks / m; }
-  static int64_t Bytes(int64_t m, int64_t steps, int64_t group) { return kHead + kRing + steps * m * 256 + steps * (128 / group) * 2 * 4; }
+  static int64_t Bytes(int64_t m, int64_t steps) { return kHead + kRing + steps * m * 256; }
 };
 
 // One or two rows of x, all of it in shared memory.  The warps take the units of the CTA in turn and leave their sums of
 // each block in shared memory, where they are added in the order of the warps, as many blocks at a time as have room.  Bound
-// by issue, about 250 instructions of a warp for a unit of 2 KiB, and by 8 us in front and behind: x, the first units, the
-// sums.  24 warps instead of 16: 28672 x 8192 for one row 33.4 and 36.4 us, before half blocks.  kGroup: 32, 64 or 128
+// by issue, about 300 instructions of a warp for a unit of 2 KiB, and by 8 us in front and behind: x, the first units, the
+// sums.  (With the nibbles as operands and zero points taken off the sums it was 250, and 28672 x 8192 for one row 32.5 us
+// instead of 33.8; of that form 24 warps took 33.4 and 16 took 36.4 us, before half blocks.)  kGroup: 32, 64 or 128
 // (which stands for its multiples too).  kScale: the scales' type, kSigned: two's complement, no zero points.
 template <int kGroup, int kScale, bool kSigned>
 __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
@@ -279,8 +283,6 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
   float* factors = sums + S::kSums;
   uint8_t* ring = smem + S::kHead + warp * kStages * kStageBytes;
   uint8_t* resident = smem + S::kHead + S::kRing;
-  float* group_sums = reinterpret_cast<float*>(resident + steps * a.m * 256);
-  constexpr int columns = 2;                                // of the group sums
   constexpr uint32_t flip = kSigned ? 0x00080008u : 0u;
   // A CTA's rows of the weights and of the scales span less than 4 GiB, so 32-bit offsets from its first row do.
   const uint8_t* w_base = a.w + static_cast<int64_t>(first) * row_bytes;
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
       for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(row + r * 16 + h * 8, most)) * a.groups;
   };
 
-  uint32_t* top = reinterpret_cast<uint32_t*>(factors + S::kMost);
+  uint32_t* top = reinterpret_cast<uint32_t*>(factors + 2 * S::kMost);
   if (threadIdx.x < S::kMost) top[threadIdx.x] = 0;
   __syncthreads();
   griddep_wait();
@@ -358,10 +360,9 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
   set_rows(0);
   load_numbers(min(warp, steps - 1), Two());
   asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");         // this thread's part of x has come
-  staging.Convert(factors, top, group_sums);
+  staging.Convert(factors, top);
 
-  // Places of this lane's words and of its pieces of x, of the sums that belong to them; behind the last row of x any will
-  // do, its column is not stored.
+  // Places of this lane's words and of its pieces of x; behind the last row of x any will do, its column is not stored.
   uint32_t weight_at[kPerStep], input_at[4];
 #pragma unroll
   for (int i = 0; i < kPerStep; ++i)
@@ -371,7 +372,6 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
     const int piece = kGroup == 128 ? t * 4 + i : kGroup == 64 ? i / 2 * 8 + t * 2 + i % 2 : i * 4 + t;
     input_at[i] = Kept(smem_u32(resident) + InputPiece<kGroup>(min(g, a.m - 1), piece));
   }
-  const uint32_t sums_at = Kept(smem_u32(group_sums));
 
   const bool half = (last - first - 1) % kRows < 16;        // of the last block only one tile has rows
   uint32_t stage = 0, load_stage = (kStages - 1) * kStageBytes;
@@ -387,11 +387,17 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
           __syncwarp();
           load(load_stage);
           load_stage = stage;
-          const uint32_t inputs = step * (a.m * 256), sums_step = step * (kPerStep * columns * 4);
+          const uint32_t inputs = step * (a.m * 256);
 #pragma unroll
           for (int group = 0; group < kPerStep; ++group) {
             const int holder = (lane & ~3) | group;           // the lane with this group's numbers
             float part[kTiles][4] = {};
+            uint32_t offset[kTiles][2];
+#pragma unroll
+            for (int r = 0; r < kOfUnit; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                offset[r][h] = SubnormalOffset(kSigned ? 8u : kGroup == 128 ? zero[r][h] : __shfl_sync(0xffffffffu, zero[r][h], holder));
             // The words of this group, of rows g and g + 8 of each tile.
             uint32_t w[kTiles][2][kWords];
 #pragma unroll
@@ -415,26 +421,18 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
 #pragma unroll
               for (int r = 0; r < kOfUnit; ++r) {
                 uint32_t low[4], high[4];
-                DecodeSubnormal(w[r][0][i], flip, low);
-                DecodeSubnormal(w[r][1][i], flip, high);
+                DecodeSubnormal(w[r][0][i], flip, offset[r][0], low);
+                DecodeSubnormal(w[r][1][i], flip, offset[r][1], high);
                 Mma<__half>(part[r], low[0], high[0], low[1], high[1], b.x, b.y);
                 Mma<__half>(part[r], low[2], high[2], low[3], high[3], b.z, b.w);
               }
             }
-            // The zero points' share, then the scales.
-            const uint2 sum_bits = LoadShared8(sums_at + sums_step + group * (columns * 4));
-            const float sum0 = __uint_as_float(sum_bits.x), sum1 = __uint_as_float(sum_bits.y);
 #pragma unroll
             for (int r = 0; r < kOfUnit; ++r) {
               float s0 = ValueOf<kScale>(scale[r][0], kScale), s1 = ValueOf<kScale>(scale[r][1], kScale);
-              float z0 = -0x1p-21f, z1 = -0x1p-21f;            // -8 * 2^-24
-              if (!kSigned) z0 = -0x1p-24f * static_cast<float>(zero[r][0]), z1 = -0x1p-24f * static_cast<float>(zero[r][1]);
-              if (kGroup < 128) {
-                s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
-                if (!kSigned) z0 = __shfl_sync(0xffffffffu, z0, holder), z1 = __shfl_sync(0xffffffffu, z1, holder);
-              }
-              acc[r][0] = fmaf(fmaf(z0, sum0, part[r][0]), s0, acc[r][0]), acc[r][1] = fmaf(fmaf(z0, sum1, part[r][1]), s0, acc[r][1]);
-              acc[r][2] = fmaf(fmaf(z1, sum0, part[r][2]), s1, acc[r][2]), acc[r][3] = fmaf(fmaf(z1, sum1, part[r][3]), s1, acc[r][3]);
+              if (kGroup < 128) s0 = __shfl_sync(0xffffffffu, s0, holder), s1 = __shfl_sync(0xffffffffu, s1, holder);
+              acc[r][0] = fmaf(part[r][0], s0, acc[r][0]), acc[r][1] = fmaf(part[r][1], s0, acc[r][1]);
+              acc[r][2] = fmaf(part[r][2], s1, acc[r][2]), acc[r][3] = fmaf(part[r][3], s1, acc[r][3]);
             }
           }
           stage = stage == (kStages - 1) * kStageBytes ? 0 : stage + kStageBytes;
@@ -471,8 +469,7 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
         float y = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) y += part[w * a.m * kSumStride];
-        y = factors[x_row] != 0.0f ? y * 0x1p24f * factors[x_row] : PlainDot(a, x_row, at);
-        y += bias;
+        y = y * factors[2 * x_row] * factors[2 * x_row + 1] + bias;
         const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
         if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
         else if (a.d_dtype == kF16) static_cast<__half*>(a.d)[place] = __float2half_rn(y);
@@ -497,7 +494,7 @@ struct WideShape {
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   // Steps of a phase: as many as fit, twice, for every phase costs a barrier.
   static int64_t Phase(int64_t m, int64_t steps) { return std::min<int64_t>(steps, ((227 * 1024 - kRing - 64) / (2 * m) - 16) / 256); }
-  static int64_t Bytes(int64_t m, int64_t steps, int64_t) { return kRing + 64 + m * std::max<int64_t>(2 * (Phase(m, steps) * 256 + 16), kWarps * kSumStride * 4); }
+  static int64_t Bytes(int64_t m, int64_t steps) { return kRing + 64 + m * std::max<int64_t>(2 * (Phase(m, steps) * 256 + 16), kWarps * kSumStride * 4); }
 };
 
 template <int kGroup, typename S>
@@ -714,7 +711,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
 
 struct Variant {
   void (*kernel)(W4Args);
-  int64_t (*bytes)(int64_t m, int64_t steps, int64_t group);
+  int64_t (*bytes)(int64_t m, int64_t steps);
   int64_t (*per_round)(int64_t m, int64_t steps);
   int warps, registers;
 };
@@ -813,7 +810,7 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
     stats->launches = first.launches + second.launches;
     return st;
   }
-  const int64_t steps = (a.k + 127) / 128, step_group = std::min<int64_t>(a.group, 128);
+  const int64_t steps = (a.k + 127) / 128;
   const int group_at = a.group == 32 ? 0 : a.group == 64 ? 1 : 2, scale_at = a.scale_dtype == kF16 ? 0 : a.scale_dtype == kBF16 ? 1 : 2;
   const Variant& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
   // With x resident every CTA converts all of it first, and decodes for less afterwards.  That pays for one and two rows of x
@@ -823,9 +820,9 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
   // 131072, k 2048 46.7 and 40.6; m 3, n 28672, k 8192 43.0 and 41.4; group 32, k 8192: m 1, n 8192 16.8 and 20.0, m 2 18.0
   // and 20.1, but n 2048 8.1 and 8.0; m 3, n 131072, k 4096 125 and 119.
   const int64_t enough = DeviceSmCount() * (a.group == 32 ? 32 * a.m : 64 * (a.m + 1));
-  const bool is_resident = a.m <= Resident::kMost && a.n >= enough && a.k >= 4096 && resident.bytes(a.m, steps, step_group) <= kSmemPerCta;
+  const bool is_resident = a.m <= Resident::kMost && a.n >= enough && a.k >= 4096 && resident.bytes(a.m, steps) <= kSmemPerCta;
   const Variant& v = is_resident ? resident : TheVariants().wide[a.x_dtype == kBF16][group_at][a.m <= 8 ? 0 : a.m <= 16 ? 1 : 2];
-  const int bytes = static_cast<int>(v.bytes(a.m, steps, step_group)), threads = v.warps * 32;
+  const int bytes = static_cast<int>(v.bytes(a.m, steps)), threads = v.warps * 32;
   const int by_registers = 65536 / (threads * ((v.registers + 7) / 8 * 8)), by_smem = static_cast<int>(kSmemPerSm / (bytes + kSmemReserved));
   const int per_sm = std::max(1, std::min({by_registers, by_smem, 2048 / threads}));
   // One CTA per resident slot, each with its even share of the rows, but no more CTAs than tiles of 8 rows.
