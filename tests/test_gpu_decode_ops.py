@@ -123,6 +123,54 @@ def test_dot_w4_many_rows_large_magnitudes_and_infinities(cuda_device):
         assert torch.equal(out[1].isposinf(), want.isposinf()) and torch.equal(out[1].isneginf(), want.isneginf()) and torch.equal(out[1].isnan(), want.isnan())
 
 
+@pytest.mark.parametrize("m,n,k,group,dtype,zeros,bias,scale_dtype", [
+    (1, 1, 32, 32, BF16, False, True, F32),        # groups of 32: any size ...
+    (1, 7, 64, 32, F16, True, False, BF16),
+    (1, 300, 96, 32, BF16, True, True, F16),
+    (1, 5003, 4416, 32, F16, False, True, F16),
+    (2, 100, 2080, 32, F16, True, False, F32),
+    (2, 9, 8192, 32, BF16, False, True, BF16),
+    (2, 300, 1024, 32, BF16, True, True, BF16),    # ... but not a short k for two rows
+    (1, 77, 32768, 32, F16, True, True, F32),      # and x has to fit
+    (1, 50000, 4096, 128, F16, True, True, F32),   # longer groups: 200 million weights
+    (1, 50001, 4096, 256, BF16, True, False, BF16),
+    (1, 49000, 4160, 64, F16, False, True, F16),   # k ends inside a step
+    (1, 49000, 4160, 64, BF16, True, True, F32),
+    (2, 49000, 4224, 384, BF16, False, True, BF16),
+    (2, 49000, 4160, 64, F16, False, False, F32),
+    (1, 20000, 12800, 640, F16, True, True, BF16),
+    (2, 50000, 4096, 128, F16, True, True, F16),   # not two rows with zero points
+])
+def test_dot_w4_of_one_and_two_rows(cuda_device, m, n, k, group, dtype, zeros, bias, scale_dtype):
+    """Both sides of the choice between the two kernels."""
+    inputs = _dot_inputs(cuda_device, m, n, k, group, dtype, zeros, bias, scale_dtype, seed=m + n + k)
+    x, w, scale, zero, b = inputs
+    _check_dot(xla_b200.dot_w4(x, w, scale, zero=zero, bias=b), inputs, k)
+    _check_dot(xla_b200.dot_w4(x, w, scale, zero=zero, bias=b, out_dtype=F32), inputs, k)
+    x[m - 1, k - 1] = math.inf                     # reaches its own row only, with the sign of the last weight
+    out = xla_b200.dot_w4(x, w, scale, zero=zero, out_dtype=F32)
+    if m == 2:
+        _check_dot(out[:1], [x[:1], w, scale, zero, None], k)
+    last = ref.weights(w[:, -1:], None if zero is None else zero[:, -1:], 2)[:, 1]
+    assert torch.equal(out[m - 1].isposinf(), last > 0) and torch.equal(out[m - 1].isneginf(), last < 0) and torch.equal(out[m - 1].isnan(), last == 0)
+    assert _status() == 0
+
+
+def test_dot_w4_every_nibble_of_many_rows_and_longer_groups(cuda_device):
+    """Powers of two at one place of k: exact, for every nibble and zero point, in groups of 64 and 128."""
+    n, k = 50000, 4096
+    w = (torch.arange(n * k // 2, device=cuda_device) * 2654435761 // 65536 % 256).to(torch.uint8).reshape(n, k // 2)
+    for group in (64, 128):
+        scale = torch.ones((n, k // group), dtype=F32, device=cuda_device)
+        for zero in (None, (torch.arange(n * k // group, device=cuda_device) % 16).to(torch.uint8).reshape(n, k // group)):
+            for at in (0, 3, 6, 31, 32, 77, 127, 2050, 4095):
+                x = torch.zeros((1, k), dtype=BF16, device=cuda_device)
+                x[0, at] = -2.0 ** (at % 7)
+                byte = w[:, at // 2] >> (4 * (at % 2)) & 15
+                want = (byte ^ 8).double() - 8 if zero is None else byte.double() - zero[:, at // group].double()
+                assert torch.equal(xla_b200.dot_w4(x, w, scale, zero=zero, out_dtype=F32)[0].double(), want * -2.0 ** (at % 7))
+
+
 @pytest.mark.parametrize("m,n,k,group,dtype,zeros,outlier", [
     (1, 50000, 4096, 128, BF16, False, 99840.0),
     (1, 50000, 4096, 128, F16, True, 60000.0),

@@ -813,14 +813,21 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
   const int64_t steps = (a.k + 127) / 128;
   const int group_at = a.group == 32 ? 0 : a.group == 64 ? 1 : 2, scale_at = a.scale_dtype == kF16 ? 0 : a.scale_dtype == kBF16 ? 1 : 2;
   const Variant& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
-  // With x resident every CTA converts all of it first, and decodes for less afterwards.  That pays for one and two rows of x
-  // where a CTA has many rows of weights, fewer of them where groups are short, and a line of k long enough for its warps.
-  // Resident against wide in us, two's complement: m 1, group 128, k 8192: n 8192 15.1 and 13.6, n 16384 22.3 and 23.0, n
-  // 28672 33.0 and 40.9; m 2, the same: n 16384 24.8 and 22.9, n 28672 37.5 and 41.0; m 2, n 28672, k 4096 23.8 and 22.1, n
-  // 131072, k 2048 46.7 and 40.6; m 3, n 28672, k 8192 43.0 and 41.4; group 32, k 8192: m 1, n 8192 16.8 and 20.0, m 2 18.0
-  // and 20.1, but n 2048 8.1 and 8.0; m 3, n 131072, k 4096 125 and 119.
-  const int64_t enough = DeviceSmCount() * (a.group == 32 ? 32 * a.m : 64 * (a.m + 1));
-  const bool is_resident = a.m <= Resident::kMost && a.n >= enough && a.k >= 4096 && resident.bytes(a.m, steps) <= kSmemPerCta;
+  // With x resident every CTA pairs all of it first, and has fewer instructions for the weights afterwards.  Which of the two
+  // is faster, resident against wide in us, calls one after the other in a graph:
+  //   groups of 32: m 1, 256 x 512 2.9 and 3.2, 4096 x 4096 6.9 and 8.4, 28672 x 8192 39.2 and 54.7; m 2 the same 3.0 and
+  //     3.2, 7.7 and 8.4, 41.9 and 55.0, but 65536 x 1024 20.8 and 18.3, 16384 x 1024 7.3 and 7.2: a short k does not pay for
+  //     the second row.
+  //   longer groups, two's complement (groups of 128): m 1, 8192 x 8192 15.6 and 13.5, 16384 x 8192 22.0 and 22.0, 36864 x 4608
+  //     25.5 and 25.1, 24576 x 8192 29.9 and 35.0, 28672 x 8192 33.8 and 38.7, 57344 x 8192 57.6 and 73.4; m 2, 16384 x 8192 24.4
+  //     and 22.0, 24576 x 8192 33.0 and 35.0, 57344 x 8192 61.7 and 73.5, 131072 x 2048 45.5 and 41.7.
+  //   zero points, which cost this kernel more: m 1, 28672 x 6144 31.2 and 31.2, 24576 x 8192 35.7 and 37.0, 57344 x 8192 69.8 and
+  //     76.1; m 2, 24576 x 8192 39.0 and 37.1, 131072 x 4096 80.2 and 75.4.
+  // So groups of 32 have it unless k is short for two rows, and of the others many weights, about 200 million, with k long
+  // enough for the warps of a CTA, two rows with zero points never.
+  const bool pays = a.group == 32 ? a.m == 1 || a.k >= 2048
+                                  : a.n * a.k >= 200'000'000 && a.k >= 4096 && (a.m == 1 || a.weight_type == kS4);
+  const bool is_resident = a.m <= Resident::kMost && pays && resident.bytes(a.m, steps) <= kSmemPerCta;
   const Variant& v = is_resident ? resident : TheVariants().wide[a.x_dtype == kBF16][group_at][a.m <= 8 ? 0 : a.m <= 16 ? 1 : 2];
   const int bytes = static_cast<int>(v.bytes(a.m, steps)), threads = v.warps * 32;
   const int by_registers = 65536 / (threads * ((v.registers + 7) / 8 * 8)), by_smem = static_cast<int>(kSmemPerSm / (bytes + kSmemReserved));
