@@ -3,8 +3,9 @@
 // It declares the structs, numbers and function-table entries that ffi_handlers.cc and mock_ffi_runtime.cc use, and
 // nothing else, so that the handlers can be built and driven by the mock runtime where XLA's own headers are not at
 // hand.  Both libraries of such a build agree with each other; the order of the fields is this file's own.  A process
-// that holds the real XLA needs a build against its headers (`make XLA_ROOT=<xla checkout>`): the version number
-// below is one that no XLA has, and registration compares it, so that a mixed pair is refused.
+// that holds the real XLA needs a build against its headers (`make XLA_ROOT=<xla checkout>`).  A mixed pair is refused: the
+// version number below is one that no XLA has, and b200sd_ffi_register compares it; and a call frame's size, which is the
+// first field of everybody's frames, has a mark above any real size, without which a handler leaves a frame alone.
 #ifndef B200SD_FFI_STANDIN_C_API_H_
 #define B200SD_FFI_STANDIN_C_API_H_
 
@@ -178,7 +179,7 @@ struct XLA_FFI_Api {
 #define XLA_FFI_Args_STRUCT_SIZE sizeof(XLA_FFI_Args)
 #define XLA_FFI_Attrs_STRUCT_SIZE sizeof(XLA_FFI_Attrs)
 #define XLA_FFI_Buffer_STRUCT_SIZE sizeof(XLA_FFI_Buffer)
-#define XLA_FFI_CallFrame_STRUCT_SIZE sizeof(XLA_FFI_CallFrame)
+#define XLA_FFI_CallFrame_STRUCT_SIZE (sizeof(XLA_FFI_CallFrame) | size_t{XLA_FFI_API_MAJOR} << 32)
 #define XLA_FFI_Error_Destroy_Args_STRUCT_SIZE sizeof(XLA_FFI_Error_Destroy_Args)
 #define XLA_FFI_Error_GetDetails_Args_STRUCT_SIZE sizeof(XLA_FFI_Error_GetDetails_Args)
 #define XLA_FFI_Metadata_STRUCT_SIZE sizeof(XLA_FFI_Metadata)

@@ -3,6 +3,7 @@
 #ifndef B200SD_FFI_STANDIN_FFI_H_
 #define B200SD_FFI_STANDIN_FFI_H_
 
+#include <cstdio>
 #include <cstring>
 #include <exception>
 #include <initializer_list>
@@ -217,9 +218,15 @@ inline XLA_FFI_Error* Report(const XLA_FFI_Api* api, int code, const char* messa
   return api->XLA_FFI_Error_Create(&a);
 }
 
-// One call of a handler.  No exception leaves it.
+// One call of a handler.  No exception leaves it.  A frame of another layout is not read, not even for what an error would
+// have to be made with: a runtime that asks the handler for its version, as all do before they register one, gets none and
+// refuses it.
 template <typename Fn>
 XLA_FFI_Error* Invoke(const XLA_FFI_CallFrame* f, Fn fn, Binding binding, uint32_t traits) {
+  if (f->struct_size != XLA_FFI_CallFrame_STRUCT_SIZE) {
+    std::fprintf(stderr, "libb200_scaled_dot was built without XLA's FFI headers and cannot be called by XLA; rebuild it with XLA_ROOT=<xla checkout>\n");
+    return nullptr;
+  }
   for (XLA_FFI_Extension_Base* e = f->extension_start; e != nullptr; e = e->next) {
     if (e->type != XLA_FFI_Extension_Metadata) continue;
     XLA_FFI_Metadata* m = reinterpret_cast<XLA_FFI_Metadata_Extension*>(e)->metadata;
