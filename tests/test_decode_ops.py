@@ -1,6 +1,7 @@
 """What the decode-step calls accept and refuse, without a device: call frames at the instantiate stage, the C entry
 points' checks, and the plain 64-bit forms that the device tests compare with."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -189,3 +190,28 @@ def test_plain_attention_against_torch():
     assert torch.allclose(out[0].transpose(0, 1), want, atol=1e-12)
     scores = (q[0].transpose(0, 1).double() @ full[0].transpose(1, 2) * 32 ** -0.5).masked_fill(~mask, float("-inf"))
     assert torch.allclose(lse[0].t(), torch.logsumexp(scores, -1), atol=1e-12)
+
+
+def test_threads_on_one_call_site_get_their_own_messages(monkeypatch):
+    """Both calls have failed before either reads its message."""
+    both, got = threading.Barrier(2), {}
+
+    def failing(handle, stream, device, err, size):
+        err.value = threading.current_thread().name.encode()
+        both.wait(10)
+        return INVALID
+
+    call = _dot()
+    monkeypatch.setattr(_native.mock, "mockffi_call_execute", failing)
+
+    def work():
+        with pytest.raises(XlaFfiError) as e:
+            call.execute()
+        got[threading.current_thread().name] = str(e.value)
+
+    threads = [threading.Thread(target=work, name=name) for name in ("first", "second")]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert "first" in got["first"] and "second" in got["second"], got

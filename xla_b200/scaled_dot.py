@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 import dataclasses
 import enum
+import threading
 from typing import NamedTuple, Optional, Sequence
 
 from . import _native
@@ -120,13 +121,22 @@ def _err_buf():
     return C.create_string_buffer(1024)
 
 
+class _OfThread(threading.local):
+    """A thread's message buffer of `execute`, kept: a site is executed many times, and by any number of threads."""
+
+    def __init__(self):
+        self.err = _err_buf()
+
+
+_of_thread = _OfThread()
+
+
 class FfiCall:
     """One custom-call site bound to a target registered with the (mock) XLA FFI runtime."""
 
     def __init__(self, target: str, operands: Sequence, results: Sequence, attrs: dict):
         _native.ensure_registered()
         self._h = _native.mock.mockffi_call_new(target.encode())
-        self._err = _err_buf()              # of `execute`, kept: a site is executed many times
         self.target = target
         self._keep = []
         for op in operands:
@@ -178,9 +188,10 @@ class FfiCall:
         self._check(_native.mock.mockffi_call_run(self._h, stream, device, err, len(err)), err)
 
     def execute(self, stream: int = 0, device: int = 0) -> None:
-        rc = _native.mock.mockffi_call_execute(self._h, stream, device, self._err, 1024)
+        err = _of_thread.err
+        rc = _native.mock.mockffi_call_execute(self._h, stream, device, err, 1024)
         if rc != 0:
-            self._check(rc, self._err)
+            self._check(rc, err)
 
     def set_operand(self, index: int, tensor) -> None:
         _native.mock.mockffi_call_set_arg_data(self._h, index, tensor.data_ptr())
