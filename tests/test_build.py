@@ -47,3 +47,39 @@ def test_other_ffi_headers_rebuild_what_includes_them(make, tmp_path):
     assert make(f"XLA_ROOT={xla}") == set()
     assert make() == OF_THE_FFI_LAYER
     assert make() == set()
+
+
+@pytest.mark.parametrize("compiler,ready,named,last,want", [
+    (True, True, None, "ffi_standin", []),                 # the stand-in headers
+    (True, False, None, None, []),
+    (True, True, "xla", "ffi_standin", ["xla"]),
+    (True, True, None, "xla", ["xla"]),                    # built for an XLA that is still there ...
+    (True, True, None, "gone", None),                      # ... or not any more: the libraries stay as they are
+    (True, False, None, "gone", []),
+    (False, True, None, "ffi_standin", None),              # no compiler: ready libraries serve
+    (False, True, "xla", None, None),
+    (False, False, None, None, RuntimeError),
+])
+def test_what_build_makes(monkeypatch, tmp_path, compiler, ready, named, last, want):
+    import __graft_entry__ as entry
+
+    lib = tmp_path / "lib"
+    lib.mkdir()
+    header = tmp_path / "xla" / "xla" / "ffi" / "api" / "ffi.h"
+    header.parent.mkdir(parents=True)
+    header.write_text("")
+    for name in entry.LIBRARIES if ready else ():
+        (lib / name).write_text("")
+    if last is not None:
+        (lib / "ffi_root").write_text((last if last == "ffi_standin" else str(tmp_path / last)) + "\n")
+    made = []
+    monkeypatch.setattr(entry, "LIB", str(lib))
+    monkeypatch.setattr(entry, "XLA_ROOT", str(tmp_path / (named or "none")))
+    monkeypatch.setattr(entry.shutil, "which", lambda name: "/bin/nvcc" if compiler else None)
+    monkeypatch.setattr(entry.subprocess, "check_call", lambda command: made.append([a[len("XLA_ROOT="):] for a in command if a.startswith("XLA_ROOT=")]))
+    if want is RuntimeError:
+        with pytest.raises(RuntimeError):
+            entry._make_libraries()
+    else:
+        entry._make_libraries()
+    assert made == ([] if want in (None, RuntimeError) else [[str(tmp_path / w) for w in want]])
