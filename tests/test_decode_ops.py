@@ -215,3 +215,15 @@ def test_threads_on_one_call_site_get_their_own_messages(monkeypatch):
     for t in threads:
         t.join()
     assert "first" in got["first"] and "second" in got["second"], got
+
+
+def test_workspace_bytes_are_those_of_a_call_that_is_served():
+    """Zero for what the call refuses or does nothing for, sizes whose products leave 64 bits among them."""
+    size = xla_b200.paged_attention_workspace_bytes
+    assert size(4096, 64, 4096, 1024, 128) > 0 and size(1, 1, 1, 1, 16) > 0
+    base = dict(batch=2, new_tokens=1, heads=4, kv_heads=2, head_dim=64)
+    for kw in (dict(batch=0), dict(new_tokens=0), dict(batch=-1), dict(new_tokens=-1), dict(batch=4097), dict(new_tokens=65), dict(heads=5), dict(heads=0), dict(heads=8192), dict(kv_heads=0),
+               dict(heads=4096, kv_heads=2048), dict(head_dim=20), dict(head_dim=0), dict(head_dim=272), dict(new_tokens=2 ** 62), dict(heads=2 ** 62),
+               dict(batch=4096, new_tokens=64, heads=4096, kv_heads=512, head_dim=256)):
+        sizes = {**base, **kw}
+        assert size(*sizes.values()) == 0, kw

@@ -919,7 +919,11 @@ Status ValidatePagedAttention(const B200SD_PagedAttention& a, bool check_pointer
 }
 
 size_t PagedAttentionWorkspaceBytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-  if (batch < 1 || new_tokens < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || head_dim < 16 || head_dim > 256) return 0;
+  B200SD_PagedAttention a{};
+  a.struct_size = sizeof(a);
+  a.batch = batch, a.new_tokens = new_tokens, a.heads = heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
+  a.page_tokens = 16, a.q_dtype = kBF16, a.cache_dtype = kS8;
+  if (batch == 0 || new_tokens == 0 || !ValidatePagedAttention(a, /*check_pointers=*/false).ok()) return 0;
   const Variant& v = kVariants[0][ShapeIndex(head_dim, new_tokens * (heads / kv_heads))];
   return kMaxCtas * (2 * v.slot * sizeof(float) + sizeof(int4));
 }
