@@ -436,6 +436,18 @@ def test_attention_of_many_sequences(cuda_device):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("window", [2 ** 30 - 1, 2 ** 30, 2 ** 31, 2 ** 63 - 64, 2 ** 63 - 1])
+def test_attention_with_a_window_larger_than_any_sequence(cuda_device, window):
+    """Such a window is none, and the work is split over the card as without one: the second launch joins it."""
+    args = _attention_inputs(cuda_device, 4, 1, 128, 64, [9000, 70], 2, E4M3, BF16)
+    want = xla_b200.paged_attention_kv8(*args, return_lse=True)
+    before = xla_b200.launch_count()
+    got = xla_b200.paged_attention_kv8(*args, window=window, return_lse=True)
+    assert xla_b200.launch_count() - before == 2
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _check_attention(args, window=window, out=got)
+
+
 def test_attention_keeps_a_bad_page_scale_to_the_rows_that_see_it(cuda_device):
     """The second drafted token opens a page whose scales are no numbers: the first token's rows do not see it."""
     for bad in (math.nan, math.inf):

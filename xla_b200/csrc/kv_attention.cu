@@ -941,7 +941,8 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
   // cost more than it saves.  (Cut and not, in us: 4 sequences, 8 heads of 128, up to 250 tokens 10.5 and 8.8, 500 10.9 and
   // 11.4, 1000 11.3 and 16.5; heads of 64, 500 tokens 10.7 and 10.3, 1000 13.4 and 14.8; of 256, 250 tokens 11.8 and 12.2; 64
   // sequences, heads of 128, 250 tokens 17.8 and 16.7, 500 24.4 and 25.2.)
-  const int64_t capacity = a.table_width * a.page_tokens, seen = a.window > 0 ? std::min(capacity, a.window + a.new_tokens + kTile) : capacity;
+  const int64_t window = std::min(a.window, int64_t{1} << 30);          // as good as none: no sequence is longer
+  const int64_t capacity = a.table_width * a.page_tokens, seen = window > 0 ? std::min(capacity, window + a.new_tokens + kTile) : capacity;
   const bool cut = seen * v.dim > (48 << 10);
   int unit_shift = 30;
   if (cut)
@@ -956,7 +957,7 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
                      reinterpret_cast<int4*>(static_cast<float*>(a.workspace) + int64_t{kMaxCtas} * 2 * v.slot),
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
-                     static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(a.window < (1 << 30) ? a.window : 1 << 30),
+                     static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(window),
                      unit_shift, extra, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
   CUtensorMap key_map, value_map;
   const bool none = a.num_pages == 0;                                 // then no page is valid, and no tile is loaded
