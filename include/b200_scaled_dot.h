@@ -266,6 +266,9 @@ typedef struct B200SD_PagedAttention {
 /* One-time set-up for the current device (kernel attributes, SM count).  Called implicitly by the
  * first launch on a device; call it yourself before capturing a stream into a CUDA graph. */
 int b200sd_init_device(char* err, size_t err_len);
+/* The same, and what the 4-bit dot and the attention need beyond it.  Their first launch on a device calls it, too; its
+ * failure is theirs and leaves the scaled dots alone. */
+int b200sd_init_decode_operators(char* err, size_t err_len);
 
 /* Replaces the cublasLtMatmul call of xla/stream_executor/cuda/cuda_blas_lt.cc:559-564 (FP8). */
 int b200sd_scaled_dot_f8(const B200SD_ScaledDotF8* args, void* cuda_stream, char* err, size_t err_len);

@@ -154,6 +154,7 @@ mock = _load(MOCK_LIB)
 
 _ERR = (C.c_char_p, C.c_size_t)
 product.b200sd_init_device.argtypes = [*_ERR]
+product.b200sd_init_decode_operators.argtypes = [*_ERR]
 product.b200sd_scaled_dot_f8.argtypes = [C.POINTER(ScaledDotF8Args), C.c_void_p, *_ERR]
 product.b200sd_dot_s8.argtypes = [C.POINTER(DotS8Args), C.c_void_p, *_ERR]
 product.b200sd_check_scaled_dot_f8.argtypes = [C.POINTER(ScaledDotF8Args), *_ERR]

@@ -35,6 +35,8 @@ struct DeviceState {
   Status init_status;
   int sm_count = 0;
   uint32_t* status_word = nullptr;
+  std::once_flag decode_once;
+  Status decode_status;
 };
 DeviceState g_state[64];
 std::atomic<uint64_t> g_launches{0};
@@ -91,8 +93,6 @@ Status InitDevice(int device) {
     st.init_status = InitDenseKernels();
     if (st.init_status.ok()) st.init_status = InitSkinnyKernels();
     if (st.init_status.ok()) st.init_status = InitMxKernels();
-    if (st.init_status.ok()) st.init_status = InitAttentionKernels();
-    if (st.init_status.ok()) st.init_status = InitW4Kernels();
     // A persisted tuning result named by the environment is loaded with the first device (a file
     // that cannot be read or parsed makes the first call fail loudly instead of being ignored).
     static std::once_flag table_once;
@@ -105,6 +105,20 @@ Status InitDevice(int device) {
     });
   });
   return st.init_status;
+}
+
+// Beyond that, what the operators of a decode step need.  On its own, so that a scaled dot neither waits for their kernels
+// to be loaded nor fails where they cannot be.
+Status InitDecodeOperators(int device) {
+  Status base = InitDevice(device);
+  if (!base.ok()) return base;
+  DeviceState& st = g_state[device];
+  std::call_once(st.decode_once, [&] {
+    st.decode_status = InitAttentionKernels();
+    if (st.decode_status.ok()) st.decode_status = InitW4Kernels();
+    if (TuningEnvInt("B200SD_FAIL_DECODE_SETUP", 0)) st.decode_status = Status::Error(kInternal, "set-up of the decode-step operators made to fail");
+  });
+  return st.decode_status;
 }
 
 int DeviceSmCount() {
@@ -288,6 +302,11 @@ int b200sd_init_device(char* err, size_t err_len) {
   if (e != cudaSuccess) return CopyStatus(Status::Error(kInternal, std::string("cudaGetDevice: ") + cudaGetErrorString(e)), err, err_len);
   return CopyStatus(InitDevice(device), err, err_len);
 }
+int b200sd_init_decode_operators(char* err, size_t err_len) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return CopyStatus(Status::Error(kInternal, "cudaGetDevice failed"), err, err_len);
+  return CopyStatus(InitDecodeOperators(device), err, err_len);
+}
 
 int b200sd_scaled_dot_f8(const B200SD_ScaledDotF8* args, void* cuda_stream, char* err, size_t err_len) {
   if (args == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args is null"), err, err_len);
@@ -375,15 +394,15 @@ int b200sd_check_paged_attention(const B200SD_PagedAttention* args, char* err, s
 
 }  // extern "C"
 namespace {
-// Checks, sets the device up and launches one operator of a decode step.
+// Checks, sets the device up (`init`) and launches one operator of a decode step.
 template <typename Args>
-int RunDecodeOp(const Args* args, void* cuda_stream, Status (*validate)(const Args&, bool),
+int RunDecodeOp(const Args* args, void* cuda_stream, Status (*validate)(const Args&, bool), Status (*init)(int),
                 Status (*launch)(const Args&, cudaStream_t, LaunchStats*), char* err, size_t err_len) {
   if (args == nullptr) return CopyStatus(Status::Error(kInvalidArgument, "args is null"), err, err_len);
   Status st = validate(*args, /*check_pointers=*/true);
   int device = 0;
   if (st.ok() && cudaGetDevice(&device) != cudaSuccess) st = Status::Error(kInternal, "cudaGetDevice failed");
-  if (st.ok()) st = InitDevice(device);
+  if (st.ok()) st = init(device);
   LaunchStats stats;
   if (st.ok()) st = launch(*args, static_cast<cudaStream_t>(cuda_stream), &stats);
   if (st.ok()) g_launches.fetch_add(stats.launches, std::memory_order_relaxed);
@@ -393,13 +412,13 @@ int RunDecodeOp(const Args* args, void* cuda_stream, Status (*validate)(const Ar
 extern "C" {
 
 int b200sd_dot_w4(const B200SD_DotW4* args, void* cuda_stream, char* err, size_t err_len) {
-  return RunDecodeOp(args, cuda_stream, ValidateDotW4, LaunchDotW4, err, err_len);
+  return RunDecodeOp(args, cuda_stream, ValidateDotW4, InitDecodeOperators, LaunchDotW4, err, err_len);
 }
 int b200sd_kv_cache_append(const B200SD_KvCacheAppend* args, void* cuda_stream, char* err, size_t err_len) {
-  return RunDecodeOp(args, cuda_stream, ValidateKvCacheAppend, LaunchKvCacheAppend, err, err_len);
+  return RunDecodeOp(args, cuda_stream, ValidateKvCacheAppend, InitDevice, LaunchKvCacheAppend, err, err_len);
 }
 int b200sd_paged_attention(const B200SD_PagedAttention* args, void* cuda_stream, char* err, size_t err_len) {
-  return RunDecodeOp(args, cuda_stream, ValidatePagedAttention, LaunchPagedAttention, err, err_len);
+  return RunDecodeOp(args, cuda_stream, ValidatePagedAttention, InitDecodeOperators, LaunchPagedAttention, err, err_len);
 }
 size_t b200sd_paged_attention_workspace_bytes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
   return PagedAttentionWorkspaceBytes(batch, new_tokens, heads, kv_heads, head_dim);

@@ -315,6 +315,10 @@ ffi::Error InitializeDevice() {
   char msg[512];
   return FromCode(b200sd_init_device(msg, sizeof(msg)), msg);
 }
+ffi::Error InitializeDecodeOperators() {
+  char msg[512];
+  return FromCode(b200sd_init_decode_operators(msg, sizeof(msg)), msg);
+}
 ffi::Error ScaledDotF8Execute(cudaStream_t stream, ffi::RemainingArgs operands, ffi::RemainingRets results,
                               ffi::Dictionary attrs) {
   B200SD_ScaledDotF8 a;
@@ -679,7 +683,7 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_s8, DotS8Execute,
 
 XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4_instantiate, DotW4Instantiate,
                               ffi::Ffi::BindInstantiate().RemainingArgs().RemainingRets().Attrs());
-XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4_initialize, InitializeDevice, ffi::Ffi::BindInitialize());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4_initialize, InitializeDecodeOperators, ffi::Ffi::BindInitialize());
 XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_dot_w4, DotW4Execute,
                               ffi::Ffi::Bind()
                                   .Ctx<ffi::PlatformStream<cudaStream_t>>()
@@ -701,7 +705,7 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_kv_cache_append, KvCacheAppendExecute,
 
 XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention_instantiate, PagedAttentionInstantiate,
                               ffi::Ffi::BindInstantiate().RemainingArgs().RemainingRets().Attrs());
-XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention_initialize, InitializeDevice, ffi::Ffi::BindInitialize());
+XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention_initialize, InitializeDecodeOperators, ffi::Ffi::BindInitialize());
 XLA_FFI_DEFINE_HANDLER_SYMBOL(b200sd_ffi_paged_attention, PagedAttentionExecute,
                               ffi::Ffi::Bind()
                                   .Ctx<ffi::PlatformStream<cudaStream_t>>()

@@ -160,6 +160,7 @@ struct LaunchStats {
 // One-time per-device set-up (function attributes, SM count).  Not a stream operation; must not
 // be called for the first time while the stream is being captured.
 Status InitDevice(int device);
+Status InitDecodeOperators(int device);
 
 // `variant`: kKernelDense picks between the CTA-pair and the single-CTA instantiation.
 Status LaunchDense(const GemmProblem& p, cudaStream_t stream, LaunchStats* stats, int variant = kKernelDense);

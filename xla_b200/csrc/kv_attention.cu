@@ -38,6 +38,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "kv_cache.cuh"
 
@@ -872,7 +873,7 @@ constexpr int kShapes = 5;
 #define B200SD_ATTENTION_VARIANTS(code) MakeVariant<code, 64, 1>(), MakeVariant<code, 64, 2>(), MakeVariant<code, 128, 1>(), MakeVariant<code, 128, 2>(), MakeVariant<code, 256, 1>()
 const Variant kVariants[3][kShapes] = {{B200SD_ATTENTION_VARIANTS(kF8E4M3FN)}, {B200SD_ATTENTION_VARIANTS(kF8E5M2)}, {B200SD_ATTENTION_VARIANTS(kS8)}};
 #undef B200SD_ATTENTION_VARIANTS
-int g_ctas_per_sm[3][kShapes];                  // the same on every B200; set by InitAttentionKernels
+int g_ctas_per_sm[3][kShapes];                  // the same on every B200; written once, by the first InitAttentionKernels
 
 int ShapeIndex(int64_t head_dim, int64_t rows) {
   if (head_dim > 128) return 4;
@@ -882,6 +883,7 @@ int ShapeIndex(int64_t head_dim, int64_t rows) {
 }  // namespace
 
 Status InitAttentionKernels() {
+  int ctas[3][kShapes];
   for (int c = 0; c < 3; ++c)
     for (int s = 0; s < kShapes; ++s) {
       const Variant& v = kVariants[c][s];
@@ -892,8 +894,10 @@ Status InitAttentionKernels() {
       if (e == cudaSuccess) e = cudaFuncSetAttribute(v.join, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
       if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, v.main, kThreads, v.bytes);
       if (e != cudaSuccess) return Status::Error(kInternal, std::string("kv_attention_kernel set-up: ") + cudaGetErrorString(e));
-      g_ctas_per_sm[c][s] = n > 0 ? n : 1;
+      ctas[c][s] = n > 0 ? n : 1;
     }
+  static std::once_flag once;                   // another device may be launching already
+  std::call_once(once, [&] { std::copy(&ctas[0][0], &ctas[0][0] + 3 * kShapes, &g_ctas_per_sm[0][0]); });
   return Status::Ok();
 }
 

@@ -29,6 +29,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -760,13 +761,19 @@ Variants& TheVariants() {
 Status InitW4Kernels() {
   static_assert(std::is_standard_layout_v<Variants>);
   Variant* v = reinterpret_cast<Variant*>(&TheVariants());
-  for (size_t i = 0; i < sizeof(Variants) / sizeof(Variant); ++i) {
+  constexpr size_t kCount = sizeof(Variants) / sizeof(Variant);
+  int registers[kCount];
+  for (size_t i = 0; i < kCount; ++i) {
     cudaFuncAttributes attr{};
     cudaError_t e = cudaFuncSetAttribute(v[i].kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerCta);
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, v[i].kernel);
     if (e != cudaSuccess) return Status::Error(kInternal, std::string("w4_dot_kernel set-up: ") + cudaGetErrorString(e));
-    v[i].registers = attr.numRegs;
+    registers[i] = attr.numRegs;
   }
+  static std::once_flag once;                               // the same on every device; another one may be launching already
+  std::call_once(once, [&] {
+    for (size_t i = 0; i < kCount; ++i) v[i].registers = registers[i];
+  });
   return Status::Ok();
 }
 
