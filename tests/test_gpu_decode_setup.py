@@ -1,4 +1,4 @@
-"""The device set-up of the decode-step operators, each case in a process that has done nothing else."""
+"""The device set-up of the decode-step operators and the end of their waits, each case in a process of its own."""
 import os
 import subprocess
 import sys
@@ -71,3 +71,38 @@ assert torch.equal(y, xla_b200.dot_w4(x, w, scale, out_dtype=torch.float32))
 assert torch.equal(out, xla_b200.paged_attention_kv8(q, *cache, table, lens)) and bool((out != 0).any())
 assert xla_b200.device_status() == 0
 """)
+
+
+def test_a_copy_that_does_not_come():
+    """Its wait expires (20 ms in this build), the call ends and reports it, and the next one is right."""
+    _run("""
+import os
+import sys
+sys.path.insert(0, "tests")
+import decode_reference as ref
+g = torch.Generator().manual_seed(0)
+
+def expires(call):
+    os.environ["B200SD_LOSE_COPY"] = "1"
+    call()
+    del os.environ["B200SD_LOSE_COPY"]
+    status = xla_b200.device_status()
+    assert status == 128, status
+    return call()
+
+for m, n, k in ((8, 3000, 8192), (20, 100000, 640), (3, 40, 128), (64, 200, 1024)):
+    x = torch.randn((m, k), generator=g).to(torch.bfloat16).to(dev)
+    w = torch.randint(0, 256, (n, k // 2), generator=g).to(torch.uint8).to(dev)
+    scale = torch.rand((n, k // 128), generator=g).to(dev)
+    out = expires(lambda: xla_b200.dot_w4(x, w, scale, out_dtype=torch.float32))
+    want, size = ref.dot(x, w, scale)
+    assert bool(((out.double() - want).abs() <= (k + 4) * 2.0 ** -23 * size).all())
+for heads, kv_heads, dim, lens in ((8, 2, 128, [9000, 40]), (32, 1, 64, [100, 300, 2]), (4, 2, 256, [5000])):
+    pages = sum(-(-n // 16) for n in lens) + 1
+    args = [torch.randn((len(lens), 1, heads, dim), generator=g).to(torch.bfloat16).to(dev), *ref.make_cache(pages, kv_heads, 16, dim, ref.E4M3, dev),
+            ref.make_table(lens, 16, pages, dev), torch.tensor(lens, dtype=torch.int32, device=dev)]
+    want = xla_b200.paged_attention_kv8(*args)
+    assert xla_b200.device_status() == 0
+    assert torch.equal(expires(lambda: xla_b200.paged_attention_kv8(*args)), want)
+assert xla_b200.device_status() == 0
+""", B200SD_LIBRARY=os.path.join(ROOT, "xla_b200", "lib", "libb200_scaled_dot_tuning.so"))

@@ -37,6 +37,11 @@ inline int TuningEnvInt(const char* name, int dflt) {
 #endif
 }
 
+// Of the decode-step operators: B200SD_LOSE_COPY=1 in a tuning build leaves out the first copy of a call that is waited for, and
+// waits 20 ms for it, so that the way out of an expired wait can be tested.
+inline int LoseCopy() { return TuningEnvInt("B200SD_LOSE_COPY", 0); }
+constexpr uint64_t kLostCopyNs = 20'000'000;
+
 // xla::PrimitiveType numbers (mirrored by XLA_FFI_DataType, xla/ffi/api/c_api.h:233-266).
 enum PrimitiveType : int32_t {
   kInvalidType = 0,

@@ -73,6 +73,7 @@ struct AttentionArgs {
   int32_t min_units;                            // a CTA's share is not smaller
   float scale;                                  // softmax_scale * log2(e)
   int32_t is_bf16;
+  int32_t lose;                                 // LoseCopy()
   uint32_t* status;
 };
 
@@ -406,7 +407,8 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     int32_t pages[kPair];
 #pragma unroll
     for (int i = 0; i < kPair; ++i) pages[i] = __shfl_sync(0xffffffffu, page_of, batch_at + i);
-    if (lane == 0) {
+    const bool lost = kTiming && a.lose && share.begin == 0 && warp == 0 && load_pos == ahead.Begin(a) && ahead.left == share.left;
+    if (lane == 0 && !lost) {
       int tiles = 0;
 #pragma unroll
       for (int i = 0; i < kPair; ++i) tiles += pages[i] >= 0 ? 1 : 0;
@@ -496,7 +498,12 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
     for (int32_t pos = begin + warp * (kTile * kPair); pos < end; pos += kStep) {
       flush();
       const uint8_t* tiles = ring + stage * kStageBytes;
-      (void)mbar_wait(&full[stage], parity, &abort_flag, a.status, kStatusTileTimeout);
+      const uint64_t limit = kTiming && a.lose ? kLostCopyNs : kWaitLimitNs;
+      if (!mbar_wait_warp(&full[stage], parity, &abort_flag, a.status, kStatusTileTimeout, limit)) {      // this warp leaves, and what the CTA writes is not the result
+        const int ahead_by = load_stage - stage;
+        await_copies(full, kStages, stage, parity, ahead_by > 0 ? ahead_by : ahead_by + kStages, a.status, kStatusTileTimeout, limit);
+        return;
+      }
       __syncwarp();
       float4 num[kPair];
 #pragma unroll
@@ -962,7 +969,7 @@ Status LaunchPagedAttention(const B200SD_PagedAttention& a, cudaStream_t stream,
                      static_cast<int32_t>(a.batch), static_cast<int32_t>(a.new_tokens), static_cast<int32_t>(a.heads), static_cast<int32_t>(a.kv_heads),
                      static_cast<int32_t>(a.head_dim), shift, static_cast<int32_t>(rows), static_cast<int32_t>(blocks),
                      static_cast<int32_t>(a.num_pages), static_cast<int32_t>(a.table_width), static_cast<int32_t>(window),
-                     unit_shift, extra, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, StatusWordPtr()};
+                     unit_shift, extra, cut ? 2 : 1, a.softmax_scale * 1.4426950408889634f, a.q_dtype == kBF16, LoseCopy(), StatusWordPtr()};
   CUtensorMap key_map, value_map;
   const bool none = a.num_pages == 0;                                 // then no page is valid, and no tile is loaded
   const int64_t matrices = none ? 1 : a.num_pages * a.kv_heads;

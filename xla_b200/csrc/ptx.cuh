@@ -98,6 +98,38 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same by a whole warp together, which gets one answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status,
+                                               uint32_t status_bit, uint64_t limit_ns = kWaitLimitNs) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  uint64_t t0 = 0;
+  uint32_t polls = 0;
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((++polls & 4095u) == 0) {
+      const bool aborted = *abort_flag != 0;
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      if (__any_sync(0xffffffffu, aborted || now - t0 > limit_ns)) {
+        *abort_flag = 1;
+        if (!aborted) atomicOr(status, status_bit);
+        return false;
+      }
+    }
+  }
+}
+
+// What a warp does that gave up waiting: the copies that it has sent for have to land before the memory that they go to is
+// another CTA's.  `count` waits from barrier `at` of a ring of `size`, `parity` that of the first; limited as a whole.
+static __device__ __noinline__ void await_copies(uint64_t* bars, int size, int at, uint32_t parity, int count, uint32_t* status,
+                                                 uint32_t status_bit, uint64_t limit_ns) {
+  int gave_up = 0;
+  for (int i = 0; i < count; ++i) {
+    (void)mbar_wait(&bars[at], parity, &gave_up, status, status_bit, limit_ns);
+    if (++at == size) at = 0, parity ^= 1;
+  }
+}
+
 // ----------------------------------------------------------------------------- flags between ranks
 // Counters in global memory that another GPU (or another CTA) increments after it has written
 // data for us: release-add on the writer's side, acquire-load on ours, both at system scope.

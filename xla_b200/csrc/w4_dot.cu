@@ -54,6 +54,7 @@ struct W4Args {
   uint32_t* status;
   uint32_t piece_inverse;                       // 2^32 / (16 * steps), rounded up
   int32_t x_is_bf16, scale_dtype, bias_dtype, d_dtype, is_signed;
+  int32_t lose;                                 // LoseCopy()
 };
 
 // Scales and bias: their bits, loaded ahead, and what they stand for.  kType 0 takes the type from the arguments.
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
   const int steps = a.steps, row_bytes = a.k / 2, phase_steps = a.per_round, phases = (steps + phase_steps - 1) / phase_steps;
   uint8_t* ring = smem + warp * kStages * 2048;
   uint64_t* arrived = reinterpret_cast<uint64_t*>(smem + S::kRing);          // of the two halves of the buffer of x
-  int* abort_flag = reinterpret_cast<int*>(arrived + 2);
+  volatile int* abort_flag = reinterpret_cast<int*>(arrived + 2);
   uint8_t* x_buffer = smem + S::kRing + 64;
   float* sums = reinterpret_cast<float*>(x_buffer);                          // at the end
   const int x_pitch = phase_steps * 256 + 16;               // bytes between two rows of x in a phase: neighbours not in the same banks
@@ -524,11 +525,24 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
   __syncthreads();
   griddep_wait();
 
+  uint32_t x_parity = 0;                                    // bit h: parity of the next wait for half h
+  const uint64_t limit = kTiming && a.lose ? kLostCopyNs : kWaitLimitNs;
+  // After an expired wait, in front of phase `next`'s: the copies of the phase before it and of its own are waited for, once.
+  auto land = [&](int next) {
+    const int late = (next - 1) & 1;
+    await_copies(arrived, 2, late, (x_parity >> late & 1) ^ 1, 1, a.status, kStatusTileTimeout, limit);
+    if (next < phases) await_copies(arrived, 2, next & 1, x_parity >> (next & 1) & 1, 1, a.status, kStatusTileTimeout, limit);
+    *abort_flag = 2;
+  };
   auto load_x = [&](int phase) {                            // one copy per row, by the first warp; and zeros behind the end of k
     if (phase >= phases) return;
+    if (warp == 0 && *abort_flag) {                         // nothing is sent for any more, the last barrier may never complete
+      if (lane == 0 && *abort_flag == 1) land(phase - 1);
+      return;
+    }
     uint8_t* to = x_buffer + (phase & 1) * (a.m * x_pitch);
     const int begin = phase * phase_steps * 128, end = min(a.k, begin + phase_steps * 128), bytes = (end - begin) * 2;
-    if (warp == 0) {
+    if (warp == 0 && !(kTiming && a.lose && blockIdx.x == 0 && phase == 0)) {
       if (lane == 0) mbar_arrive_expect_tx(&arrived[phase & 1], a.m * bytes);
       __syncwarp();
       if (lane < a.m)
@@ -539,7 +553,6 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
     for (int i = threadIdx.x; i < a.m * missing; i += kWarps * 32)
       *reinterpret_cast<uint4*>(to + i / missing * x_pitch + bytes + i % missing * 16) = make_uint4(0, 0, 0, 0);
   };
-  uint32_t x_parity = 0;                                    // bit h: parity of the next wait for half h
   uint32_t row_offset[kCols];                               // of this lane's rows of x; behind the last one any will do
 #pragma unroll
   for (int c = 0; c < kCols; ++c) row_offset[c] = min(c * 8 + g, a.m - 1) * x_pitch;
@@ -602,7 +615,7 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
     for (int phase = 0; phase < phases; ++phase) {
       __syncthreads();                                      // the phase before has been read by all warps
       load_x(phase + 1);
-      (void)mbar_wait(&arrived[phase & 1], (x_parity >> (phase & 1)) & 1, abort_flag, a.status, kStatusTileTimeout);
+      (void)mbar_wait(&arrived[phase & 1], (x_parity >> (phase & 1)) & 1, abort_flag, a.status, kStatusTileTimeout, limit);
       x_parity ^= 1u << (phase & 1);
       const uint32_t x_at = smem_u32(x_buffer) + (phase & 1) * (a.m * x_pitch) + t * (kGroup == 128 ? 64 : kGroup == 64 ? 32 : 16);
       const int end = min(steps, (phase + 1) * phase_steps);
@@ -676,6 +689,11 @@ __global__ void __launch_bounds__(S::kWarps * 32) w4_dot_wide_kernel(const __gri
       else if (works) run(Two());
     }
     __syncthreads();                                        // x has been read: its place takes the sums
+    if (*abort_flag) {                                      // a wait expired: no result
+      if (threadIdx.x == 0 && *abort_flag == 1) land(phases);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      return;
+    }
     if (works) {
       float* mine = sums + warp * a.m * kSumStride;
 #pragma unroll
@@ -849,7 +867,7 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
                     static_cast<int32_t>(a.m), static_cast<int32_t>(a.n), static_cast<int32_t>(a.k), static_cast<int32_t>(a.k / a.group),
                     group_shift, static_cast<int32_t>(blocks_per_group),
                     static_cast<int32_t>(a.n / ctas), static_cast<int32_t>(a.n % ctas), static_cast<int32_t>(steps), static_cast<int32_t>(v.per_round(a.m, steps)), StatusWordPtr(),
-                    0xffffffffu / static_cast<uint32_t>(steps * 16) + 1, a.x_dtype == kBF16, a.scale_dtype, a.bias_dtype, a.d_dtype, a.weight_type == kS4};
+                    0xffffffffu / static_cast<uint32_t>(steps * 16) + 1, a.x_dtype == kBF16, a.scale_dtype, a.bias_dtype, a.d_dtype, a.weight_type == kS4, LoseCopy()};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;     // see griddep_wait() in the kernel
   attr.val.programmaticStreamSerializationAllowed = 1;
