@@ -775,26 +775,23 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const __grid_con
 }
 
 // Joins the pieces of the item that the end of CTA blockIdx.x's share cuts first: maximum over the pieces, then the
-// pieces' sums and values times exp2(their maximum - it), in the order of the pieces.
-
-// Small blocks of 8 rows come in as soon as one block of the first kernel has left, and send for more pieces at once (32
-// sequences of 0 to 4096 tokens: 33.7 us; with 512 threads and 4 pieces 34.1, with 256 and 4 34.4).
+// pieces' sums and values times exp2(their maximum - it), in the order of the pieces.  A warp has a row, and sends for 8
+// pieces at once, or 4 where a block has 16 rows.  (Blocks of 8 rows come in as soon as one block of the first kernel has left; 32
+// sequences of 0 to 4096 tokens 33.7 us, with 4 pieces at once 34.4, and with two warps for a row and 4 pieces each 34.1.)
 template <int kRowTiles>
-constexpr int kJoinThreads = kRowTiles == 1 ? 256 : 512;
+constexpr int kJoinThreads = 256 * kRowTiles;
 
 template <int kDim, int kRowTiles>
 __global__ void __launch_bounds__(kJoinThreads<kRowTiles>) kv_attention_join_kernel(const AttentionArgs a) {
   using L = Layout<kDim, kRowTiles>;
-  constexpr int kParts = kJoinThreads<kRowTiles> / 32 / L::kRows;      // warps of a row
+  static_assert(kJoinThreads<kRowTiles> == 32 * L::kRows);
   constexpr int kVectors = kDim == 256 ? 2 : 1;             // of four columns, per lane
-  __shared__ float4 part_values[kParts][L::kRows][kDim / 4];
-  __shared__ float part_sum[kParts][L::kRows];
-  const int c = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = warp % L::kRows, part = warp / L::kRows;
+  const int c = blockIdx.x, row = threadIdx.x / 32, lane = threadIdx.x % 32;
   griddep_wait();
   if (threadIdx.x == 0) griddep_launch_dependents();
   const int4 cut = a.cut[c];
-  const int pieces = cut.z;
-  if (pieces == 0) return;
+  const int pieces = cut.z, item_row = (cut.y % a.blocks) * L::kRows + row;
+  if (pieces == 0 || item_row >= a.rows) return;
   auto slot_of = [&](int p) { return a.work + (static_cast<int64_t>(c + p) * 2 + (p == 0 ? 1 : 0)) * L::kSlot; };
   // A few pieces are sent for at once; their maximum is known when they come.
   constexpr int kAtOnce = kRowTiles == 1 ? 8 : 4;
@@ -802,17 +799,16 @@ __global__ void __launch_bounds__(kJoinThreads<kRowTiles>) kv_attention_join_ker
   float first_max[kAtOnce], first_sum[kAtOnce];
   float4 first_values[kAtOnce][kVectors];
 #pragma unroll
-  for (int j = 0; j < kAtOnce; ++j) {
-    const int p = part + j * kParts;
-    first_max[j] = -INFINITY, first_sum[j] = 0.0f;
+  for (int p = 0; p < kAtOnce; ++p) {
+    first_max[p] = -INFINITY, first_sum[p] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) first_values[j][i] = make_float4(0, 0, 0, 0);
+    for (int i = 0; i < kVectors; ++i) first_values[p][i] = make_float4(0, 0, 0, 0);
     if (p < pieces) {
       const float* slot = slot_of(p);
-      first_max[j] = slot[L::kRows * kDim + row], first_sum[j] = slot[L::kRows * kDim + L::kRows + row];
+      first_max[p] = slot[L::kRows * kDim + row], first_sum[p] = slot[L::kRows * kDim + L::kRows + row];
 #pragma unroll
       for (int i = 0; i < kVectors; ++i)
-        if (mine) first_values[j][i] = *reinterpret_cast<const float4*>(slot + row * kDim + i * 128 + lane * 4);
+        if (mine) first_values[p][i] = *reinterpret_cast<const float4*>(slot + row * kDim + i * 128 + lane * 4);
     }
   }
   float m = -INFINITY;
@@ -828,9 +824,9 @@ __global__ void __launch_bounds__(kJoinThreads<kRowTiles>) kv_attention_join_ker
     for (int i = 0; i < kVectors; ++i) y[i].x = fmaf(v[i].x, fade, y[i].x), y[i].y = fmaf(v[i].y, fade, y[i].y), y[i].z = fmaf(v[i].z, fade, y[i].z), y[i].w = fmaf(v[i].w, fade, y[i].w);
   };
 #pragma unroll
-  for (int j = 0; j < kAtOnce; ++j) add(first_max[j], first_sum[j], first_values[j]);
+  for (int p = 0; p < kAtOnce; ++p) add(first_max[p], first_sum[p], first_values[p]);
 #pragma unroll 8
-  for (int p = part + kAtOnce * kParts; p < pieces; p += kParts) {
+  for (int p = kAtOnce; p < pieces; ++p) {
     const float* slot = slot_of(p);
     const float piece_max = slot[L::kRows * kDim + row], piece_sum = slot[L::kRows * kDim + L::kRows + row];
     float4 v[kVectors] = {};
@@ -838,24 +834,6 @@ __global__ void __launch_bounds__(kJoinThreads<kRowTiles>) kv_attention_join_ker
     for (int i = 0; i < kVectors; ++i)
       if (mine) v[i] = *reinterpret_cast<const float4*>(slot + row * kDim + i * 128 + lane * 4);
     add(piece_max, piece_sum, v);
-  }
-  if (part > 0) {
-    if (lane == 0) part_sum[part][row] = total;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (mine) part_values[part][row][i * 32 + lane] = y[i];
-  }
-  __syncthreads();
-  const int item_row = (cut.y % a.blocks) * L::kRows + row;
-  if (part > 0 || item_row >= a.rows) return;
-  for (int p = 1; p < kParts; ++p) {
-    total += part_sum[p][row];
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (mine) {
-        const float4 v = part_values[p][row][i * 32 + lane];
-        y[i].x += v.x, y[i].y += v.y, y[i].z += v.z, y[i].w += v.w;
-      }
   }
 #pragma unroll
   for (int i = 0; i < kVectors; ++i)
