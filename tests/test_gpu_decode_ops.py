@@ -424,6 +424,22 @@ def test_attention_of_long_and_short_sequences_together(cuda_device):
     _check_attention(_attention_inputs(cuda_device, 2, 1, 256, 128, [6000, 1], 1, E4M3, BF16))
 
 
+@pytest.mark.parametrize("lens,kv_heads", [([131072] + [0] * 15, 1), ([5, 0, 131072, 40], 1), ([131072], 1), ([0] * 63 + [100000], 2), ([131072, 131072], 1)])
+def test_attention_cuts_a_sequence_into_a_limited_number_of_pieces(cuda_device, lens, kv_heads):
+    """Idle and short sequences beside a long one do not add to its pieces, which one warp joins for each row.
+
+    Each CTA leaves word of the item that the end of its share cuts, (sequence, item, pieces, new tokens), at the workspace's
+    end.  A share is no smaller than the largest item over 128, to the nearest unit and two at least: 320 units in shares of
+    two and a half, or 319 in shares of two, are 160 pieces at most, and the item's ends may lie inside of shares."""
+    args = _attention_inputs(cuda_device, 4 * kv_heads, kv_heads, 128, 64, lens, 1, E4M3, BF16)
+    fresh = torch.tensor([min(n, 1) for n in lens], dtype=torch.int32, device=cuda_device)
+    work = torch.zeros(xla_b200.paged_attention_workspace_bytes(len(lens), 1, 4 * kv_heads, kv_heads, 128), dtype=torch.int8, device=cuda_device)
+    out = xla_b200.paged_attention_kv8(*args, new_lens=fresh, workspace=work, return_lse=True)
+    pieces = work[-148 * 5 * 16:].view(torch.int32).reshape(-1, 4)[:, 2]
+    assert 64 <= int(pieces.max()) <= 162, int(pieces.max())
+    _check_attention(args, fresh.tolist(), out=out)
+
+
 def test_attention_of_many_sequences(cuda_device):
     """More sequences than a warp has lanes, their work in shares that begin and end anywhere."""
     for heads, kv_heads, dim, new, code in ((8, 2, 64, 1, E4M3), (16, 1, 128, 2, S8), (2, 2, 256, 1, E5M2)):
