@@ -413,6 +413,27 @@ def test_attention(cuda_device, heads, kv_heads, dim, page, lens, new, code, dty
     assert _status() == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page,lens,new,code", [
+    (8, 2, 64, 16, [37, 500], 1, E4M3),
+    (6, 1, 256, 16, [1000, 47], 1, E4M3),
+    (16, 1, 128, 32, [300, 90], 3, S8),
+    (5, 1, 96, 64, [9000], 1, E5M2),
+    (32, 2, 64, 128, [2000, 77], 1, S8),
+    (40, 4, 128, 32, [5000, 5], 5, S8),
+])
+def test_attention_of_f16_is_rounded_once(cuda_device, heads, kv_heads, dim, page, lens, new, code):
+    """The weights of f16 results are no coarser than the sums: only the last rounding is one to 11 bits.
+
+    The bound is _attention_tolerance's without the weights' 2^-11: each weight is held to 2^-22, below its 2^-18."""
+    args = _attention_inputs(cuda_device, heads, kv_heads, dim, page, lens, new, code, F16, seed=dim)
+    want, _, size, slack = ref.attention(*args)
+    off = (xla_b200.paged_attention_kv8(*args).double() - want).abs()
+    tolerance = size * (2 * slack[..., None] + 2.0 ** -18) + HALF_STEP[F16] * (1 + 2.0 ** -7) * want.abs() + 2.0 ** -25
+    assert bool((off <= tolerance).all()), float((off / tolerance).max())
+    nearest = want.to(F16).double() - want                   # what the last rounding alone leaves
+    assert float(off.norm()) <= 1.01 * float(nearest.norm())
+
+
 def test_attention_of_long_and_short_sequences_together(cuda_device):
     """One sequence far longer than the others: its work is split over the card and joined."""
     for dtype, new in ((BF16, 1), (F16, 2)):
