@@ -199,6 +199,26 @@ def test_dot_w4_outliers_of_x_where_the_weight_is_its_zero_point(cuda_device, m,
     assert _status() == 0
 
 
+@pytest.mark.parametrize("n,k,group,dtype,zeros", [
+    (5488, 608, 32, F16, False),
+    (1000, 2048, 32, F16, True),
+    (5488, 608, 32, BF16, True),
+    (50000, 4096, 128, F16, True),
+    (50000, 4096, 64, BF16, False),
+])
+@pytest.mark.parametrize("m", [1, 3])
+def test_dot_w4_sums_keep_the_bits_of_f32(cuda_device, m, n, k, group, dtype, zeros):
+    """One large value of x and its products, of at most 11 + 5 bits, in the same sums as all the others.
+
+    At most 64 additions follow one another: a warp's products (8 for 128 of k, every 16th or 24th step), its groups, and the
+    sums of up to 24 warps; each is off by at most a step of 2^-23 of a sum that is no larger than about the result."""
+    x, w, scale, zero, _ = inputs = _dot_inputs(cuda_device, m, n, k, group, dtype, zeros, False, F32, seed=n + k)
+    x[:, k // 3] = 7720.0
+    out = xla_b200.dot_w4(x, w, scale, zero=zero, out_dtype=F32)
+    want, _ = ref.dot(*inputs)
+    assert float((out.double() - want).norm() / want.norm()) <= 8 * 2.0 ** -23
+
+
 def test_dot_w4_many_rows_one_value_at_a_time(cuda_device):
     """Powers of two at one place of k: exact, for every nibble and zero point."""
     n, k = 4800, 4096

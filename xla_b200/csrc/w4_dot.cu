@@ -12,15 +12,15 @@
 // A CTA owns n / CTAs consecutive rows, whole rows of bytes with none read twice or by two CTAs whatever n is.  A block of
 // 32 of its rows and 128 of k are a unit, which a warp brings in through its own cp.async ring.
 //
-// The wide kernel takes x as it is, in phases that the warps of a CTA share.  A masked nibble plus an offset is an f16 or
-// bf16 number (1024 + n, 128 + n), and one subtraction leaves w - z, exactly; 9 and 11 instructions for 8 weights.
-// The other one, for one or two rows against many weights, first puts all of x into shared memory, paired, as f16 whatever
-// its type: f16 as it is, a bf16 row multiplied by the power of two that brings its largest finite value to 2^15 (what lies
-// 2^32 below that is rounded, to 2^-40 of it).  A nibble under a mask then is an f16 number as it stands, the subnormal n *
-// 2^-24, or 16 n * 2^-24 for the nibbles one place higher, and one subtraction leaves (w - z) 2^-24, exactly: 9 instructions
-// for 8 weights of either type of x.  (The nibbles themselves as operands are 5, but then the zero points come off a
-// group's sum, as z times the sum of x: where w = z at an outlier of x, the sum before is many times the one after, and what
-// it loses below the outlier's last bit is larger than f32 sums of the definition's terms lose.)
+// A masked nibble plus an offset is an f16 or bf16 number (1024 + n, 128 + n), and one subtraction leaves w - z, exactly: 9
+// instructions for 8 weights in f16, 11 in bf16.  The wide kernel takes x as it is, in phases that the warps of a CTA share.
+// The other one, for one or two rows, first puts all of x into shared memory, paired, as f16 whatever its type: f16 as it is, a
+// bf16 row multiplied by the power of two that brings its largest finite value to 2^15 (what lies 2^32 below that is rounded,
+// to 2^-40 of it).
+// (Cheaper operands were tried and lost bits.  The nibbles as they stand under a mask, 16-bit subnormals, are 5 instructions, but
+// the zero points then come off a group's sum as z times the sum of x: at an outlier of x whose weight is z, the sum before is
+// many times the one after.  And products of subnormals are lined up for the sum by the exponent that they would have if they
+// were normal, so that 10 of the 24 bits of an f32 sum are zeros.)
 //
 // Measured with cold caches: 28672 x 8192 in groups of 128 for one row 34 us (3.6 TB/s; the bytes alone take 18.5), 8192 x
 // 28672 with zero points for 16 rows 58.6 us, 5003 x 4416 in groups of 32 for 5 rows 10.7 us, 1024 x 2048 for one row 7.6
@@ -105,18 +105,8 @@ __device__ __forceinline__ uint32_t MaskXor(uint32_t w, uint32_t mask, uint32_t 
   return v;
 }
 
-// How a word's nibbles become operands; `flip` (8 for two's complement) turns -8 .. 7 into 0 .. 15 with zero point 8.
-// As (w - z) 2^-24, see above; the offset -z 2^-24 has z in its low bits.
-__device__ __forceinline__ uint32_t SubnormalOffset(uint32_t z) { return 0x80008000u | z * 0x00010001u; }
-__device__ __forceinline__ void DecodeSubnormal(uint32_t w, uint32_t flip, uint32_t offset, uint32_t (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t a = MaskXor(w >> (8 * i), 0x000f000fu, flip), b = MaskXor(w >> (8 * i), 0x00f000f0u, flip << 4);
-    asm("add.f16x2 %0, %1, %2;" : "=r"(v[2 * i]) : "r"(a), "r"(offset));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[2 * i + 1]) : "r"(b), "r"(0x2c002c00u), "r"(offset));              // times 1 / 16
-  }
-}
-// As w - z, exactly.  The offsets -(1024 + z), -(64 + z) and -(128 + z) of one weight row and group have z in their low bits,
+// How a word's nibbles become operands, w - z, exactly; `flip` (8 for two's complement) turns -8 .. 7 into 0 .. 15 with zero point 8.
+// The offsets -(1024 + z), -(64 + z) and -(128 + z) of one weight row and group have z in their low bits,
 // so they are put together, not converted.
 template <typename T> struct Offset;
 template <> struct Offset<__half> {
@@ -181,8 +171,8 @@ __device__ __forceinline__ float2 Unpack(uint32_t w, bool is_bf16) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// All of x to shared memory, `inputs`: paired, as f16, scaled if it was bf16; `factors` [row][2] what brings a row's sums back,
-// as two powers of two between which nothing overflows.  The copies are under way before the weights', so that they do not
+// All of x to shared memory, `inputs`: paired, as f16, scaled if it was bf16; `factors` [row] what brings a row's sums
+// back.  The copies are under way before the weights', so that they do not
 // queue behind them; a thread works on the pieces that it has copied itself, in place.  The loops are not unrolled: this
 // code runs once, and its instructions are fetched cold.
 template <int kGroup, int kThreads>
@@ -244,11 +234,7 @@ struct Staging {
         v = make_uint4(scaled(v.x), scaled(v.y), scaled(v.z), scaled(v.w));
       }
       StoreShared16(at, Paired(v));
-      if (c == 0) {
-        const int back = 24 - power, half = back / 2;
-        factors[2 * r] = __uint_as_float(static_cast<uint32_t>(127 + half) << 23);
-        factors[2 * r + 1] = __uint_as_float(static_cast<uint32_t>(127 + back - half) << 23);
-      }
+      if (c == 0) factors[r] = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
     }
     __syncthreads();
   }
@@ -258,17 +244,17 @@ struct Resident {
   static constexpr int kWarps = 24, kMost = 2;              // kMost: rows of x
   static constexpr int kBlocks = 8;                         // whose sums have room, for one row of x
   static constexpr int kSums = kBlocks * kWarps * kSumStride;
-  // Each row's factors, its largest value, and what is behind them up to whole lines of banks.
-  static constexpr int kHead = (kSums * 4 + 3 * kMost * 4 + 127) / 128 * 128, kRing = kWarps * kStages * kStageBytes;
+  // Each row's factor, its largest value, and what is behind them up to whole lines of banks.
+  static constexpr int kHead = (kSums * 4 + 2 * kMost * 4 + 127) / 128 * 128, kRing = kWarps * kStages * kStageBytes;
   static int64_t PerRound(int64_t m, int64_t) { return kBlocks / m; }
   static int64_t Bytes(int64_t m, int64_t steps) { return kHead + kRing + steps * m * 256; }
 };
 
 // One or two rows of x, all of it in shared memory.  The warps take the units of the CTA in turn and leave their sums of
 // each block in shared memory, where they are added in the order of the warps, as many blocks at a time as have room.  Bound
-// by issue, about 300 instructions of a warp for a unit of 2 KiB, and by 8 us in front and behind: x, the first units, the
-// sums.  (With the nibbles as operands and zero points taken off the sums it was 250, and 28672 x 8192 for one row 32.5 us
-// instead of 33.8; of that form 24 warps took 33.4 and 16 took 36.4 us, before half blocks.)  kGroup: 32, 64 or 128
+// by issue, about 380 instructions of a warp for a unit of 2 KiB with all that surrounds it, and by 8 us in front and
+// behind: x, the first units, the sums.  (With the nibbles as operands 24 warps took 33.4 us for 28672 x 8192 and one row, and
+// 16 took 36.4.)  kGroup: 32, 64 or 128
 // (which stands for its multiples too).  kScale: the scales' type, kSigned: two's complement, no zero points.
 template <int kGroup, int kScale, bool kSigned>
 __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __grid_constant__ W4Args a) {
@@ -351,7 +337,7 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
       for (int h = 0; h < 2; ++h) row_at[r][h] = static_cast<uint32_t>(min(row + r * 16 + h * 8, most)) * a.groups;
   };
 
-  uint32_t* top = reinterpret_cast<uint32_t*>(factors + 2 * S::kMost);
+  uint32_t* top = reinterpret_cast<uint32_t*>(factors + S::kMost);
   if (threadIdx.x < S::kMost) top[threadIdx.x] = 0;
   __syncthreads();
   griddep_wait();
@@ -394,12 +380,11 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
           for (int group = 0; group < kPerStep; ++group) {
             const int holder = (lane & ~3) | group;           // the lane with this group's numbers
             float part[kTiles][4] = {};
-            uint32_t offset[kTiles][2];
+            Offset<__half> decoder[kTiles][2];
 #pragma unroll
             for (int r = 0; r < kOfUnit; ++r)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                offset[r][h] = SubnormalOffset(kSigned ? 8u : kGroup == 128 ? zero[r][h] : __shfl_sync(0xffffffffu, zero[r][h], holder));
+              for (int h = 0; h < 2; ++h) decoder[r][h].Set(kSigned ? 8u : kGroup == 128 ? zero[r][h] : __shfl_sync(0xffffffffu, zero[r][h], holder));
             // The words of this group, of rows g and g + 8 of each tile.
             uint32_t w[kTiles][2][kWords];
 #pragma unroll
@@ -423,8 +408,8 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
 #pragma unroll
               for (int r = 0; r < kOfUnit; ++r) {
                 uint32_t low[4], high[4];
-                DecodeSubnormal(w[r][0][i], flip, offset[r][0], low);
-                DecodeSubnormal(w[r][1][i], flip, offset[r][1], high);
+                decoder[r][0].Decode8(w[r][0][i], flip, low);
+                decoder[r][1].Decode8(w[r][1][i], flip, high);
                 Mma<__half>(part[r], low[0], high[0], low[1], high[1], b.x, b.y);
                 Mma<__half>(part[r], low[2], high[2], low[3], high[3], b.z, b.w);
               }
@@ -471,7 +456,7 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
         float y = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) y += part[w * a.m * kSumStride];
-        y = y * factors[2 * x_row] * factors[2 * x_row + 1] + bias;
+        y = y * factors[x_row] + bias;
         const int64_t place = static_cast<int64_t>(x_row) * a.n + at;
         if (a.d_dtype == kBF16) static_cast<__nv_bfloat16*>(a.d)[place] = __float2bfloat16_rn(y);
         else if (a.d_dtype == kF16) static_cast<__half*>(a.d)[place] = __float2half_rn(y);
@@ -840,14 +825,14 @@ Status LaunchDotW4(const B200SD_DotW4& a, cudaStream_t stream, LaunchStats* stat
   const Variant& resident = TheVariants().resident[group_at][scale_at][a.weight_type == kS4];
   // With x resident every CTA pairs all of it first, and has fewer instructions for the weights afterwards.  Which of the two
   // is faster, resident against wide in us, calls one after the other in a graph:
-  //   groups of 32: m 1, 256 x 512 2.9 and 3.2, 4096 x 4096 6.9 and 8.4, 28672 x 8192 39.2 and 54.7; m 2 the same 3.0 and
+  //   groups of 32: m 1, 256 x 512 2.9 and 3.2, 4096 x 4096 6.9 and 8.4, 28672 x 8192 39.3 and 55.0; m 2 the same 3.0 and
   //     3.2, 7.7 and 8.4, 41.9 and 55.0, but 65536 x 1024 20.8 and 18.3, 16384 x 1024 7.3 and 7.2: a short k does not pay for
   //     the second row.
   //   longer groups, two's complement (groups of 128): m 1, 8192 x 8192 15.6 and 13.5, 16384 x 8192 22.0 and 22.0, 36864 x 4608
-  //     25.5 and 25.1, 24576 x 8192 29.9 and 35.0, 28672 x 8192 33.8 and 38.7, 57344 x 8192 57.6 and 73.4; m 2, 16384 x 8192 24.4
+  //     25.5 and 25.1, 24576 x 8192 29.9 and 35.0, 28672 x 8192 33.5 and 38.6, 57344 x 8192 57.8 and 73.5; m 2, 16384 x 8192 24.4
   //     and 22.0, 24576 x 8192 33.0 and 35.0, 57344 x 8192 61.7 and 73.5, 131072 x 2048 45.5 and 41.7.
-  //   zero points, which cost this kernel more: m 1, 28672 x 6144 31.2 and 31.2, 24576 x 8192 35.7 and 37.0, 57344 x 8192 69.8 and
-  //     76.1; m 2, 24576 x 8192 39.0 and 37.1, 131072 x 4096 80.2 and 75.4.
+  //   zero points, which cost this kernel more: m 1, 28672 x 6144 31.2 and 31.2, 24576 x 8192 35.7 and 37.0, 57344 x 8192 70.0 and
+  //     76.5; m 2, 24576 x 8192 38.8 and 37.1, 131072 x 4096 80.8 and 74.2.
   // So groups of 32 have it unless k is short for two rows, and of the others many weights, about 200 million, with k long
   // enough for the warps of a CTA, two rows with zero points never.
   const bool pays = a.group == 32 ? a.m == 1 || a.k >= 2048
