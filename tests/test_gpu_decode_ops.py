@@ -581,6 +581,17 @@ def test_attention_reports_pages_outside_of_the_cache(cuda_device):
     assert _status() == 64 and _status() == 0
 
 
+@pytest.mark.parametrize("window", [1, 16, 100, 5000, 2 ** 30])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30 + 3, 4096 + 77, 4096 + 1])
+def test_attention_of_a_length_far_outside_of_the_table(cuda_device, length, window):
+    """What a window sees behind the table's end is not there, whatever the length, and the other sequences are as ever."""
+    for heads, dim, new, new_lens in ((4, 128, 3, [3, 3, 3, 3]), (2, 64, 1, [1, 0, 1, 1]), (4, 256, 2, [2, 2, 0, 1])):
+        args = _attention_inputs(cuda_device, heads, 2, dim, 64, [4096, 70, 4096, 0], new, E4M3, BF16)
+        args[6][0] = args[6][2] = length
+        _check_attention(args, new_lens, window)
+        assert _status() == 64 and _status() == 0
+
+
 def test_attention_over_a_cache_of_more_than_4_gib(cuda_device):
     pages, kv_heads, page, dim = 70000, 4, 128, 128        # 4.6 GB each for keys and values
     k, v = (torch.zeros((pages, kv_heads, page, dim), dtype=torch.uint8, device=cuda_device).view(E4M3) for _ in range(2))

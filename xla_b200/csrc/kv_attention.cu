@@ -84,7 +84,7 @@ struct AttentionArgs {
 struct Span {
   int32_t base;                                 // position of the first new token
   int32_t count;                                // new tokens
-  int32_t lo, hi;
+  int32_t lo, hi;                               // hi is at most 2^30
   int32_t units;
 };
 
@@ -95,7 +95,8 @@ __device__ __forceinline__ Span SpanOf(const AttentionArgs& a, int b) {
   s.base = max(len, 0) - s.count;               // below 0 for a length that does not hold the new tokens
   const int32_t capacity = a.table_width << a.page_shift;
   s.hi = s.count > 0 ? min(max(len, 0), capacity) : 0;
-  s.lo = a.window > 0 ? max(0, s.base + 1 - a.window) & ~(kTile - 1) : 0;
+  // The window of a length far outside of the table begins behind it; positions a CTA's step beyond `lo` stay 32-bit numbers.
+  s.lo = a.window > 0 ? min(max(0, s.base + 1 - a.window) & ~(kTile - 1), s.hi) : 0;
   s.units = max(1, a.extra + (s.hi > s.lo ? ((s.hi - s.lo - 1) >> a.unit_shift) + 1 : 0));      // an item without tokens still has rows to write
   return s;
 }
