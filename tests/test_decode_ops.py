@@ -195,11 +195,14 @@ def test_plain_attention_against_torch():
 def test_threads_on_one_call_site_get_their_own_messages(monkeypatch):
     """Both calls have failed before either reads its message."""
     both, got = threading.Barrier(2), {}
+    sites = {"first": _dot(zero=Buffer(U8, (48, 4))), "second": _dot(groups=3)}
+    wants = {"first": "got 4", "second": "k / group"}
+    execute = _native.mock.mockffi_call_execute
 
-    def failing(handle, stream, device, err, size):
-        err.value = threading.current_thread().name.encode()
+    def failing(handle, stream, device, *message):
+        rc = execute(sites[threading.current_thread().name]._h, stream, device, *message)
         both.wait(10)
-        return INVALID
+        return rc
 
     call = _dot()
     monkeypatch.setattr(_native.mock, "mockffi_call_execute", failing)
@@ -214,7 +217,7 @@ def test_threads_on_one_call_site_get_their_own_messages(monkeypatch):
         t.start()
     for t in threads:
         t.join()
-    assert "first" in got["first"] and "second" in got["second"], got
+    assert all(wants[name] in got[name] for name in wants), got
 
 
 def test_workspace_bytes_are_those_of_a_call_that_is_served():

@@ -204,6 +204,7 @@ mock.mockffi_call_attr_i64_array.argtypes = [C.c_void_p, C.c_char_p, C.POINTER(C
 mock.mockffi_call_invoke.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, *_ERR]
 mock.mockffi_call_run.argtypes = [C.c_void_p, C.c_void_p, C.c_int, *_ERR]
 mock.mockffi_call_execute.argtypes = [C.c_void_p, C.c_void_p, C.c_int, *_ERR]
+mock.mockffi_last_error.restype = C.c_char_p
 
 _registered = False
 

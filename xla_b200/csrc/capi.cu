@@ -110,10 +110,11 @@ Status InitDevice(int device) {
 // Beyond that, what the operators of a decode step need.  On its own, so that a scaled dot neither waits for their kernels
 // to be loaded nor fails where they cannot be.
 Status InitDecodeOperators(int device) {
-  Status base = InitDevice(device);
-  if (!base.ok()) return base;
+  if (device < 0 || device >= 64) return Status::Error(kInvalidArgument, "device ordinal out of range");
   DeviceState& st = g_state[device];
   std::call_once(st.decode_once, [&] {
+    st.decode_status = InitDevice(device);
+    if (!st.decode_status.ok()) return;
     st.decode_status = InitAttentionKernels();
     if (st.decode_status.ok()) st.decode_status = InitW4Kernels();
     if (TuningEnvInt("B200SD_FAIL_DECODE_SETUP", 0)) st.decode_status = Status::Error(kInternal, "set-up of the decode-step operators made to fail");

@@ -282,12 +282,15 @@ void Build(Call& c, bool null_data, XLA_FFI_InvokeContext* ctx, XLA_FFI_Executio
   f.attrs.attrs = b->attr_ptrs.data();
 }
 
+thread_local std::string last_error;             // message of the last call of this thread that failed
+
 int Finish(XLA_FFI_Error* e, char* err, size_t err_len) {
   if (e == nullptr) {
     if (err && err_len) err[0] = '\0';
     return 0;
   }
-  if (err && err_len) snprintf(err, err_len, "%s", e->message.c_str());
+  last_error = e->message;
+  if (err && err_len) snprintf(err, err_len, "%s", last_error.c_str());
   const int code = static_cast<int>(e->code);
   delete e;
   return code ? code : static_cast<int>(XLA_FFI_Error_Code_UNKNOWN);
@@ -401,7 +404,8 @@ MOCK_EXPORT int mockffi_call_invoke(void* call, int stage, void* stream, int dev
     std::lock_guard<std::mutex> lock(g_mu);
     auto it = Registry().find("CUDA:" + c->target);
     if (it == Registry().end()) {
-      if (err && err_len) snprintf(err, err_len, "No FFI handler registered for %s on platform CUDA", c->target.c_str());
+      last_error = "No FFI handler registered for " + c->target + " on platform CUDA";
+      if (err && err_len) snprintf(err, err_len, "%s", last_error.c_str());
       return XLA_FFI_Error_Code_NOT_FOUND;
     }
     c->handlers = it->second;
@@ -442,6 +446,9 @@ MOCK_EXPORT int mockffi_call_run(void* call, void* stream, int device_ordinal, c
   }
   return 0;
 }
+
+// The message of the last call on this thread that failed: for callers that pass no buffer.
+MOCK_EXPORT const char* mockffi_last_error() { return last_error.c_str(); }
 
 // Execute stage only (the steady state of a compiled executable).
 MOCK_EXPORT int mockffi_call_execute(void* call, void* stream, int device_ordinal, char* err, size_t err_len) {

@@ -16,7 +16,6 @@ from __future__ import annotations
 import ctypes as C
 import dataclasses
 import enum
-import threading
 from typing import NamedTuple, Optional, Sequence
 
 from . import _native
@@ -121,16 +120,6 @@ def _err_buf():
     return C.create_string_buffer(1024)
 
 
-class _OfThread(threading.local):
-    """A thread's message buffer of `execute`, kept: a site is executed many times, and by any number of threads."""
-
-    def __init__(self):
-        self.err = _err_buf()
-
-
-_of_thread = _OfThread()
-
-
 class FfiCall:
     """One custom-call site bound to a target registered with the (mock) XLA FFI runtime."""
 
@@ -188,10 +177,10 @@ class FfiCall:
         self._check(_native.mock.mockffi_call_run(self._h, stream, device, err, len(err)), err)
 
     def execute(self, stream: int = 0, device: int = 0) -> None:
-        err = _of_thread.err
-        rc = _native.mock.mockffi_call_execute(self._h, stream, device, err, 1024)
+        # Executed many times, by any number of threads: no buffer for a message that is hardly ever needed.
+        rc = _native.mock.mockffi_call_execute(self._h, stream, device, None, 0)
         if rc != 0:
-            self._check(rc, err)
+            raise XlaFfiError(rc, _native.mock.mockffi_last_error().decode(errors="replace"))
 
     def set_operand(self, index: int, tensor) -> None:
         _native.mock.mockffi_call_set_arg_data(self._h, index, tensor.data_ptr())
