@@ -214,7 +214,7 @@ typedef struct B200SD_DotW4 {
  * least at which the largest finite new magnitude fits the type (448, 57344 or 127), at least 2^-126, and
  * at least the scale before when the page holds earlier tokens of the sequence; their codes are rounded
  * to it again where it grew.  Roundings go to the nearest, ties to even; infinities become the largest
- * value, NaN stays NaN (s8: 0).  Two sequences of one call must not append to the same page. */
+ * value, NaN stays NaN (s8: 0).  The pages that one call appends to must differ from one another. */
 typedef struct B200SD_KvCacheAppend {
   size_t struct_size;            /* sizeof(B200SD_KvCacheAppend) */
   const void* k_new;             /* [batch, new_tokens, kv_heads, head_dim] */

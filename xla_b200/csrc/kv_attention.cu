@@ -24,7 +24,7 @@
 // Token m of the 16 is row m ^ ((m & 1) << 2) of the tile in both products.
 //
 // Measured with cold caches: two sequences of 100003 to 131072 tokens, 8 key heads of 128, 86 us (5.5 TB/s of codes); 32 of 0
-// to 4096 tokens 34 us (4.0 TB/s: 9 us pass before the tiles flow and 3 to 4 in joining the pieces); 16 of 5 to 8191 with 5
+// to 4096 tokens 35 us (3.9 TB/s: 9 us pass before the tiles flow and 3 to 4 in joining the pieces); 16 of 5 to 8191 with 5
 // new tokens, 40 rows for each of 4 key heads, 59 us (bound by issue: the codes are decoded for each 16 rows); one of 37
 // tokens 7.8 us, the host's part of the call.
 //

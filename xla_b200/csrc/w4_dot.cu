@@ -23,7 +23,7 @@
 // were normal, so that 10 of the 24 bits of an f32 sum are zeros.)
 //
 // Measured with cold caches: 28672 x 8192 in groups of 128 for one row 34 us (3.6 TB/s; the bytes alone take 18.5), 8192 x
-// 28672 with zero points for 16 rows 58.6 us, 5003 x 4416 in groups of 32 for 5 rows 10.7 us, 1024 x 2048 for one row 7.6
+// 28672 with zero points for 16 rows 59.4 us, 5003 x 4416 in groups of 32 for 5 rows 10.8 us, 1024 x 2048 for one row 7.6
 // us, the host's part of a call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(Resident::kWarps * 32) w4_dot_kernel(const __g
 // CTA (per 512 of its rows).  Bound by issue and the matrix pipe: 463 instructions of a warp for a unit and 16 rows.
 // (x through each warp's ring beside the weights, once for every block of 32 rows, took 292 us instead of 149 for 33 rows
 // against 28672 x 8192, 15.0 instead of 11.7 for 5 rows against 5003 x 4416.)  16 warps leave 128 registers to a thread;
-// 20 and 24 were slower, by 3 % and 7 % at 8 rows and, short of registers, by half and more at 16.
+// 20 and 24 were slower, by 3 % and 7 % at 8 rows and, short of registers, by half and more at 16.  Four columns of products, for
+// 17 to 32 rows, spill up to 140 bytes of a thread: 28672 x 8192 takes 51 us for 16 rows, 89 for 17 and 96 for 32.
 template <typename T_, int kCols_>
 struct WideShape {
   using T = T_;
