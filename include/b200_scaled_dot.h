@@ -237,7 +237,8 @@ typedef struct B200SD_KvCacheAppend {
  *   out[b,i,h] = sum_t softmax_t( softmax_scale * q[b,i,h] . k[t, h / (heads / kv_heads)] ) * v[t, ...]
  *
  * over the positions t <= p = seq_lens[b] - new_lens[b] + i, and t > p - window when window > 0.  Rows
- * that see nothing (i >= new_lens[b] among them) get zeros, and -inf as their logarithm of the sum.
+ * that see nothing (i >= new_lens[b] among them), or nothing but scores of -inf, get zeros, and -inf as their
+ * logarithm of the sum.
  * Scores, softmax sums and products are held in f32; a row's weights are rounded for the product with the
  * values, to 11 bits where the result is BF16 and to 22 where it is F16.  new_tokens is at most 64, head_dim a multiple of 16 up to 256, page_tokens
  * 16, 32, 64 or 128, batch at most 4096.  Calls that may run at the same time need a workspace each. */

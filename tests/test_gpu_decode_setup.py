@@ -8,6 +8,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TUNING = os.path.join(ROOT, "xla_b200", "lib", "libb200_scaled_dot_tuning.so")
+with_tuning_build = pytest.mark.skipif(not os.path.exists(TUNING), reason="the tuning build is not there (make tuning)")
 
 COMMON = """
 import ctypes as C
@@ -30,6 +32,7 @@ def _run(program, **env):
     assert done.returncode == 0, done.stdout[-2000:] + done.stderr[-2000:]
 
 
+@with_tuning_build
 def test_its_failure_leaves_the_other_calls_alone():
     _run("""
 a = torch.ones((16, 64), device=dev).to(torch.float8_e4m3fn)
@@ -48,7 +51,7 @@ for _ in range(2):
 assert _native.product.b200sd_init_device(err, len(err)) == 0
 assert _native.product.b200sd_init_decode_operators(err, len(err)) == 13
 torch.cuda.synchronize()
-""", B200SD_LIBRARY=os.path.join(ROOT, "xla_b200", "lib", "libb200_scaled_dot_tuning.so"), B200SD_FAIL_DECODE_SETUP="1")
+""", B200SD_LIBRARY=TUNING, B200SD_FAIL_DECODE_SETUP="1")
 
 
 @pytest.mark.parametrize("first", ["b200sd_init_decode_operators", "b200sd_init_device"])
@@ -73,6 +76,7 @@ assert xla_b200.device_status() == 0
 """)
 
 
+@with_tuning_build
 def test_a_copy_that_does_not_come():
     """Its wait expires (20 ms in this build), the call ends and reports it, and the next one is right."""
     _run("""
@@ -105,4 +109,4 @@ for heads, kv_heads, dim, lens in ((8, 2, 128, [9000, 40]), (32, 1, 64, [100, 30
     assert xla_b200.device_status() == 0
     assert torch.equal(expires(lambda: xla_b200.paged_attention_kv8(*args)), want)
 assert xla_b200.device_status() == 0
-""", B200SD_LIBRARY=os.path.join(ROOT, "xla_b200", "lib", "libb200_scaled_dot_tuning.so"))
+""", B200SD_LIBRARY=TUNING)
